@@ -15,7 +15,7 @@ if os.environ.get("DERL_AMD_LIBRARY", "") == "diag":
   LIB_PATH = os.path.join(_PKG, "libderl_amd_diag.so")
 elif os.environ.get("DERL_AMD_LIBRARY", "").endswith(".so"):  # another build of the library (tools/: A/B on one box)
   LIB_PATH = os.path.join(_PKG, os.path.basename(os.environ["DERL_AMD_LIBRARY"]))
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 c_int, c_float, c_void_p, c_char_p = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p
 c_size_t, c_int64, c_uint64, c_double = ctypes.c_size_t, ctypes.c_int64, ctypes.c_uint64, ctypes.c_double
@@ -50,6 +50,18 @@ SIGNATURES = {
     "dx_categorical_act_f32": [P, c_int, c_int, P, c_uint64, c_uint64, P, P, P, P],
     "dx_categorical_loss_f32": [P, P, P, P, P, P, c_int, c_int, c_int, c_float, c_float,
                                 c_float, c_longlong, P, P, c_int, P, P],
+    "dx_token_log_prob": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, P, P],
+    "dx_sequence_log_prob": [P, P, c_longlong, c_int, P, P],
+    "dx_token_policy_loss": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, P, P, c_longlong, P, c_float,
+                             c_float, c_float, c_longlong, P, c_longlong, P, P, c_longlong, P, P],
+    "dx_preference_loss": [P, c_int, c_longlong, c_int, c_longlong, P, P, c_int, P, P, c_float, c_float,
+                           c_longlong, P, c_longlong, P, P, P, c_longlong, P, P],
+    "dx_scale_rows": [P, c_int, c_longlong, c_int, c_longlong, P, P],
+    "dx_orthogonalize_workspace": [c_int, c_int, c_int, c_int],
+    "dx_orthogonalize": [P, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, c_float, P, P,
+                         c_longlong, P],
+    "dx_muon_momentum_f32": [P, P, P, c_longlong, P, c_int, c_double, c_double, c_int, P, P],
+    "dx_muon_apply_f32": [P, P, c_longlong, c_double, c_double, P],
     "dx_synth_atari_step": [P, c_longlong, P, P, c_int, c_uint64, c_uint64, c_float, c_float, P],
     "dx_synth_mujoco_step": [P, P, P, c_int, c_int, c_uint64, c_uint64, c_float, P],
     "dx_mlp_init": [P],
@@ -108,7 +120,7 @@ class CnnCtx(ctypes.Structure):
                                           "ps_c2f", "ps_wc", "ps_c1d", "ps_c2d")]
       + [(n, c_void_p) for n in ("params", "grads", "packed", "y0", "y1", "y2", "hid", "head",
                                  "dy0", "dy1", "dy2", "dhid", "dhead", "slabs", "hid_slabs")])
-_RESTYPES = {"dx_last_error": c_char_p, "dx_launch_count": c_longlong, "dx_cnn_last_route": c_char_p}
+_RESTYPES = {"dx_last_error": c_char_p, "dx_orthogonalize_workspace": c_longlong, "dx_launch_count": c_longlong, "dx_cnn_last_route": c_char_p}
 
 _lib = None
 
@@ -121,6 +133,9 @@ class NativeError(RuntimeError):
 
 # return codes of include/derl_amd.h
 DX_EINVAL, DX_EHIP, DX_ENOSUP, DX_EWS, DX_ETIMEOUT = -1, -2, -3, -4, -5
+# element types and the scratch of the token losses (doubles), include/derl_amd.h
+DX_F32, DX_BF16, DX_F16 = 0, 1, 2
+DX_TOKEN_WORKSPACE = 16392
 
 
 def load():

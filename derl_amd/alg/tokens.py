@@ -1,0 +1,112 @@
+"""Losses of policies over a vocabulary: derl's clipped policy loss (derl/alg/ppo.py:24-64) for logits of any
+width, with the KL term such policies are trained with, and the loss of paired log ratios.
+
+The model is any ``torch.nn.Module`` on the GPU that maps ``data["observations"]`` to logits (..., V); the loss
+kernels produce the gradient with respect to the logits in the forward pass, autograd carries it through the model."""
+import torch
+
+from .common import Loss
+from .. import ops, summary
+
+
+class _LogitsLoss(torch.autograd.Function):
+  """A scalar computed from logits together with its gradient.  The gradient is handed on once: it is scaled in
+  place by the incoming gradient (left alone where that is 1)."""
+
+  @staticmethod
+  def forward(ctx, logits, evaluate):
+    terms, dlogits = evaluate(logits.detach())
+    ctx.dlogits = dlogits
+    return terms[0].clone()
+
+  @staticmethod
+  def backward(ctx, grad_output):
+    dlogits, ctx.dlogits = ctx.dlogits, None
+    if dlogits is None:
+      raise RuntimeError("the gradient of this loss was already handed on: evaluate the loss again to differentiate it again")
+    ops.scale_rows(dlogits, grad_output.to(torch.float32).contiguous())
+    return dlogits, None
+
+
+class TokenLoss(Loss):
+  """Shared machinery: one model forward, one fused loss on the flattened logits."""
+  tags = ()
+
+  def __init__(self, model, name=None):
+    super().__init__(model=model, name=name)
+    self.last_terms = None  # device float32[8]
+
+  def _logits(self, data):
+    logits = self.model(data["observations"])
+    if not isinstance(logits, torch.Tensor) or logits.ndim < 2:
+      raise ValueError("the model of a token loss must return logits of shape (..., vocab)")
+    return logits.reshape(-1, logits.shape[-1])
+
+  def _flat(self, data, key, dtype=None, required=True):
+    if data.get(key) is None:
+      if required:
+        raise ValueError(f"data does not contain '{key}'")
+      return None
+    return self.to_device(data[key], dtype).reshape(-1)
+
+  def _mask(self, data):
+    mask = data.get("mask")
+    return None if mask is None else self.to_device(mask, torch.bool).reshape(-1)
+
+  def _evaluate(self, logits, data):
+    raise NotImplementedError
+
+  def _summaries(self, terms):
+    for i, tag in enumerate(self.tags):
+      summary.add_scalar(f"{self.name}/{tag}", terms[i], global_step=self.call_count)
+
+  def __call__(self, data):
+    logits = self._logits(data)
+
+    def evaluate(raw):
+      terms, dlogits, _ = self._evaluate(raw, data)
+      self.last_terms = terms
+      return terms, dlogits
+
+    loss = _LogitsLoss.apply(logits, evaluate)
+    if summary.should_record():
+      self._summaries(self.last_terms)
+    self.call_count += 1
+    return loss
+
+
+class TokenPolicyLoss(TokenLoss):
+  """Clipped policy loss with a KL term and an entropy bonus (``ops.token_policy_loss``).  ``data``: observations,
+  actions, log_prob (of the policy that acted), advantages; optional ref_log_prob or ref_logits (of the reference
+  policy), mask."""
+  tags = ("loss", "policy_loss", "entropy", "kl", "clip_fraction", "ratio", "log_prob", "tokens")
+
+  def __init__(self, model, cliprange=0.2, kl_coef=0., entropy_coef=0., name=None):
+    super().__init__(model, name=name)
+    self.cliprange, self.kl_coef, self.entropy_coef = cliprange, kl_coef, entropy_coef
+
+  def _evaluate(self, logits, data):
+    f32 = torch.float32
+    ref_logits = data.get("ref_logits")
+    if ref_logits is not None:
+      ref_logits = self.to_device(ref_logits, logits.dtype).reshape(logits.shape)
+    return ops.token_policy_loss(
+        logits, self._flat(data, "actions", torch.int64), self._flat(data, "log_prob", f32),
+        self._flat(data, "advantages", f32), self.cliprange, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef,
+        ref_log_prob=self._flat(data, "ref_log_prob", f32, required=False), ref_logits=ref_logits, mask=self._mask(data))
+
+
+class PreferenceLoss(TokenLoss):
+  """Loss of paired log ratios (``ops.preference_loss``).  ``data``: observations of the packed sequences (chosen,
+  rejected, chosen, ...), actions, offsets (their borders); optional ref_log_prob (per sequence), mask."""
+  tags = ("loss", "accuracy", "margin", "chosen_reward", "rejected_reward", "chosen_log_prob", "rejected_log_prob", "pairs")
+
+  def __init__(self, model, beta=0.1, label_smoothing=0., name=None):
+    super().__init__(model, name=name)
+    self.beta, self.label_smoothing = beta, label_smoothing
+
+  def _evaluate(self, logits, data):
+    return ops.preference_loss(
+        logits, self._flat(data, "actions", torch.int64), self._flat(data, "offsets", torch.int32),
+        self._flat(data, "ref_log_prob", torch.float32, required=False), self.beta,
+        label_smoothing=self.label_smoothing, mask=self._mask(data))

@@ -5,7 +5,7 @@ from ..alg.common import Trainer
 from ..alg.ppo import PPO
 from ..anneal import LinearAnneal
 from ..models import make_model
-from ..optim import Adam
+from ..optim import Adam, Muon
 from ..policies import ActorCriticPolicy, sampling_seed
 from ..runners.onpolicy import make_ppo_runner
 from .factory import Factory
@@ -65,7 +65,11 @@ class PPOFactory(Factory):
       adam = dict(lr=schedule.get_tensor())
       if self.has_arg("optimizer_epsilon"):
         adam["eps"] = self.get_arg("optimizer_epsilon")
-      return Trainer(Adam(runner.policy.model, **adam), anneals=[schedule],
+      kinds = {"adam": Adam, "muon": Muon}
+      kind = self.get_arg_default("optimizer", "adam")
+      if kind not in kinds:
+        raise ValueError(f"optimizer must be one of {sorted(kinds)}, got {kind!r}")
+      return Trainer(kinds[kind](runner.policy.model, **adam), anneals=[schedule],
                      max_grad_norm=self.get_arg("max_grad_norm"))
 
   def make_alg(self, runner, trainer, **kwargs):

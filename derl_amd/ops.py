@@ -239,3 +239,266 @@ def normal_loss(head_out, logstd, actions, old_log_prob, advantages, old_values,
             float(entropy_coef), int(global_batch), _lib.ptr(dhead_out), _lib.ptr(dlogstd_out),
             _lib.ptr(partials), partials.numel(), _lib.ptr(loss_out), _lib.stream_ptr(dev))
   return loss_out
+
+
+# ---- policies over a vocabulary -----------------------------------------------------------------
+
+_ELEMENT_TYPES = {torch.float32: _lib.DX_F32, torch.bfloat16: _lib.DX_BF16, torch.float16: _lib.DX_F16}
+
+
+def _call_on(device, name, *args):
+  """One native call with ``device`` current (kernels launch on the current device)."""
+  if device.index == torch.cuda.current_device():
+    _lib.call(name, *args)
+  else:
+    with torch.cuda.device(device):
+      _lib.call(name, *args)
+
+
+def _rows_of(t, name, like=None):
+  """(rows, columns, pitch) of a 2-D tensor whose rows are contiguous; any distance between rows."""
+  if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    raise ValueError(f"{name} must be a tensor on the GPU (derl_amd has no CPU path)")
+  if t.dtype not in _ELEMENT_TYPES:
+    raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+  if t.ndim != 2 or t.shape[1] < 1:
+    raise ValueError(f"{name} must be (rows, vocab) with vocab >= 1, got {tuple(t.shape)}")
+  rows, columns = t.shape
+  pitch = t.stride(0) if rows > 1 else columns
+  if (columns > 1 and t.stride(1) != 1) or pitch < columns:
+    raise ValueError(f"the rows of {name} must be contiguous and must not overlap: strides {t.stride()}")
+  if like is not None and (t.dtype != like.dtype or t.shape != like.shape or t.device != like.device):
+    raise ValueError(f"{name} must match logits ({like.dtype}, {tuple(like.shape)}, {like.device}): "
+                     f"{t.dtype}, {tuple(t.shape)}, {t.device}")
+  return rows, columns, pitch
+
+
+def _vector(t, name, n, device, dtype):
+  """A contiguous vector of ``n`` on the logits' device; its pointer (None stays None)."""
+  if t is None:
+    return None
+  _dev(t, name)
+  if t.dtype not in dtype:
+    raise ValueError(f"{name} must have dtype {' or '.join(map(str, dtype))}, got {t.dtype}")
+  if tuple(t.shape) != (n,) or t.device != device:
+    raise ValueError(f"{name} must be ({n},) on {device}, got {tuple(t.shape)} on {t.device}")
+  return _lib.ptr(t)
+
+
+_INDEX, _FLAG, _FLOAT, _OFFSET = (torch.int64,), (torch.bool, torch.uint8), (torch.float32,), (torch.int32,)
+
+
+def _span(t):
+  """First and last byte address of a tensor with non-negative strides."""
+  if t.numel() == 0:
+    return 0, 0
+  last = sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+  return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _gradient_buffer(dlogits_out, logits, *others):
+  """The tensor the gradient goes to: new, the caller's, or ``logits`` itself (in place)."""
+  if dlogits_out is None:
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+  _rows_of(dlogits_out, "dlogits_out", like=logits)
+  same = dlogits_out.data_ptr() == logits.data_ptr() and (logits.shape[0] <= 1 or dlogits_out.stride(0) == logits.stride(0))
+  begin, end = _span(dlogits_out)
+  for other in others + (() if same else (logits,)):
+    if other is not None:
+      b, e = _span(other)
+      if b < end and begin < e:
+        raise ValueError("dlogits_out overlaps an input (it may only be logits itself)")
+  return dlogits_out
+
+
+def token_log_prob(logits, actions, mask=None):
+  """Log-probability of each row's action and the entropy of its distribution.
+
+  logits (N, V) float32 / bfloat16 / float16 with contiguous rows (any row stride >= V), actions (N,)
+  int64, mask (N,) bool or uint8: rows that are False are not read and give 0.  Returns (log_prob,
+  entropy), float32 (N,).  A logit of -inf is an action that cannot be chosen; a row without any
+  distribution (all -inf, NaN, +inf) or an action outside [0, V) gives NaN.  N = 1 .. is the form for
+  single tokens of sequences being generated."""
+  rows, vocab, pitch = _rows_of(logits, "logits")
+  dev = logits.device
+  out = torch.empty((2, rows), dtype=torch.float32, device=dev)
+  log_prob, entropy = out[0], out[1]
+  act = _vector(actions, "actions", rows, dev, _INDEX)
+  keep = _vector(mask, "mask", rows, dev, _FLAG)
+  _call_on(dev, "dx_token_log_prob", _lib.ptr(logits), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, keep,
+           _lib.ptr(log_prob), _lib.ptr(entropy), _lib.stream_ptr(dev))
+  return log_prob, entropy
+
+
+def _check_offsets(offsets, device):
+  _dev(offsets, "offsets", torch.int32)
+  if offsets.ndim != 1 or offsets.numel() < 1 or offsets.device != device:
+    raise ValueError(f"offsets must be a vector of sequence borders on {device}, got {tuple(offsets.shape)} on {offsets.device}")
+  return offsets.numel() - 1
+
+
+def sequence_log_prob(logits, actions, offsets, mask=None):
+  """Summed log-probabilities of packed sequences: sequence s holds the rows offsets[s] .. offsets[s + 1]
+  of ``logits`` (offsets int32 (S + 1,), non-decreasing; empty sequences give 0).  float32 (S,): what
+  ``preference_loss`` takes as ``ref_log_prob`` when the logits are the reference's."""
+  rows, _, _ = _rows_of(logits, "logits")
+  dev = logits.device
+  sequences = _check_offsets(offsets, dev)
+  log_prob, _ = token_log_prob(logits, actions, mask)
+  out = torch.empty(sequences, dtype=torch.float32, device=dev)
+  _call_on(dev, "dx_sequence_log_prob", _lib.ptr(log_prob), _lib.ptr(offsets), rows, sequences, _lib.ptr(out),
+           _lib.stream_ptr(dev))
+  return out
+
+
+def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_coef=0., entropy_coef=0.,
+                      ref_log_prob=None, ref_logits=None, mask=None, global_batch=0, dlogits_out=None):
+  """Clipped policy loss with a KL term and an entropy bonus over wide logits, and its gradient.
+
+  Per unmasked row: ratio = exp(log p(action) - old_log_prob); ``-min(ratio A, clip(ratio, 1 - cliprange,
+  1 + cliprange) A) - entropy_coef H + kl_coef KL`` (cliprange None: not clipped).  The divergence from
+  the reference policy is estimated from the action alone, ``e^d - 1 - d`` with ``d = ref_log_prob - log p``,
+  or summed over the vocabulary where ``ref_logits`` are given (at most one of the two).  The loss is the
+  mean over the unmasked rows; ``global_batch`` > 0 divides the gradient by that instead (shards add up).
+
+  logits (N, V) float32 / bfloat16 / float16 (rows contiguous, any row stride), actions (N,) int64,
+  old_log_prob / advantages / ref_log_prob (N,) float32, ref_logits like logits, mask (N,) bool / uint8.
+  Returns (loss float32 (8,), dlogits (N, V), log_prob float32 (N,)); loss = {loss, policy loss, entropy, KL,
+  share of ratios outside the range, mean ratio, mean log-probability, unmasked rows}.  ``dlogits_out`` may
+  be ``logits``.  Masked rows have gradient and log_prob 0; without an unmasked row the loss is 0."""
+  rows, vocab, pitch = _rows_of(logits, "logits")
+  dev = logits.device
+  if ref_log_prob is not None and ref_logits is not None:
+    raise ValueError("give ref_log_prob or ref_logits, not both")
+  if cliprange is not None and not cliprange >= 0:
+    raise ValueError(f"cliprange must be None or >= 0, got {cliprange}")
+  ref_pitch = vocab
+  if ref_logits is not None:
+    _, _, ref_pitch = _rows_of(ref_logits, "ref_logits", like=logits)
+  act = _vector(actions, "actions", rows, dev, _INDEX)
+  old = _vector(old_log_prob, "old_log_prob", rows, dev, _FLOAT)
+  adv = _vector(advantages, "advantages", rows, dev, _FLOAT)
+  ref = _vector(ref_log_prob, "ref_log_prob", rows, dev, _FLOAT)
+  keep = _vector(mask, "mask", rows, dev, _FLAG)
+  dlogits = _gradient_buffer(dlogits_out, logits, ref_logits)
+  log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
+  loss_out = torch.empty(8, dtype=torch.float32, device=dev)
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
+  _call_on(dev, "dx_token_policy_loss", _lib.ptr(logits), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, old, adv, ref,
+           _lib.ptr(ref_logits), ref_pitch, keep, -1.0 if cliprange is None else float(cliprange), float(kl_coef),
+           float(entropy_coef), int(global_batch), _lib.ptr(dlogits), dlogits.stride(0) if rows > 1 else vocab,
+           _lib.ptr(log_prob), _lib.ptr(workspace), workspace.numel(), _lib.ptr(loss_out), _lib.stream_ptr(dev))
+  return loss_out, dlogits, log_prob
+
+
+def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothing=0., mask=None, global_pairs=0,
+                    dlogits_out=None):
+  """Loss of paired log ratios over packed sequences, and its gradient.
+
+  Sequences 2 p (chosen) and 2 p + 1 (rejected) are the rows offsets[s] .. offsets[s + 1] of logits (N, V);
+  offsets int32 (2 P + 1,), non-decreasing.  With a sequence's log-probability summed over its unmasked
+  rows, ``h = beta ((chosen - ref_chosen) - (rejected - ref_rejected))`` and the loss is the mean over the
+  pairs of ``-(1 - s) log sigmoid(h) - s log sigmoid(-h)``, s = label_smoothing.  ref_log_prob float32 (2 P,)
+  (``sequence_log_prob`` of the reference policy) or None for 0.  ``global_pairs`` > 0 divides the gradient
+  by that instead of P.
+
+  Returns (loss float32 (8,), dlogits (N, V), sequence log-probabilities float32 (2 P,)); loss = {loss, share of
+  pairs with h > 0, h, beta (chosen - ref), beta (rejected - ref), chosen, rejected, P}.  Rows that are masked
+  or belong to no sequence have gradient 0.  ``dlogits_out`` may be ``logits``."""
+  rows, vocab, pitch = _rows_of(logits, "logits")
+  dev = logits.device
+  sequences = _check_offsets(offsets, dev)
+  if sequences < 2 or sequences % 2:
+    raise ValueError(f"offsets must have 2 pairs + 1 entries, got {offsets.numel()}")
+  if not 0 <= label_smoothing <= 1:
+    raise ValueError(f"label_smoothing must lie in [0, 1], got {label_smoothing}")
+  act = _vector(actions, "actions", rows, dev, _INDEX)
+  ref = _vector(ref_log_prob, "ref_log_prob", sequences, dev, _FLOAT)
+  keep = _vector(mask, "mask", rows, dev, _FLAG)
+  dlogits = _gradient_buffer(dlogits_out, logits)
+  sequence = torch.empty(sequences, dtype=torch.float32, device=dev)
+  loss_out = torch.empty(8, dtype=torch.float32, device=dev)
+  row_stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
+  _call_on(dev, "dx_preference_loss", _lib.ptr(logits), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act,
+           _lib.ptr(offsets), sequences // 2, ref, keep, float(beta), float(label_smoothing), int(global_pairs),
+           _lib.ptr(dlogits), dlogits.stride(0) if rows > 1 else vocab, _lib.ptr(sequence), _lib.ptr(row_stats),
+           _lib.ptr(workspace), workspace.numel(), _lib.ptr(loss_out), _lib.stream_ptr(dev))
+  return loss_out, dlogits, sequence
+
+
+def scale_rows(x, factor):
+  """x *= factor in place, ``factor`` a float32 device scalar; nothing but the factor is read when it is 1."""
+  rows, columns, pitch = _rows_of(x, "x")
+  _dev(factor, "factor", torch.float32)
+  if factor.numel() != 1 or factor.device != x.device:
+    raise ValueError(f"factor must be one float32 on {x.device}, got {tuple(factor.shape)} on {factor.device}")
+  _call_on(x.device, "dx_scale_rows", _lib.ptr(x), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, _lib.ptr(factor),
+           _lib.stream_ptr(x.device))
+  return x
+
+
+# ---- matrix optimizer ---------------------------------------------------------------------------
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
+  """Newton-Schulz orthogonalisation of (..., m, n) matrices: X = G / (|G|_F + eps), then ``steps`` times
+  X <- a X + (b A + c A A) X with A = X X^T (of the shorter side).  The singular vectors stay, the singular
+  values approach 1.  float32 (fp32 accuracy throughout), bfloat16 or float16 (11-bit intermediates);
+  contiguous; the result has update's type and shape.  ``out`` may be ``update``.  A zero matrix gives zeros."""
+  if not isinstance(update, torch.Tensor) or not update.is_cuda:
+    raise ValueError("update must be a tensor on the GPU (derl_amd has no CPU path)")
+  if update.dtype not in _ELEMENT_TYPES:
+    raise ValueError(f"update must be float32, bfloat16 or float16, got {update.dtype}")
+  if update.ndim < 2 or not update.is_contiguous():
+    raise ValueError(f"update must be contiguous (..., m, n), got {tuple(update.shape)}, strides {update.stride()}")
+  if int(steps) < 1:
+    raise ValueError(f"steps must be >= 1, got {steps}")
+  a, b, c = (float(v) for v in coefficients)
+  if not all(math.isfinite(v) for v in (a, b, c, eps)) or eps < 0:
+    raise ValueError(f"coefficients and eps must be finite, eps >= 0: {coefficients}, {eps}")
+  if out is None:
+    out = torch.empty_like(update)
+  else:
+    _dev(out, "out", update.dtype)
+    if out.shape != update.shape or out.device != update.device:
+      raise ValueError(f"out must match update: {tuple(out.shape)} on {out.device}")
+    (b0, e0), (b1, e1) = _span(update), _span(out)
+    if b0 != b1 and b0 < e1 and b1 < e0:
+      raise ValueError("out overlaps update (it may only be update itself)")
+  m, n = update.shape[-2:]
+  if update.numel() == 0:
+    return out
+  batch = update.numel() // (m * n)
+  kind = _ELEMENT_TYPES[update.dtype]
+  need = _lib.load().dx_orthogonalize_workspace(kind, batch, m, n)
+  _lib.check(min(need, 0), "dx_orthogonalize_workspace")
+  workspace = torch.empty(need, dtype=torch.uint8, device=update.device)
+  _call_on(update.device, "dx_orthogonalize", _lib.ptr(update), kind, batch, m, n, int(steps), a, b, c, float(eps),
+           _lib.ptr(out), _lib.ptr(workspace), need, _lib.stream_ptr(update.device))
+  return out
+
+
+def muon_momentum(grads, momentum, update, partials, max_norm, mu, nesterov=True, norm_out=None):
+  """First half of a Muon step on flat float32 buffers: clips ``grads`` in place, advances ``momentum`` and
+  writes the direction to orthogonalise to ``update``."""
+  for name, t in (("grads", grads), ("momentum", momentum), ("update", update)):
+    _dev(t, name, torch.float32)
+    if t.numel() != grads.numel():
+      raise ValueError(f"{name} must have {grads.numel()} elements, got {t.numel()}")
+  _lib.call("dx_muon_momentum_f32", _lib.ptr(grads), _lib.ptr(momentum), _lib.ptr(update), grads.numel(),
+            _lib.ptr(partials), 0 if partials is None else partials.numel(),
+            float(max_norm) if max_norm is not None else 0.0, float(mu), int(bool(nesterov)), _lib.ptr(norm_out),
+            _lib.stream_ptr(grads.device))
+
+
+def muon_apply(params, update, decay, step):
+  """params <- params * decay - step * update (flat float32 buffers)."""
+  for name, t in (("params", params), ("update", update)):
+    _dev(t, name, torch.float32)
+  if params.numel() != update.numel():
+    raise ValueError(f"update must have {params.numel()} elements, got {update.numel()}")
+  _lib.call("dx_muon_apply_f32", _lib.ptr(params), _lib.ptr(update), params.numel(), float(decay), float(step),
+            _lib.stream_ptr(params.device))

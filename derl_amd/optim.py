@@ -124,3 +124,66 @@ class RMSprop(_FlatOptimizer):
 
   def state_dict(self):
     return dict(step=self.step_count, square_avg=self.square_avg)
+
+
+def _is_output_layer(name):
+  """Weights of the layer a model's outputs come from (``output_layers.*`` of the CNN, the last layer of each MLP)."""
+  return name.startswith("output_layers.") or name.endswith(".4.weight")
+
+
+class Muon(_FlatOptimizer):
+  """torch.optim.Muon semantics for the weight matrices: momentum, Newton-Schulz orthogonalisation of the update
+  (``ops.orthogonalize``, in float32), step of lr * sqrt(max(1, rows / columns)), decoupled weight decay.  Convolution
+  weights count as (out, in * h * w).  Everything else -- biases, ``logstd``, and the output layers, whose rows are
+  separate functions rather than a mixing matrix -- takes the Adam step at ``adam_lr`` (default: ``lr``, annealed
+  with it).  ``matrices``: names of the parameters to orthogonalise instead of the default choice."""
+
+  def __init__(self, model, lr=1e-3, momentum=0.95, nesterov=True, ns_steps=5, weight_decay=0., adam_lr=None,
+               betas=(0.9, 0.999), eps=1e-8, matrices=None):
+    super().__init__(model, lr)
+    self.momentum, self.nesterov, self.ns_steps, self.weight_decay = momentum, nesterov, int(ns_steps), weight_decay
+    self.adam_lr, self.betas, self.eps = adam_lr, betas, eps
+    views = self.engine.named_views(self.engine.params)
+    if matrices is None:
+      matrices = [name for name, view in views.items() if view.ndim >= 2 and not _is_output_layer(name)]
+    wrong = [name for name in matrices if name not in views or views[name].ndim < 2]
+    if wrong:
+      raise ValueError(f"matrices must name weights of two or more dimensions, got {wrong}")
+    base, size = self.engine.params.data_ptr(), self.engine.params.element_size()
+    self._matrices, taken = [], []
+    for name in matrices:
+      view = views[name]
+      begin = (view.data_ptr() - base) // size
+      self._matrices.append((begin, begin + view.numel(), view.shape[0], view.numel() // view.shape[0]))
+      taken.append((begin, begin + view.numel()))
+    self._spans, at = [], 0  # what lies between the matrices
+    for begin, end in sorted(taken) + [(self.engine.params.numel(),) * 2]:
+      if begin < at:
+        raise ValueError(f"matrices names a weight twice: {matrices}")
+      if begin > at:
+        self._spans.append((at, begin))
+      at = end
+    self.exp_avg = torch.zeros_like(self.engine.params)     # momentum of the matrices, first moment of the rest
+    self.exp_avg_sq = torch.zeros_like(self.engine.params)  # second moment of the rest
+    self._update = torch.zeros_like(self.engine.params)
+
+  def step(self):
+    self.step_count += 1
+    lr = self.current_lr()
+    adam_lr = lr if self.adam_lr is None else float(self.adam_lr)
+    params, grads = self.engine.params, self.engine.grads
+    for begin, end, rows, columns in self._matrices:
+      update = self._update[begin:end]
+      ops.muon_momentum(grads[begin:end], self.exp_avg[begin:end], update, self.partials, self.max_grad_norm, self.momentum,
+                        self.nesterov, self.grad_norm)
+      update = update.view(rows, columns)
+      ops.orthogonalize(update, self.ns_steps, out=update)
+      ops.muon_apply(params[begin:end], update.view(-1), 1 - lr * self.weight_decay, lr * max(1, rows / columns) ** 0.5)
+    for begin, end in self._spans:
+      ops.clip_adam_step(params[begin:end], grads[begin:end], self.exp_avg[begin:end], self.exp_avg_sq[begin:end],
+                         self.partials, self.max_grad_norm, adam_lr, self.step_count, self.betas[0], self.betas[1],
+                         self.eps, self.grad_norm)
+    self.engine.mark_dirty()
+
+  def state_dict(self):
+    return dict(step=self.step_count, exp_avg=self.exp_avg, exp_avg_sq=self.exp_avg_sq)

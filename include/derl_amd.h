@@ -40,7 +40,7 @@ extern "C" {
 #define DX_EWS (-4)      /* workspace too small                                     */
 #define DX_ETIMEOUT (-5) /* a persistent kernel's grid barrier gave up (dx_mlp_ppo_epoch) */
 
-#define DX_ABI_VERSION 6
+#define DX_ABI_VERSION 7
 
 int dx_abi_version(void);
 /* The DX_* environment switches ("Diagnostic switches") are parsed when a call first needs them and cached.
@@ -186,6 +186,83 @@ int dx_reward_summary_f32(const float *rewards, const uint8_t *resets, int T, in
                           double *acc, double *ep_len, uint8_t *ended, double *queue, int *qlen,
                           int *qpos, long long *step_count, double *rows, int max_rows, int *nrows,
                           void *stream);
+
+/* ---------------------------------------------------------------------------------
+ * Policies over a vocabulary.  derl's losses (derl/alg/ppo.py:24-64: clipped ratio, entropy bonus)
+ * for logits too wide for the padded head below, with the KL term such policies are trained with,
+ * and the loss of paired log ratios.  `logits` is (rows, vocab) of `dtype`, one row per token, rows
+ * `pitch` elements apart (pitch >= vocab; a row may start at any element); vocab 1 .. 2^30.
+ * A row whose `mask` byte is 0 is not read and not counted: log-probability, entropy and gradient 0,
+ * its action may be anything.  -inf logits are columns that cannot be chosen (probability and
+ * gradient 0); a row with nothing but -inf, a NaN, +inf or an action outside [0, vocab) gives NaN.
+ *   token_log_prob : log p(action) and (optional) entropy of every row.
+ *   sequence_log_prob : sums of token log-probabilities over rows [offsets[s], offsets[s + 1]).
+ *   token_policy_loss : per unmasked row, lp = log p(action), ratio = exp(lp - old_log_prob),
+ *        -min(ratio A, clip(ratio, 1 - cliprange, 1 + cliprange) A) (cliprange < 0: no clipping)
+ *        - entropy_coef H + kl_coef KL, with KL = e^d - 1 - d, d = ref_log_prob - lp, or with
+ *        ref_logits (same dtype, rows ref_pitch apart) the divergence sum_j p_j (log p_j - log q_j).
+ *        dlogits = gradient of the mean over the unmasked rows (global_batch > 0: of the sum divided
+ *        by global_batch, so that shards add up); dlogits may be logits (in place).
+ *        loss_out[8] = {loss, policy loss, entropy, KL, share of clipped ratios, mean ratio, mean lp,
+ *        unmasked rows}, means over the unmasked rows, all 0 if there is none.
+ *   preference_loss : sequences 2 p (chosen) and 2 p + 1 (rejected), rows [offsets[s], offsets[s + 1]) of
+ *        the logits, offsets int32 (2 pairs + 1) non-decreasing.  h = beta ((chosen - ref) - (rejected -
+ *        ref)) with the sequences' summed log-probabilities (ref_log_prob (2 pairs) or NULL = 0);
+ *        loss = mean[-(1 - s) log sigmoid(h) - s log sigmoid(-h)], s = label_smoothing.  Rows of no
+ *        sequence have gradient 0.  row_stats: scratch of 4 floats per row, 16-byte aligned.
+ *        loss_out[8] = {loss, share with h > 0, h, beta (chosen - ref), beta (rejected - ref), chosen,
+ *        rejected, pairs}.  global_pairs > 0 divides the gradient instead of pairs.
+ *   scale_rows : x *= *factor (device scalar) in place; reads nothing but the factor when it is 1.
+ * `workspace`: scratch of DX_TOKEN_WORKSPACE doubles.  Sums of a row in fp32, over rows in fp64, every
+ * result independent of timing (no atomics).
+ * --------------------------------------------------------------------------------- */
+#define DX_F32 0
+#define DX_BF16 1
+#define DX_F16 2
+#define DX_TOKEN_WORKSPACE 16392
+int dx_token_log_prob(const void *logits, int dtype, long long rows, int vocab, long long pitch,
+                      const int64_t *actions, const uint8_t *mask, float *log_prob, float *entropy,
+                      void *stream);
+int dx_sequence_log_prob(const float *token_log_prob, const int32_t *offsets, long long rows,
+                         int sequences, float *out, void *stream);
+int dx_token_policy_loss(const void *logits, int dtype, long long rows, int vocab, long long pitch,
+                         const int64_t *actions, const float *old_log_prob, const float *advantages,
+                         const float *ref_log_prob, const void *ref_logits, long long ref_pitch,
+                         const uint8_t *mask, float cliprange, float kl_coef, float entropy_coef,
+                         long long global_batch, void *dlogits, long long dlogits_pitch,
+                         float *log_prob, double *workspace, long long workspace_count,
+                         float *loss_out, void *stream);
+int dx_preference_loss(const void *logits, int dtype, long long rows, int vocab, long long pitch,
+                       const int64_t *actions, const int32_t *offsets, int pairs,
+                       const float *ref_log_prob, const uint8_t *mask, float beta,
+                       float label_smoothing, long long global_pairs, void *dlogits,
+                       long long dlogits_pitch, float *sequence_log_prob, float *row_stats,
+                       double *workspace, long long workspace_count, float *loss_out, void *stream);
+int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pitch,
+                  const float *factor, void *stream);
+
+/* ---------------------------------------------------------------------------------
+ * Orthogonalised update of a matrix optimizer: `batch` contiguous (m, n) matrices of `dtype`, each
+ *   X = G / (|G|_F + eps);  `steps` times: A = X X^T (of the shorter side), X <- a X + (b A + c A^2) X
+ * and `out` = X in the same type (out may be update).  Products on the fp16 matrix cores: fp32 input as
+ * two fp16 terms per operand and three products (22 bits, fp32 accuracy), bf16 / fp16 input as one.
+ * Intermediate entries are held scaled: |X| < 16 and |b A + c A^2 + a| < 256 must hold, which any
+ * coefficients whose iteration keeps singular values near 1 do.
+ * dx_orthogonalize_workspace: bytes of `workspace` (256-byte aligned), negative DX_E* on bad shapes.
+ * --------------------------------------------------------------------------------- */
+long long dx_orthogonalize_workspace(int dtype, int batch, int m, int n);
+int dx_orthogonalize(const void *update, int dtype, int batch, int m, int n, int steps, float a,
+                     float b, float c, float eps, void *out, void *workspace,
+                     long long workspace_bytes, void *stream);
+/* The two elementwise halves of a Muon step around it (torch.optim.Muon's order of operations), fp32, `n` elements:
+ *   momentum : g <- g * coef (clip as in dx_clip_adam_step_f32, written back); m <- m + (1 - mu)(g - m);
+ *              update = nesterov ? g + mu (m - g) : m;   norm_out (optional) = the pre-clip norm
+ *   apply    : p <- p * decay - step * update */
+int dx_muon_momentum_f32(float *grads, float *momentum, float *update, long long n, const double *partials,
+                         int npartials, double max_norm, double mu, int nesterov, float *norm_out,
+                         void *stream);
+int dx_muon_apply_f32(float *params, const float *update, long long n, double decay, double step,
+                      void *stream);
 
 /* ---------------------------------------------------------------------------------
  * Categorical head -- replaces the distribution part of derl/policies.py:61-80
