@@ -12,17 +12,25 @@
 //
 // Every matrix product is C = P Q^T with both operands' k contiguous: X for A = X X^T, A = A^T for A^2 = A A^T, and for
 // B X the transposed copy X^T, which the epilogue of each update writes beside X.  A and B are symmetric: only tiles on
-// and above the diagonal are formed and stored twice.  All sizes are padded to the tile with zeros in the workspace.
+// and above the diagonal are formed and stored twice.  Both sides are padded
+// to a multiple of 64 with zeros in the workspace.
+#include <cmath>
+#include <type_traits>
+
 #include "igemm_dev.hpp"
 
 namespace dx {
 namespace {
 
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 constexpr float kScaleX = 4096.f, kScaleA = 256.f;
-constexpr int kPad = 128, kBK = 64, kNormParts = 64;
+constexpr int kPad = 64, kBK = 64, kNormParts = 512;
+constexpr int kSplitGroups = 256;  // workgroups of a product that is split over K, at most; its tiles are half as many
 
 enum Epilogue { GRAM, POLY, UPDATE, FINAL };
 
@@ -32,11 +40,16 @@ struct NsArgs {
   Terms P, Q;             // operands: rows of K contiguous values
   long long p_stride, q_stride;  // values from one matrix of the batch to the next
   int ldp, ldq, K;
-  int tiles_m, tiles_n;   // tiles of TM rows of P / Q
+  int rows_p, rows_q;     // rows of P / Q, multiples of kPad
+  int tiles_m, tiles_n;   // tiles of TM rows of them
   Terms D, DT;            // [m][n] and its transpose [n][m]
   long long d_stride, dt_stride;
   int ldd, lddt;
   float a, b, c;
+  // split K: `splits` workgroups a tile, each over `split_stages` stages; their sums, and a count of arrivals per tile
+  int splits, split_stages;
+  float *partials;
+  unsigned *arrivals;
   // FINAL
   void *out;
   int dtype, r, cols, tall;
@@ -58,6 +71,26 @@ __device__ __forceinline__ void put_terms4(const Terms &t, long long at, const f
   if (two) *reinterpret_cast<f16x4 *>(t.lo + at) = l;
 }
 
+// two fp16 values of consecutive rows and their successors: d0 = (row 0, row 1), d1 = (row 2, row 3) of this lane's column.
+// Transposed over the four lanes of a quad: lane j ends with row j of the quad's four columns.
+struct Pair2 { uint32_t x, y; };
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad_move(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ Pair2 quad_transpose(uint32_t d0, uint32_t d1, int lane) {
+  const uint32_t pick = lane & 1 ? 0x03020706u : 0x05040100u;  // the pair's rows 0 / 2 in the even lane, 1 / 3 in the odd one
+  const uint32_t a0 = __builtin_amdgcn_perm(quad_move<0xB1>(d0), d0, pick), a1 = __builtin_amdgcn_perm(quad_move<0xB1>(d1), d1, pick);
+  const bool high = lane & 2;
+  const uint32_t other = quad_move<0x4E>(high ? a0 : a1);
+  return high ? Pair2{other, a1} : Pair2{a0, other};
+}
+// (x, y) of a lane and of lane ^ 32 -> both halves' x in the lower lane, both halves' y in the upper one (inline asm: hipcc
+// folds the builtin's results where an operand is uniform)
+__device__ __forceinline__ void swap_halves(uint32_t &x, uint32_t &y) {
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+}
+
 __device__ __forceinline__ void put_out(void *out, int dtype, long long at, float v) {
   if (dtype == DX_F32) static_cast<float *>(out)[at] = v;
   else if (dtype == DX_BF16) static_cast<__bf16 *>(out)[at] = static_cast<__bf16>(v);
@@ -69,28 +102,86 @@ __device__ __forceinline__ float get_in(const void *in, int dtype, long long at)
   return static_cast<float>(static_cast<const _Float16 *>(in)[at]);
 }
 
-// 256 threads: 2 x 2 waves of TM/2 x TM/2 (32 x 32 x 16 instructions).  Operands arrive by LDS-DMA, two K stages of 64;
-// a row of a stage is 128 bytes = 8 chunks of 16, slot s holds chunk s ^ ((row >> 1) & 7) (conflict-free ds_read_b128:
-// the 16 lanes of a group meet every bank once).
-template <int TM, int TERMS, Epilogue EPI>
-__global__ __launch_bounds__(256) void ns_gemm_kernel(const NsArgs a) {
+// four results of the last step, rows m .. m + 3 of column n, to the caller's matrix (which may start at any element);
+// quad: the first column of this lane's quad
+__device__ __forceinline__ void put_final(const NsArgs &a, int z, int m, int n, int quad, int lane, const float (&v)[4]) {
+  typedef f32x4 Loose4 __attribute__((aligned(4)));
+  typedef u32x2 Loose2 __attribute__((aligned(2)));
+  const long long base = static_cast<long long>(z) * a.r * a.cols;
+  if (a.dtype == DX_F32) {
+    float *out = static_cast<float *>(a.out) + base;
+    if (a.tall && m + 3 < a.r && n < a.cols) {
+      *reinterpret_cast<Loose4 *>(out + static_cast<long long>(n) * a.r + m) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (m + k < a.r && n < a.cols) out[a.tall ? static_cast<long long>(n) * a.r + m + k : static_cast<long long>(m + k) * a.cols + n] = v[k];
+    }
+    return;
+  }
+  uint16_t *out = static_cast<uint16_t *>(a.out) + base, bits[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    bits[k] = a.dtype == DX_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(v[k])) : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v[k]));
+  const uint32_t d0 = bits[0] | static_cast<uint32_t>(bits[1]) << 16, d1 = bits[2] | static_cast<uint32_t>(bits[3]) << 16;
+  if (a.tall) {
+    if (n >= a.cols) return;
+    if (m + 3 < a.r) *reinterpret_cast<Loose2 *>(out + static_cast<long long>(n) * a.r + m) = u32x2{d0, d1};
+    else
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (m + k < a.r) out[static_cast<long long>(n) * a.r + m + k] = bits[k];
+    return;
+  }
+  const Pair2 t = quad_transpose(d0, d1, lane);  // row m + lane % 4, columns quad .. quad + 3
+  const int row = m + (lane & 3);
+  if (row >= a.r) return;
+  uint16_t *to = out + static_cast<long long>(row) * a.cols + quad;
+  if (quad + 3 < a.cols) *reinterpret_cast<Loose2 *>(to) = u32x2{t.x, t.y};
+  else
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (quad + k < a.cols) to[k] = static_cast<uint16_t>((k < 2 ? t.x : t.y) >> (k & 1) * 16);
+}
+
+// WR x WC waves, each FM x FN tiles of 32 x 32 x 16 instructions; K stages of 64, a ring of RING in LDS filled by LDS-DMA.
+// A row of a stage is 128 bytes -- one cache line: a CU has about 64 requests to the L2 in flight, and with rows of 64 bytes
+// (stages of 32) half of what they can carry bounded the copies (4096^3, one term: 143 us, 120 with whole lines).  Slot s of row R
+// holds the row's 16-byte chunk s ^ ((R >> 1) & 7), so that the 16 lanes of a ds_read_b128 group meet every bank once; the
+// swizzle is applied to the source address, the DMA writes LDS linearly.
+// One barrier per stage, in front of its last 16 k, whose fragments are in registers by then: behind it the stage's slot is
+// free and is filled again, and the next stage has landed everywhere, so that its first fragments are read in the shadow of
+// the last products: the matrix pipe does not wait at the barrier.  Rows past the matrix repeat its last row and are not stored.
+template <int TM, int WR, int WC, int TERMS, int RING, Epilogue EPI>
+__global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
-  constexpr int F = TM / 64;                 // 32 x 32 tiles per wave and side
-  constexpr int kArray = TM * kBK * 2;       // bytes of one operand term of a stage
+  constexpr int kWaves = WR * WC, FM = TM / WR / 32, FN = TM / WC / 32;
+  constexpr int kArray = TM * kBK * 2;           // bytes of one operand term of a stage
   constexpr int kStage = 2 * TERMS * kArray;
-  constexpr int kPieces = TM / 8;            // 1 KiB pieces of an array
+  constexpr int NP = TM / 8 / kWaves;            // 1 KiB pieces (8 rows) of an array that a wave copies
+  constexpr int kPieces = 2 * TERMS * NP;
+  static_assert(NP * 8 * kWaves == TM && FM * 32 * WR == TM && FN * 32 * WC == TM, "tile");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int z = blockIdx.y;
-  int bm, bn;
-  if (EPI == GRAM || EPI == POLY) {  // the upper triangle, row by row
-    int left = blockIdx.x, row = 0;
-    while (left >= a.tiles_m - row) left -= a.tiles_m - row++;
-    bm = row;
-    bn = row + left;
-  } else {
-    bm = blockIdx.x % a.tiles_m;
-    bn = blockIdx.x / a.tiles_m;
+  int bm, bn, split;
+  {
+    // consecutive workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles
+    const int splits = EPI == GRAM && TM == 64 ? a.splits : 1, total = gridDim.x / splits, per = (total + 7) / 8, full = total - 8 * (per - 1);  // XCDs 0 .. full - 1 hold `per` tiles
+    const int id = blockIdx.x / splits, xcd = id & 7, k = id >> 3;
+    split = blockIdx.x - id * splits;
+    int left = xcd * per - (xcd > full ? xcd - full : 0) + k;
+    if (EPI == GRAM || EPI == POLY) {  // the upper triangle, row by row
+      int row = 0;
+      while (left >= a.tiles_m - row) left -= a.tiles_m - row++;
+      bm = row;
+      bn = row + left;
+    } else {  // bands of four tile rows, column by column
+      const int band = left / (4 * a.tiles_n), rows = min(4, a.tiles_m - 4 * band);
+      left -= band * 4 * a.tiles_n;
+      bn = left / rows;
+      bm = 4 * band + left % rows;
+    }
   }
   const _Float16 *src[2 * TERMS];
   src[0] = a.P.hi + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp;
@@ -99,64 +190,157 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(const NsArgs a) {
     src[1] = a.P.lo + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp;
     src[TERMS + TERMS - 1] = a.Q.lo + z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq;
   }
-  auto issue = [&](int stage, int buffer) {
+  uint32_t off[2][NP];
 #pragma unroll
-    for (int s = 0; s < 2 * TERMS; ++s) {
-      const int ld = s < TERMS ? a.ldp : a.ldq;
+  for (int p = 0; p < NP; ++p) {
+    const int R = (wave * NP + p) * 8 + (lane >> 3);
+    const int chunk = (lane & 7) ^ ((R >> 1) & 7);
+    off[0][p] = static_cast<uint32_t>(min(R, a.rows_p - 1 - bm * TM)) * a.ldp * 2 + chunk * 16;
+    off[1][p] = static_cast<uint32_t>(min(R, a.rows_q - 1 - bn * TM)) * a.ldq * 2 + chunk * 16;
+  }
+  const int first = split * a.split_stages, stages = min(a.split_stages, a.K / kBK - first);
+  const char *from[2 * TERMS];
 #pragma unroll
-      for (int p = 0; p < kPieces / 4; ++p) {
-        const int piece = wave * (kPieces / 4) + p;
-        const int R = piece * 8 + (lane >> 3);
-        const int chunk = (lane & 7) ^ ((R >> 1) & 7);
-        const uint32_t lane_bytes = static_cast<uint32_t>(lane >> 3) * ld * 2 + chunk * 16;
-        dma_piece(src[s] + static_cast<long long>(piece) * 8 * ld + stage * kBK, lane_bytes,
-                  smem + (buffer * kStage + s * kArray + piece * 1024) / 4);
+  for (int s = 0; s < 2 * TERMS; ++s) from[s] = reinterpret_cast<const char *>(src[s] + static_cast<long long>(first) * kBK);
+  // piece k of the next stage to copy, into `slot`; the last one moves on
+  auto copy = [&](int k, int slot) {
+    const int s = k / NP, p = k % NP;
+    dma_piece(from[s], off[s < TERMS ? 0 : 1][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
+    if (p == NP - 1) from[s] += kBK * 2;
+  };
+  // a wave of one tile keeps a sum for each product and 16 k of a stage: dependent instructions issue at half the rate
+  constexpr int kSums = FM * FN == 1 ? 2 * (2 * TERMS - 1) : 1;
+  f32x16 acc[FM][FN], more[kSums];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j][e] = 0.f;
+#pragma unroll
+    for (int i = 1; i < kSums; ++i) more[i][e] = 0.f;
+  }
+  const int wm = wave / WC, wn = wave % WC, hi = lane >> 5, l31 = lane & 31;
+  const unsigned x = (l31 >> 1) & 7;
+  unsigned prow[4], qrow[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    prow[k] = (wm * FM * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
+    qrow[k] = TERMS * kArray + (wn * FN * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
+  }
+  f16x8 p[2][TERMS][FM], q[2][TERMS][FN];
+  // fragment k (of kReads) of 16 k of a slot
+  constexpr int kReads = TERMS * (FM + FN), kProducts = (2 * TERMS - 1) * FM * FN;
+  auto fetch = [&](int set, int slot, int part, int k) {
+    const char *base = reinterpret_cast<const char *>(smem) + slot * kStage;
+    const int t = k / (FM + FN), i = k % (FM + FN);
+    if (i < FM) p[set][t][i] = *reinterpret_cast<const f16x8 *>(base + prow[part] + t * kArray + i * 4096);
+    else q[set][t][i - FM] = *reinterpret_cast<const f16x8 *>(base + qrow[part] + t * kArray + (i - FM) * 4096);
+  };
+  auto multiply = [&](int set, int k) {  // lo hi, hi lo, hi hi
+    const int t = k / (FM * FN), i = k / FN % FM, j = k % FN;
+    f32x16 &sum = kSums > 1 && t * 2 + set > 0 ? more[kSums > 1 ? t * 2 + set : 0] : acc[i][j];
+    sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[set][TERMS == 2 && t == 0][i], q[set][TERMS == 2 && t == 1][j], sum, 0, 0, 0);
+  };
+  // 16 k of a stage: the products of one set of fragments, with the reads of the other and copies of a later stage between
+  // them (one or two waves a SIMD: what is not issued in a product's shadow is paid for)
+  auto part = [&](int set, int slot, int next_part, int fill, bool more_stages, auto copies) {
+    constexpr int kOps = kReads + (decltype(copies)::value ? kPieces : 0);
+#pragma unroll
+    for (int k = 0; k < kProducts; ++k) {
+      multiply(set, k);
+#pragma unroll
+      for (int o = k * kOps / kProducts; o < (k + 1) * kOps / kProducts; ++o) {
+        if (o < kReads) fetch(set ^ 1, slot, next_part, o);
+        else if (more_stages) copy(o - kReads, fill);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  f32x16 acc[F][F];
+  for (int s = 0; s < RING && s < stages; ++s)
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+    for (int k = 0; k < kPieces; ++k) copy(k, s);
+  if (stages >= RING) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 1) * kPieces) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < F; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  const int wm = wave >> 1, wn = wave & 1, hi = lane >> 5, l31 = lane & 31;
-  const unsigned x = (l31 >> 1) & 7;
-  const unsigned prow = (wm * (TM / 2) + l31) * 128, qrow = (wn * (TM / 2) + l31) * 128;
-  const int stages = a.K / kBK;
-  issue(0, 0);
+  for (int k = 0; k < kReads; ++k) fetch(0, 0, 0, k);
+  int slot = 0;
+#pragma unroll 1
   for (int s = 0; s < stages; ++s) {
-    // this wave's copies of stage s have landed and its reads of stage s - 1 are done; behind the barrier every wave's
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    const int next = slot + 1 == RING ? 0 : slot + 1;
+    part(0, slot, 1, 0, false, std::false_type{});
+    part(1, slot, 2, 0, false, std::false_type{});
+    part(0, slot, 3, 0, false, std::false_type{});
+    // this wave's copies of stage s + 1 have landed and all its reads of stage s are done; behind the barrier every wave's
+    if (s + RING <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * kPieces) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0), as the builtin: the compiler counts it
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < stages) issue(s + 1, (s + 1) & 1);
-    const char *base = reinterpret_cast<const char *>(smem) + (s & 1) * kStage;
+    part(1, next, 0, slot, s + RING < stages, std::true_type{});  // (behind the last stage: reads what the slot holds, not used)
+    slot = next;
+  }
+  if constexpr (kSums > 1) {
 #pragma unroll
-    for (int k = 0; k < kBK / 16; ++k) {
-      const unsigned slot = ((2 * k + hi) ^ x) * 16;
-      f16x8 p[TERMS][F], q[TERMS][F];
+    for (int e = 0; e < 16; ++e) {
+      float v = acc[0][0][e];
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-          p[t][i] = *reinterpret_cast<const f16x8 *>(base + t * kArray + prow + i * 32 * 128 + slot);
-          q[t][i] = *reinterpret_cast<const f16x8 *>(base + (TERMS + t) * kArray + qrow + i * 32 * 128 + slot);
-        }
-#pragma unroll
-      for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) {
-          if constexpr (TERMS == 2) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[1][i], q[0][j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0][i], q[1][j], acc[i][j], 0, 0, 0);
-          }
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0][i], q[0][j], acc[i][j], 0, 0, 0);
-        }
+      for (int i = 1; i < kSums; ++i) v += more[i][e];
+      acc[0][0][e] = v;
     }
   }
-  // accumulator e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+  if (EPI == GRAM && TM == 64 && a.splits > 1) {
+    // The last of the tile's workgroups to arrive adds all of them up in the order of their numbers (its own among them: the
+    // result does not depend on who is last) and leaves the count at zero for the next launch.  The sums are exchanged by
+    // relaxed agent-scope accesses, which pass the XCDs' own L2s by; a store has completed when vmcnt says so, and the count
+    // is raised behind the barrier that follows.  (Fences instead -- a write-back and an invalidation of the whole L2 by every
+    // wave -- cost 28 us a launch.)
+    const long long tile = z * (gridDim.x / a.splits) + blockIdx.x / a.splits;
+    constexpr int kThreads = kWaves * 64, kPairs = FM * FN * 8;
+    unsigned long long *all = reinterpret_cast<unsigned long long *>(a.partials) + tile * a.splits * kPairs * kThreads + tid;
+    unsigned long long *mine = all + static_cast<long long>(split) * kPairs * kThreads;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const float lo = acc[i][j][2 * g], up = acc[i][j][2 * g + 1];
+          const unsigned long long v = __builtin_bit_cast(uint32_t, lo) | static_cast<unsigned long long>(__builtin_bit_cast(uint32_t, up)) << 32;
+          __hip_atomic_store(mine + ((i * FN + j) * 8 + g) * kThreads, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    unsigned *arrived = reinterpret_cast<unsigned *>(smem);
+    if (tid == 0) *arrived = __hip_atomic_fetch_add(a.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*arrived != static_cast<unsigned>(a.splits - 1)) return;
+    if (tid == 0) __hip_atomic_store(a.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+#pragma unroll 1
+    for (int s = 0; s < a.splits; ++s) {
+      unsigned long long v[kPairs];
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) v[k] = __hip_atomic_load(all + (static_cast<long long>(s) * kPairs + k) * kThreads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const uint32_t lo = static_cast<uint32_t>(v[k]), up = static_cast<uint32_t>(v[k] >> 32);
+        acc[k / 8 / FN][k / 8 % FN][k % 8 * 2] += __builtin_bit_cast(float, lo);
+        acc[k / 8 / FN][k / 8 % FN][k % 8 * 2 + 1] += __builtin_bit_cast(float, up);
+      }
+    }
+    __syncthreads();  // everyone has read *arrived
+  }
+  // Accumulator e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.  Stores: rows are made of four columns
+  // per lane by a transposition within quads (8 bytes a lane, 64 a row), the transposed copy of eight rows per lane by
+  // exchanging with the lane of the other half (16 bytes).
   constexpr bool two = TERMS == 2;
   Terms D = a.D, DT = a.DT;
   D.hi += z * a.d_stride;
@@ -166,13 +350,16 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(const NsArgs a) {
     DT.lo += z * a.dt_stride;
   }
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j)
+    for (int j = 0; j < FN; ++j) {
+      const int m0 = bm * TM + (wm * FM + i) * 32, n0 = bn * TM + (wn * FN + j) * 32;
+      if (m0 >= a.rows_p || n0 >= a.rows_q) continue;  // (32-row blocks are whole)
+      const int n = n0 + l31;
+      uint32_t h[4][2], l[4][2];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int m = bm * TM + wm * (TM / 2) + i * 32 + 8 * g + 4 * hi;
-        const int n = bn * TM + wn * (TM / 2) + j * 32 + l31;
+        const int m = m0 + 8 * g + 4 * hi;
         float v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * g + k];
@@ -181,82 +368,283 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(const NsArgs a) {
           for (int k = 0; k < 4; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
         } else if constexpr (EPI == POLY) {
           const long long at = z * a.p_stride + static_cast<long long>(n) * a.ldp + m;  // A[n][m] = A[m][n]
-          const f16x4 h = *reinterpret_cast<const f16x4 *>(a.P.hi + at);
-          f16x4 l = {0, 0, 0, 0};
-          if (two) l = *reinterpret_cast<const f16x4 *>(a.P.lo + at);
+          const f16x4 ah = *reinterpret_cast<const f16x4 *>(a.P.hi + at);
+          f16x4 al = {0, 0, 0, 0};
+          if (two) al = *reinterpret_cast<const f16x4 *>(a.P.lo + at);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            v[k] = a.c * (v[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(h[k]) + static_cast<float>(l[k])) +
+            v[k] = a.c * (v[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(ah[k]) + static_cast<float>(al[k])) +
                    (m + k == n ? a.a * kScaleA : 0.f);
         } else if constexpr (EPI == UPDATE) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] *= 1.f / kScaleA;
         } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (m + k < a.r && n < a.cols) {
-              const long long at = static_cast<long long>(z) * a.r * a.cols +
-                                   (a.tall ? static_cast<long long>(n) * a.r + m + k : static_cast<long long>(m + k) * a.cols + n);
-              put_out(a.out, a.dtype, at, v[k] * (1.f / (kScaleA * kScaleX)));
-            }
-          }
+          for (int k = 0; k < 4; ++k) v[k] *= 1.f / (kScaleA * kScaleX);
+          put_final(a, z, m, n, n0 + (l31 & ~3), lane, v);
           continue;
         }
-        put_terms4(DT, static_cast<long long>(n) * a.lddt + m, v, two);
-        if (EPI == UPDATE || bm != bn) {
+        f16x4 vh, vl;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) put_terms(D, static_cast<long long>(m + k) * a.ldd + n, v[k], two);
+        for (int k = 0; k < 4; ++k) {
+          vh[k] = static_cast<_Float16>(v[k]);
+          vl[k] = static_cast<_Float16>(v[k] - static_cast<float>(vh[k]));
+        }
+        const u32x2 bh = __builtin_bit_cast(u32x2, vh), bl = __builtin_bit_cast(u32x2, vl);
+        h[g][0] = bh.x;
+        h[g][1] = bh.y;
+        l[g][0] = bl.x;
+        l[g][1] = bl.y;
+        if (EPI == UPDATE || bm != bn) {
+          const long long at = static_cast<long long>(m + (lane & 3)) * a.ldd + n0 + (l31 & ~3);
+          const Pair2 th = quad_transpose(bh.x, bh.y, lane);
+          *reinterpret_cast<u32x2 *>(D.hi + at) = u32x2{th.x, th.y};
+          if (two) {
+            const Pair2 tl = quad_transpose(bl.x, bl.y, lane);
+            *reinterpret_cast<u32x2 *>(D.lo + at) = u32x2{tl.x, tl.y};
+          }
         }
       }
+      if constexpr (EPI != FINAL) {
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {  // groups g (kept by the lower half) and g + 1 (by the upper one): eight rows each
+          const long long at = static_cast<long long>(n) * a.lddt + m0 + 8 * (g + hi);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            swap_halves(h[g][k], h[g + 1][k]);
+            if (two) swap_halves(l[g][k], l[g + 1][k]);
+          }
+          *reinterpret_cast<u32x4 *>(DT.hi + at) = u32x4{h[g][0], h[g][1], h[g + 1][0], h[g + 1][1]};
+          if (two) *reinterpret_cast<u32x4 *>(DT.lo + at) = u32x4{l[g][0], l[g][1], l[g + 1][0], l[g + 1][1]};
+        }
+      }
+    }
 }
 
-// sums of squares: kNormParts partial sums per matrix
-__global__ __launch_bounds__(256) void ns_norm_kernel(const void *in, int dtype, long long count, double *partials) {
+// sums of squares, gridDim.x partial sums per matrix
+template <typename V>
+__global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long count, double *partials) {
+  constexpr int E = 16 / sizeof(V);
+  using Vec = __attribute__((ext_vector_type(E))) V;
+  typedef Vec Loose __attribute__((aligned(sizeof(V))));  // a matrix of the batch may start at any element
   __shared__ double scratch[4];
   double s = 0;
-  const long long base = blockIdx.y * count;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < count; i += 256LL * kNormParts) {
-    const double v = get_in(in, dtype, base + i);
-    s += v * v;
+  const V *g = in + blockIdx.y * count;
+  const long long step = 256LL * gridDim.x, vectors = count / E;
+#pragma unroll 4
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < vectors; i += step) {
+    const Vec v = *reinterpret_cast<const Loose *>(g + i * E);
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const double x = static_cast<double>(static_cast<float>(v[k]));
+      s += x * x;
+    }
+  }
+  const long long last = vectors * E + threadIdx.x;
+  if (blockIdx.x == 0 && last < count) {
+    const double x = static_cast<double>(static_cast<float>(g[last]));
+    s += x * x;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) partials[blockIdx.y * static_cast<long long>(kNormParts) + blockIdx.x] = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  if (threadIdx.x == 0) partials[blockIdx.y * static_cast<long long>(gridDim.x) + blockIdx.x] = scratch[0] + scratch[1] + scratch[2] + scratch[3];
 }
 
-// X0 and its transpose from a 64 x 64 tile of G: `same` has G's orientation (ld_same), `turned` the other
-template <bool TWO>
-__global__ __launch_bounds__(256) void ns_pack_kernel(const void *in, int dtype, int m, int n, const double *partials, float eps,
-                                                      Terms same, int ld_same, Terms turned, int ld_turned, long long stride) {
+// X0 and its transpose from a 64 x 64 tile of G: `same` has G's orientation (ld_same), `turned` the other.  Also clears the
+// arrival counts of the split products.
+template <typename V, bool TWO>
+__global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n, const double *partials, int parts, float eps, Terms same,
+                                                      int ld_same, Terms turned, int ld_turned, long long stride, unsigned *arrivals, int counts) {
+  constexpr int E = 16 / sizeof(V);
+  using Vec = __attribute__((ext_vector_type(E))) V;
+  typedef Vec Loose __attribute__((aligned(sizeof(V))));
   __shared__ float tile[64][65];
-  __shared__ double total;
+  __shared__ double total[4];
   const long long z = blockIdx.z;
-  if (threadIdx.x < 64) {
-    double s = partials[z * kNormParts + threadIdx.x];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    if (threadIdx.x == 0) total = kScaleX / (sqrt(s) + eps);
-  }
-  __syncthreads();
-  const double factor = total;  // double: the norm of the largest fp32 entries is no fp32 number
   const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-  const int col = threadIdx.x & 63;
-  for (int row = threadIdx.x >> 6; row < 64; row += 4) {
+  const V *g = in + z * m * n;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && z == 0)
+    for (int i = threadIdx.x; i < counts; i += 256) arrivals[i] = 0;
+  // 64 rows of 64 / E vectors
+#pragma unroll
+  for (int k = 0; k < 64 * 64 / E / 256; ++k) {
+    const int at = k * 256 + threadIdx.x, row = at / (64 / E), col = at % (64 / E) * E;
+    Vec v = {};
+    if (r0 + row < m) {
+      const V *from = g + static_cast<long long>(r0 + row) * n + c0 + col;
+      if (c0 + col + E <= n) v = *reinterpret_cast<const Loose *>(from);
+      else
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (c0 + col + i < n) v[i] = from[i];
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) tile[row][col + i] = static_cast<float>(v[i]);
+  }
+  double s = 0;
+  for (int i = threadIdx.x; i < parts; i += 256) s += partials[z * parts + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = s;
+  __syncthreads();
+  const double factor = kScaleX / (sqrt(total[0] + total[1] + total[2] + total[3]) + eps);  // double: the norm may exceed fp32's range
+  const int mp = (m + kPad - 1) / kPad * kPad, np = (n + kPad - 1) / kPad * kPad;
+  auto put8 = [&](const Terms &t, long long at, auto value) {
+    f16x8 h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = static_cast<float>(value(i) * factor);
+      h[i] = static_cast<_Float16>(v);
+      l[i] = static_cast<_Float16>(v - static_cast<float>(h[i]));
+    }
+    *reinterpret_cast<f16x8 *>(t.hi + at) = h;
+    if (TWO) *reinterpret_cast<f16x8 *>(t.lo + at) = l;
+  };
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {  // 64 rows of 8 x 8 values; the sides are multiples of 64: a row of 8 is whole or outside
+    const int at = k * 256 + threadIdx.x, row = at >> 3, col = (at & 7) * 8;
+    if (r0 + row < mp && c0 + col < np) put8(same, z * stride + static_cast<long long>(r0 + row) * ld_same + c0 + col, [&](int i) { return tile[row][col + i]; });
+    if (c0 + row < np && r0 + col < mp) put8(turned, z * stride + static_cast<long long>(c0 + row) * ld_turned + r0 + col, [&](int i) { return tile[col + i][row]; });
+  }
+}
+
+// ---- matrices that fit a workgroup's LDS: the whole iteration in ONE launch, a workgroup per matrix -----------------
+// X, X^T, A and B stay in LDS (rows padded by 16 bytes: an odd number of 16-byte chunks, so that 16 rows' equal chunks meet
+// every bank once); 16 waves share the 16 x 16 x 32 tiles of each product.  The update holds its tiles in registers over a
+// barrier and then overwrites X and X^T.  What bounds it is the chain of 3 x steps dependent products, not their rate.
+constexpr int kSmallWaves = 16, kSmallTiles = 10;  // tiles of X a wave holds at most (the LDS limit keeps r c <= 160 x 256)
+constexpr long long kSmallLds = 160 * 1024 - 256;
+
+inline long long small_lds(int rp, int cp, int terms) {
+  return 2LL * terms * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8) + 2LL * rp * (rp + 8));
+}
+
+struct SmallArgs {
+  const void *in;
+  void *out;
+  int dtype, m, n, r, c, rp, cp, steps, tall;
+  float a, b, k, eps;
+};
+
+template <int TERMS>
+__global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ double parts[kSmallWaves];
+  constexpr bool two = TERMS == 2;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ldx = a.cp + 8, ldr = a.rp + 8;  // X: rp rows of ldx; X^T: cp rows of ldr; A, B: rp rows of ldr
+  _Float16 *at = reinterpret_cast<_Float16 *>(lds);
+  auto take = [&](int values) {
+    Terms t;
+    t.hi = at;
+    t.lo = at + values;
+    at += TERMS * values;
+    return t;
+  };
+  const Terms X = take(a.rp * ldx), XT = take(a.cp * ldr), A = take(a.rp * ldr), B = take(a.rp * ldr);
+  const int count = a.m * a.n;
+  const long long base = blockIdx.x * static_cast<long long>(count);
+  double s = 0;
+  for (int i = tid; i < count; i += kSmallWaves * 64) {
+    const double v = get_in(a.in, a.dtype, base + i);
+    s += v * v;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (lane == 0) parts[wave] = s;
+  __syncthreads();
+  s = 0;
+  for (int i = 0; i < kSmallWaves; ++i) s += parts[i];
+  const double factor = kScaleX / (sqrt(s) + a.eps);
+  for (int i = tid; i < a.rp * a.cp; i += kSmallWaves * 64) {
+    const int row = i / a.cp, col = i - row * a.cp;
     float v = 0.f;
-    if (r0 + row < m && c0 + col < n)
-      v = static_cast<float>(get_in(in, dtype, z * m * n + static_cast<long long>(r0 + row) * n + c0 + col) * factor);
-    put_terms(same, z * stride + static_cast<long long>(r0 + row) * ld_same + c0 + col, v, TWO);
-    tile[row][col] = v;
+    if (row < a.r && col < a.c) v = static_cast<float>(get_in(a.in, a.dtype, base + (a.tall ? col * a.n + row : row * a.n + col)) * factor);
+    put_terms(X, row * ldx + col, v, two);
+    put_terms(XT, col * ldr + row, v, two);
   }
   __syncthreads();
-  for (int row = threadIdx.x >> 6; row < 64; row += 4)
-    put_terms(turned, z * stride + static_cast<long long>(c0 + row) * ld_turned + r0 + col, tile[col][row], TWO);
+  const int l15 = lane & 15, quad = lane >> 4;
+  // acc = P[16 rows from pm] Q[16 rows from qn]^T; accumulator e of a lane: row 4 (lane / 16) + e, column lane % 16
+  auto product = [&](const Terms &P, int ldp, int pm, const Terms &Q, int ldq, int qn, int K) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int po = (pm + l15) * ldp + quad * 8, qo = (qn + l15) * ldq + quad * 8;
+    for (int k = 0; k < K; k += 32) {
+      const f16x8 ph = *reinterpret_cast<const f16x8 *>(P.hi + po + k), qh = *reinterpret_cast<const f16x8 *>(Q.hi + qo + k);
+      if (two) {
+        const f16x8 pl = *reinterpret_cast<const f16x8 *>(P.lo + po + k), ql = *reinterpret_cast<const f16x8 *>(Q.lo + qo + k);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, acc, 0, 0, 0);
+      }
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+    }
+    return acc;
+  };
+  const int tr = a.rp / 16, tc = a.cp / 16;
+  for (int step = 0; step < a.steps; ++step) {
+    for (int half = 0; half < 2; ++half) {  // A = X X^T, then B = a I + b A + c A A: upper triangles, stored twice
+      for (int tile = wave; tile < tr * (tr + 1) / 2; tile += kSmallWaves) {
+        int left = tile, row = 0;
+        while (left >= tr - row) left -= tr - row++;
+        const int pm = row * 16, qn = (row + left) * 16;
+        const f32x4 acc = half ? product(A, ldr, pm, A, ldr, qn, a.rp) : product(X, ldx, pm, X, ldx, qn, a.cp);
+        const int m = pm + 4 * quad, n = qn + l15;
+        float v[4];
+        if (half) {
+          const f16x4 h = *reinterpret_cast<const f16x4 *>(A.hi + n * ldr + m);
+          f16x4 l = {0, 0, 0, 0};
+          if (two) l = *reinterpret_cast<const f16x4 *>(A.lo + n * ldr + m);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[k] = a.k * (acc[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(h[k]) + static_cast<float>(l[k])) + (m + k == n ? a.a * kScaleA : 0.f);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = acc[k] * (kScaleA / (kScaleX * kScaleX));
+        }
+        const Terms &D = half ? B : A;
+        put_terms4(D, n * ldr + m, v, two);
+        if (pm != qn)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) put_terms(D, (m + k) * ldr + n, v[k], two);
+      }
+      __syncthreads();
+    }
+    f32x4 held[kSmallTiles];
+#pragma unroll
+    for (int i = 0; i < kSmallTiles; ++i) {
+      const int tile = wave + i * kSmallWaves;
+      if (tile < tr * tc) held[i] = product(B, ldr, tile % tr * 16, XT, ldr, tile / tr * 16, a.rp);
+    }
+    __syncthreads();
+    const bool last = step + 1 == a.steps;
+#pragma unroll
+    for (int i = 0; i < kSmallTiles; ++i) {
+      const int tile = wave + i * kSmallWaves;
+      if (tile >= tr * tc) continue;
+      const int m = tile % tr * 16 + 4 * quad, n = tile / tr * 16 + l15;
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = held[i][k] * (1.f / kScaleA);
+      if (last) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (m + k < a.r && n < a.c)
+            put_out(a.out, a.dtype, base + (a.tall ? n * a.n + m + k : (m + k) * a.n + n), v[k] * (1.f / kScaleX));
+      } else {
+        put_terms4(XT, n * ldr + m, v, two);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) put_terms(X, (m + k) * ldx + n, v[k], two);
+      }
+    }
+    __syncthreads();
+  }
 }
 
 struct Plan {
-  int r, c, rp, cp, terms;
+  int r, c, rp, cp, terms, parts;
   long long x, sq;             // values of X and of A per matrix, padded
   long long bytes;
 };
@@ -270,7 +658,9 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   p.x = static_cast<long long>(p.rp) * p.cp;
   p.sq = static_cast<long long>(p.rp) * p.rp;
   // X, two copies of X^T, A, B, and the norm's partial sums
-  p.bytes = batch * (p.terms * 2 * (3 * p.x + 2 * p.sq) + 8LL * kNormParts);
+  const long long blocks = (static_cast<long long>(m) * n + 8191) / 8192;  // 8192 elements a workgroup at least
+  p.parts = static_cast<int>(blocks < kNormParts ? blocks : kNormParts);
+  p.bytes = batch * (p.terms * 2 * (3 * p.x + 2 * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4LL * kSplitGroups * 64 * 64;
   return p;
 }
 int check_shape(int dtype, int batch, int m, int n) {
@@ -280,43 +670,78 @@ int check_shape(int dtype, int batch, int m, int n) {
   return DX_OK;
 }
 
-template <int TM, int TERMS, Epilogue EPI>
-int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
-  constexpr int bytes = 2 * 2 * TERMS * TM * kBK * 2;
-  DX_LDS_OPT_IN((ns_gemm_kernel<TM, TERMS, EPI>), bytes);
+template <int TM, int WR, int WC, int TERMS, int RING, Epilogue EPI>
+int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
+  constexpr int bytes = RING * 2 * TERMS * TM * kBK * 2;
+  DX_LDS_OPT_IN((ns_gemm_kernel<TM, WR, WC, TERMS, RING, EPI>), bytes);
+  a.tiles_m = cdiv(a.rows_p, TM);
+  a.tiles_n = cdiv(a.rows_q, TM);
   const int tiles = EPI == GRAM || EPI == POLY ? a.tiles_m * (a.tiles_m + 1) / 2 : a.tiles_m * a.tiles_n;
-  hipLaunchKernelGGL((ns_gemm_kernel<TM, TERMS, EPI>), dim3(tiles, batch), dim3(256), bytes, s, a);
+  a.split_stages = cdiv(a.K / kBK, splits);
+  a.splits = cdiv(a.K / kBK, a.split_stages);
+  hipLaunchKernelGGL((ns_gemm_kernel<TM, WR, WC, TERMS, RING, EPI>), dim3(tiles * a.splits, batch), dim3(WR * WC * 64), bytes, s, a);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
+// The tile whose rounds over the CUs take the shortest: a stage's time is its copies' (about 28 bytes a cycle and CU), so a
+// round's goes with the tile's SIDE.  Measured (us for the whole operator, this product's tile changed): 4096^2 bf16 gram 1475
+// at 192 (253 tiles, one round), 1555 at 256, 1600 at 128; 3 x 1023 x 769 bf16 gram 227 at 64, 251 at 128, update 252 at 128,
+// 260 at 64; 2001 x 5003 f32 gram 1528 at 128, 1623 at 64.  Ties go to the smaller tile (its epilogue is shorter).
+// X X^T of a wide matrix has few tiles and a long K: K is split until the CUs are busy, where that saves more than the 4 us
+// that the exchange of the sums takes: 512 x 3136 f32 (36 tiles, 49 stages of 0.45 us) 276 us in one piece, 224 in seven;
+// 128 x 1000 bf16 (3 tiles, 16 stages of 0.2 us) 85 against 89 in four.
+template <int TERMS, Epilogue EPI>
+int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
+  constexpr bool half = EPI == GRAM || EPI == POLY;
+  int cus = 0;
+  if (int rc = device_cus(&cus)) return rc;
+  auto tiles = [&](int tile) {
+    const long long m = cdiv(a.rows_p, tile), n = cdiv(a.rows_q, tile);
+    return (half ? m * (m + 1) / 2 : m * n) * batch;
+  };
+  int best = 64;
+  for (int tile = 128; tile <= (TERMS == 1 ? 256 : 128); tile += 64)
+    if ((tiles(tile) + cus - 1) / cus * tile < (tiles(best) + cus - 1) / cus * best) best = tile;
+  if constexpr (TERMS == 1) {
+    if (best == 256) return launch_tile<256, 2, 4, 1, 2, EPI>(a, batch, 1, s);
+    if (best == 192) return launch_tile<192, 2, 2, 1, 3, EPI>(a, batch, 1, s);
+  }
+  if (best == 128) return launch_tile<128, 2, 2, TERMS, 2, EPI>(a, batch, 1, s);
+  long long splits = 1;
+  if (EPI == GRAM && a.K / kBK >= (TERMS == 2 ? 16 : 32)) {
+    splits = (cus < kSplitGroups ? cus : kSplitGroups) / tiles(64);
+    if (splits > a.K / kBK / 6) splits = a.K / kBK / 6;
+    if (splits < 1) splits = 1;
+  }
+  return launch_tile<64, 2, 2, TERMS, 4, EPI>(a, batch, static_cast<int>(splits), s);
+}
 template <int TERMS>
 int run_steps(const Plan &p, int batch, int steps, NsArgs a, Terms X, Terms XT0, Terms XT1, Terms A, Terms B, hipStream_t s) {
-  constexpr int TM = 128;
   for (int k = 0; k < steps; ++k) {
     const Terms xt = k & 1 ? XT1 : XT0, next = k & 1 ? XT0 : XT1;
     NsArgs g = a;
     g.P = g.Q = X;
     g.p_stride = g.q_stride = p.x;
     g.ldp = g.ldq = g.K = p.cp;
-    g.tiles_m = g.tiles_n = p.rp / TM;
+    g.rows_p = g.rows_q = p.rp;
     g.D = g.DT = A;
     g.d_stride = g.dt_stride = p.sq;
     g.ldd = g.lddt = p.rp;
-    if (int rc = launch_gemm<TM, TERMS, GRAM>(g, batch, s)) return rc;
+    if (int rc = launch_gemm<TERMS, GRAM>(g, batch, s)) return rc;
     g.P = g.Q = A;
     g.p_stride = g.q_stride = p.sq;
     g.ldp = g.ldq = g.K = p.rp;
     g.D = g.DT = B;
-    if (int rc = launch_gemm<TM, TERMS, POLY>(g, batch, s)) return rc;
+    if (int rc = launch_gemm<TERMS, POLY>(g, batch, s)) return rc;
     g.P = B;
     g.Q = xt;
     g.q_stride = p.x;
-    g.tiles_n = p.cp / TM;
+    g.rows_q = p.cp;
     g.D = X;
     g.DT = next;
     g.d_stride = g.dt_stride = p.x;
     g.ldd = p.cp;
-    if (int rc = k + 1 < steps ? launch_gemm<TM, TERMS, UPDATE>(g, batch, s) : launch_gemm<TM, TERMS, FINAL>(g, batch, s)) return rc;
+    if (int rc = k + 1 < steps ? launch_gemm<TERMS, UPDATE>(g, batch, s) : launch_gemm<TERMS, FINAL>(g, batch, s)) return rc;
   }
   return DX_OK;
 }
@@ -343,6 +768,19 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   const Plan p = make_plan(dtype, batch, m, n);
   if (workspace_bytes < p.bytes) return fail(DX_EWS, "dx_orthogonalize: workspace of %lld bytes, %lld needed", workspace_bytes, p.bytes);
   hipStream_t s = as_stream(stream);
+  if (small_lds(p.rp, p.cp, p.terms) <= kSmallLds) {
+    const SmallArgs q{update, out, dtype, m, n, p.r, p.c, p.rp, p.cp, steps, m > n, a, b, c, eps};
+    const int bytes = static_cast<int>(small_lds(p.rp, p.cp, p.terms));
+    if (p.terms == 2) {
+      DX_LDS_OPT_IN(ns_small_kernel<2>, kSmallLds);
+      hipLaunchKernelGGL(ns_small_kernel<2>, dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
+    } else {
+      DX_LDS_OPT_IN(ns_small_kernel<1>, kSmallLds);
+      hipLaunchKernelGGL(ns_small_kernel<1>, dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
+    }
+    DX_LAUNCH_CHECK();
+    return DX_OK;
+  }
   _Float16 *at = static_cast<_Float16 *>(workspace);
   auto take = [&](long long values) {
     Terms t;
@@ -354,18 +792,30 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   };
   const Terms X = take(p.x), XT0 = take(p.x), XT1 = take(p.x), A = take(p.sq), B = take(p.sq);
   double *partials = reinterpret_cast<double *>(at);
-  hipLaunchKernelGGL(ns_norm_kernel, dim3(kNormParts, batch), dim3(256), 0, s, update, dtype, static_cast<long long>(m) * n, partials);
+  unsigned *arrivals = reinterpret_cast<unsigned *>(partials + static_cast<long long>(batch) * p.parts);
+  float *split = reinterpret_cast<float *>(arrivals + kSplitGroups);
+  const long long count = static_cast<long long>(m) * n;
+  if (dtype == DX_F32) hipLaunchKernelGGL(ns_norm_kernel<float>, dim3(p.parts, batch), dim3(256), 0, s, static_cast<const float *>(update), count, partials);
+  else if (dtype == DX_BF16) hipLaunchKernelGGL(ns_norm_kernel<__bf16>, dim3(p.parts, batch), dim3(256), 0, s, static_cast<const __bf16 *>(update), count, partials);
+  else hipLaunchKernelGGL(ns_norm_kernel<_Float16>, dim3(p.parts, batch), dim3(256), 0, s, static_cast<const _Float16 *>(update), count, partials);
   DX_LAUNCH_CHECK();
   const bool tall = m > n;
-  const dim3 grid((tall ? p.rp : p.cp) / 64, (tall ? p.cp : p.rp) / 64, batch);
+  const dim3 grid(cdiv(tall ? p.rp : p.cp, 64), cdiv(tall ? p.cp : p.rp, 64), batch);
   const Terms same = tall ? XT0 : X, turned = tall ? X : XT0;
   const int ld_same = tall ? p.rp : p.cp, ld_turned = tall ? p.cp : p.rp;
-  if (p.terms == 2)
-    hipLaunchKernelGGL(ns_pack_kernel<true>, grid, dim3(256), 0, s, update, dtype, m, n, partials, eps, same, ld_same, turned, ld_turned, p.x);
+  if (dtype == DX_F32)
+    hipLaunchKernelGGL((ns_pack_kernel<float, true>), grid, dim3(256), 0, s, static_cast<const float *>(update), m, n, partials, p.parts, eps,
+                       same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
+  else if (dtype == DX_BF16)
+    hipLaunchKernelGGL((ns_pack_kernel<__bf16, false>), grid, dim3(256), 0, s, static_cast<const __bf16 *>(update), m, n, partials, p.parts, eps,
+                       same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   else
-    hipLaunchKernelGGL(ns_pack_kernel<false>, grid, dim3(256), 0, s, update, dtype, m, n, partials, eps, same, ld_same, turned, ld_turned, p.x);
+    hipLaunchKernelGGL((ns_pack_kernel<_Float16, false>), grid, dim3(256), 0, s, static_cast<const _Float16 *>(update), m, n, partials, p.parts,
+                       eps, same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   DX_LAUNCH_CHECK();
   NsArgs g{};
+  g.arrivals = arrivals;
+  g.partials = split;
   g.a = a;
   g.b = b;
   g.c = c;
