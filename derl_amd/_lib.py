@@ -50,7 +50,7 @@ SIGNATURES = {
     "dx_categorical_act_f32": [P, c_int, c_int, P, c_uint64, c_uint64, P, P, P, P],
     "dx_categorical_loss_f32": [P, P, P, P, P, P, c_int, c_int, c_int, c_float, c_float,
                                 c_float, c_longlong, P, P, c_int, P, P],
-    "dx_token_log_prob": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, P, P],
+    "dx_token_log_prob": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, P, P, c_longlong, P],
     "dx_sequence_log_prob": [P, P, c_longlong, c_int, P, P],
     "dx_token_policy_loss": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, P, P, c_longlong, P, c_float,
                              c_float, c_float, c_longlong, P, c_longlong, P, P, c_longlong, P, P],
@@ -135,7 +135,7 @@ class NativeError(RuntimeError):
 DX_EINVAL, DX_EHIP, DX_ENOSUP, DX_EWS, DX_ETIMEOUT = -1, -2, -3, -4, -5
 # element types and the scratch of the token losses (doubles), include/derl_amd.h
 DX_F32, DX_BF16, DX_F16 = 0, 1, 2
-DX_TOKEN_WORKSPACE = 16392
+DX_TOKEN_WORKSPACE = 19464
 
 
 def load():

@@ -3,12 +3,14 @@
 // with X the (r, c) matrix whose shorter side is r (a tall G is worked on transposed).  Odd polynomials of the singular
 // values only: the singular vectors stay G's, the singular values approach 1.
 //
-// The products run on the fp16 matrix cores with fp32 accumulation.  fp32 input is held as TWO fp16 terms, hi + lo
-// (22 bits), and a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it): fp32 accuracy at a third of the
-// fp16 rate, where the fp32 matrix instructions have a sixteenth.  16-bit input is held as one fp16 term: 11 bits, three
-// more than bf16 keeps, which the iteration needs -- each step multiplies the error of small singular values by up to
-// `a` = 3.4.  Stored values are scaled by powers of two (X by 2^12, A and B by 2^8), so that neither large entries
-// overflow nor the second term of typical ones (1 / sqrt(c)) falls under fp16's smallest step.
+// The products run on the fp16 matrix cores with fp32 accumulation.  fp32 and fp16 matrices are held as TWO fp16 terms, hi + lo
+// (22 bits): a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), fp32 accuracy at a third of the fp16 rate,
+// where the fp32 matrix instructions have a sixteenth.  For bf16 X is one term, 11 bits, three more than the result keeps
+// (each step multiplies what is lost by up to `a` = 3.4); A and B keep two terms up to r = kOneTermRows, as the fewer entries
+// they have the less their roundings average out.  Against 64 bits, with the result's own rounding as 1: everything one
+// term 2.5 at r = 37, 1.54 at 520, 1.37 at 640, 1.35 at 769, 1.2 at 4096; A and B two terms 1.1; all of it two terms 1.0.
+// Stored values are scaled by powers of two (X by 2^12, A and B by 2^8), so that neither large entries overflow nor the second
+// term of typical ones (1 / sqrt(c)) falls under fp16's smallest step.
 //
 // Every matrix product is C = P Q^T with both operands' k contiguous: X for A = X X^T, A = A^T for A^2 = A A^T, and for
 // B X the transposed copy X^T, which the epilogue of each update writes beside X.  A and B are symmetric: only tiles on
@@ -29,6 +31,7 @@ using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 constexpr float kScaleX = 4096.f, kScaleA = 256.f;
+constexpr int kOneTermRows = 640;  // bf16: with more rows A and B are held as one fp16 term too
 constexpr int kPad = 64, kBK = 64, kNormParts = 512;
 constexpr int kSplitGroups = 256;  // workgroups of a product that is split over K, at most; its tiles are half as many
 
@@ -55,22 +58,6 @@ struct NsArgs {
   int dtype, r, cols, tall;
 };
 
-__device__ __forceinline__ void put_terms(const Terms &t, long long at, float v, bool two) {
-  const _Float16 h = static_cast<_Float16>(v);
-  t.hi[at] = h;
-  if (two) t.lo[at] = static_cast<_Float16>(v - static_cast<float>(h));
-}
-__device__ __forceinline__ void put_terms4(const Terms &t, long long at, const float (&v)[4], bool two) {
-  f16x4 h, l;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    h[k] = static_cast<_Float16>(v[k]);
-    l[k] = static_cast<_Float16>(v[k] - static_cast<float>(h[k]));
-  }
-  *reinterpret_cast<f16x4 *>(t.hi + at) = h;
-  if (two) *reinterpret_cast<f16x4 *>(t.lo + at) = l;
-}
-
 // two fp16 values of consecutive rows and their successors: d0 = (row 0, row 1), d1 = (row 2, row 3) of this lane's column.
 // Transposed over the four lanes of a quad: lane j ends with row j of the quad's four columns.
 struct Pair2 { uint32_t x, y; };
@@ -89,17 +76,6 @@ __device__ __forceinline__ Pair2 quad_transpose(uint32_t d0, uint32_t d1, int la
 // folds the builtin's results where an operand is uniform)
 __device__ __forceinline__ void swap_halves(uint32_t &x, uint32_t &y) {
   asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-}
-
-__device__ __forceinline__ void put_out(void *out, int dtype, long long at, float v) {
-  if (dtype == DX_F32) static_cast<float *>(out)[at] = v;
-  else if (dtype == DX_BF16) static_cast<__bf16 *>(out)[at] = static_cast<__bf16>(v);
-  else static_cast<_Float16 *>(out)[at] = static_cast<_Float16>(v);
-}
-__device__ __forceinline__ float get_in(const void *in, int dtype, long long at) {
-  if (dtype == DX_F32) return static_cast<const float *>(in)[at];
-  if (dtype == DX_BF16) return static_cast<float>(static_cast<const __bf16 *>(in)[at]);
-  return static_cast<float>(static_cast<const _Float16 *>(in)[at]);
 }
 
 // four results of the last step, rows m .. m + 3 of column n, to the caller's matrix (which may start at any element);
@@ -152,14 +128,14 @@ __device__ __forceinline__ void put_final(const NsArgs &a, int z, int m, int n, 
 // One barrier per stage, in front of its last 16 k, whose fragments are in registers by then: behind it the stage's slot is
 // free and is filled again, and the next stage has landed everywhere, so that its first fragments are read in the shadow of
 // the last products: the matrix pipe does not wait at the barrier.  Rows past the matrix repeat its last row and are not stored.
-template <int TM, int WR, int WC, int TERMS, int RING, Epilogue EPI>
+template <int TM, int WR, int WC, int PT, int QT, int OT, int RING, Epilogue EPI>
 __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
   constexpr int kWaves = WR * WC, FM = TM / WR / 32, FN = TM / WC / 32;
   constexpr int kArray = TM * kBK * 2;           // bytes of one operand term of a stage
-  constexpr int kStage = 2 * TERMS * kArray;
+  constexpr int kStage = (PT + QT) * kArray;
   constexpr int NP = TM / 8 / kWaves;            // 1 KiB pieces (8 rows) of an array that a wave copies
-  constexpr int kPieces = 2 * TERMS * NP;
+  constexpr int kPieces = (PT + QT) * NP;
   static_assert(NP * 8 * kWaves == TM && FM * 32 * WR == TM && FN * 32 * WC == TM, "tile");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -183,13 +159,12 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
       bm = 4 * band + left % rows;
     }
   }
-  const _Float16 *src[2 * TERMS];
-  src[0] = a.P.hi + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp;
-  src[TERMS] = a.Q.hi + z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq;
-  if (TERMS == 2) {
-    src[1] = a.P.lo + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp;
-    src[TERMS + TERMS - 1] = a.Q.lo + z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq;
-  }
+  const _Float16 *src[PT + QT];
+  const long long p_at = z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp, q_at = z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq;
+  src[0] = a.P.hi + p_at;
+  if (PT == 2) src[PT - 1] = a.P.lo + p_at;
+  src[PT] = a.Q.hi + q_at;
+  if (QT == 2) src[PT + QT - 1] = a.Q.lo + q_at;
   uint32_t off[2][NP];
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
@@ -199,17 +174,18 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
     off[1][p] = static_cast<uint32_t>(min(R, a.rows_q - 1 - bn * TM)) * a.ldq * 2 + chunk * 16;
   }
   const int first = split * a.split_stages, stages = min(a.split_stages, a.K / kBK - first);
-  const char *from[2 * TERMS];
+  const char *from[PT + QT];
 #pragma unroll
-  for (int s = 0; s < 2 * TERMS; ++s) from[s] = reinterpret_cast<const char *>(src[s] + static_cast<long long>(first) * kBK);
+  for (int s = 0; s < PT + QT; ++s) from[s] = reinterpret_cast<const char *>(src[s] + static_cast<long long>(first) * kBK);
   // piece k of the next stage to copy, into `slot`; the last one moves on
   auto copy = [&](int k, int slot) {
     const int s = k / NP, p = k % NP;
-    dma_piece(from[s], off[s < TERMS ? 0 : 1][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
+    dma_piece(from[s], off[s < PT ? 0 : 1][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
     if (p == NP - 1) from[s] += kBK * 2;
   };
   // a wave of one tile keeps a sum for each product and 16 k of a stage: dependent instructions issue at half the rate
-  constexpr int kSums = FM * FN == 1 ? 2 * (2 * TERMS - 1) : 1;
+  constexpr int kPairs = PT + QT - 1;  // products of terms: hi hi | lo hi, hi hi | lo hi, hi lo, hi hi
+  constexpr int kSums = FM * FN == 1 ? 2 * kPairs : 1;
   f32x16 acc[FM][FN], more[kSums];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
@@ -226,21 +202,20 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     prow[k] = (wm * FM * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
-    qrow[k] = TERMS * kArray + (wn * FN * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
+    qrow[k] = PT * kArray + (wn * FN * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
   }
-  f16x8 p[2][TERMS][FM], q[2][TERMS][FN];
+  f16x8 p[2][PT][FM], q[2][QT][FN];
   // fragment k (of kReads) of 16 k of a slot
-  constexpr int kReads = TERMS * (FM + FN), kProducts = (2 * TERMS - 1) * FM * FN;
+  constexpr int kReads = PT * FM + QT * FN, kProducts = kPairs * FM * FN;
   auto fetch = [&](int set, int slot, int part, int k) {
     const char *base = reinterpret_cast<const char *>(smem) + slot * kStage;
-    const int t = k / (FM + FN), i = k % (FM + FN);
-    if (i < FM) p[set][t][i] = *reinterpret_cast<const f16x8 *>(base + prow[part] + t * kArray + i * 4096);
-    else q[set][t][i - FM] = *reinterpret_cast<const f16x8 *>(base + qrow[part] + t * kArray + (i - FM) * 4096);
+    if (k < PT * FM) p[set][k / FM][k % FM] = *reinterpret_cast<const f16x8 *>(base + prow[part] + k / FM * kArray + k % FM * 4096);
+    else q[set][(k - PT * FM) / FN][(k - PT * FM) % FN] = *reinterpret_cast<const f16x8 *>(base + qrow[part] + (k - PT * FM) / FN * kArray + (k - PT * FM) % FN * 4096);
   };
-  auto multiply = [&](int set, int k) {  // lo hi, hi lo, hi hi
+  auto multiply = [&](int set, int k) {  // the small products first
     const int t = k / (FM * FN), i = k / FN % FM, j = k % FN;
     f32x16 &sum = kSums > 1 && t * 2 + set > 0 ? more[kSums > 1 ? t * 2 + set : 0] : acc[i][j];
-    sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[set][TERMS == 2 && t == 0][i], q[set][TERMS == 2 && t == 1][j], sum, 0, 0, 0);
+    sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[set][PT == 2 && t == 0][i], q[set][QT == 2 && t == kPairs - 2][j], sum, 0, 0, 0);
   };
   // 16 k of a stage: the products of one set of fragments, with the reads of the other and copies of a later stage between
   // them (one or two waves a SIMD: what is not issued in a product's shadow is paid for)
@@ -298,9 +273,9 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
     // is raised behind the barrier that follows.  (Fences instead -- a write-back and an invalidation of the whole L2 by every
     // wave -- cost 28 us a launch.)
     const long long tile = z * (gridDim.x / a.splits) + blockIdx.x / a.splits;
-    constexpr int kThreads = kWaves * 64, kPairs = FM * FN * 8;
-    unsigned long long *all = reinterpret_cast<unsigned long long *>(a.partials) + tile * a.splits * kPairs * kThreads + tid;
-    unsigned long long *mine = all + static_cast<long long>(split) * kPairs * kThreads;
+    constexpr int kThreads = kWaves * 64, kWords = FM * FN * 8;
+    unsigned long long *all = reinterpret_cast<unsigned long long *>(a.partials) + tile * a.splits * kWords * kThreads + tid;
+    unsigned long long *mine = all + static_cast<long long>(split) * kWords * kThreads;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -326,11 +301,11 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 #pragma unroll 1
     for (int s = 0; s < a.splits; ++s) {
-      unsigned long long v[kPairs];
+      unsigned long long v[kWords];
 #pragma unroll
-      for (int k = 0; k < kPairs; ++k) v[k] = __hip_atomic_load(all + (static_cast<long long>(s) * kPairs + k) * kThreads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int k = 0; k < kWords; ++k) v[k] = __hip_atomic_load(all + (static_cast<long long>(s) * kWords + k) * kThreads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-      for (int k = 0; k < kPairs; ++k) {
+      for (int k = 0; k < kWords; ++k) {
         const uint32_t lo = static_cast<uint32_t>(v[k]), up = static_cast<uint32_t>(v[k] >> 32);
         acc[k / 8 / FN][k / 8 % FN][k % 8 * 2] += __builtin_bit_cast(float, lo);
         acc[k / 8 / FN][k / 8 % FN][k % 8 * 2 + 1] += __builtin_bit_cast(float, up);
@@ -341,7 +316,7 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   // Accumulator e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.  Stores: rows are made of four columns
   // per lane by a transposition within quads (8 bytes a lane, 64 a row), the transposed copy of eight rows per lane by
   // exchanging with the lane of the other half (16 bytes).
-  constexpr bool two = TERMS == 2;
+  constexpr bool two = OT == 2;
   Terms D = a.D, DT = a.DT;
   D.hi += z * a.d_stride;
   DT.hi += z * a.dt_stride;
@@ -370,7 +345,7 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
           const long long at = z * a.p_stride + static_cast<long long>(n) * a.ldp + m;  // A[n][m] = A[m][n]
           const f16x4 ah = *reinterpret_cast<const f16x4 *>(a.P.hi + at);
           f16x4 al = {0, 0, 0, 0};
-          if (two) al = *reinterpret_cast<const f16x4 *>(a.P.lo + at);
+          if (PT == 2) al = *reinterpret_cast<const f16x4 *>(a.P.lo + at);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             v[k] = a.c * (v[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(ah[k]) + static_cast<float>(al[k])) +
@@ -421,18 +396,16 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
     }
 }
 
-// sums of squares, gridDim.x partial sums per matrix
+// this thread's share of a sum of squares over `count` values: thread `at` of `threads`
 template <typename V>
-__global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long count, double *partials) {
+__device__ __forceinline__ double sum_of_squares(const V *g, long long count, long long at, long long threads) {
   constexpr int E = 16 / sizeof(V);
   using Vec = __attribute__((ext_vector_type(E))) V;
   typedef Vec Loose __attribute__((aligned(sizeof(V))));  // a matrix of the batch may start at any element
-  __shared__ double scratch[4];
   double s = 0;
-  const V *g = in + blockIdx.y * count;
-  const long long step = 256LL * gridDim.x, vectors = count / E;
+  const long long vectors = count / E;
 #pragma unroll 4
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < vectors; i += step) {
+  for (long long i = at; i < vectors; i += threads) {
     const Vec v = *reinterpret_cast<const Loose *>(g + i * E);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
@@ -440,11 +413,18 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long cou
       s += x * x;
     }
   }
-  const long long last = vectors * E + threadIdx.x;
-  if (blockIdx.x == 0 && last < count) {
-    const double x = static_cast<double>(static_cast<float>(g[last]));
+  if (vectors * E + at < count) {  // fewer than E values are left: one each for the first threads
+    const double x = static_cast<double>(static_cast<float>(g[vectors * E + at]));
     s += x * x;
   }
+  return s;
+}
+
+// sums of squares, gridDim.x partial sums per matrix
+template <typename V>
+__global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long count, double *partials) {
+  __shared__ double scratch[4];
+  double s = sum_of_squares(in + blockIdx.y * count, count, blockIdx.x * 256LL + threadIdx.x, 256LL * gridDim.x);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = s;
@@ -514,137 +494,230 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n,
 // X, X^T, A and B stay in LDS (rows padded by 16 bytes: an odd number of 16-byte chunks, so that 16 rows' equal chunks meet
 // every bank once); 16 waves share the 16 x 16 x 32 tiles of each product.  The update holds its tiles in registers over a
 // barrier and then overwrites X and X^T.  What bounds it is the chain of 3 x steps dependent products, not their rate.
-constexpr int kSmallWaves = 16, kSmallTiles = 10;  // tiles of X a wave holds at most (the LDS limit keeps r c <= 160 x 256)
+// LDS is addressed by plain offsets into one array: through pointers that are chosen at run time the compiler cannot see that
+// they are LDS, and flat accesses and spills made a step of 64 x 64 f32 3.9 us long (1.5 now).
+constexpr int kSmallWaves = 16;
 constexpr long long kSmallLds = 160 * 1024 - 256;
 
-inline long long small_lds(int rp, int cp, int terms) {
-  return 2LL * terms * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8) + 2LL * rp * (rp + 8));
+inline long long small_lds(int rp, int cp, int tx) {
+  if (rp > 64 && rp / 32 * (cp / 32) > kSmallWaves) return kSmallLds + 1;  // more blocks of 32 x 32 than waves: see launch_small
+  return 2LL * tx * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8)) + 8LL * rp * (rp + 8);
 }
 
 struct SmallArgs {
   const void *in;
   void *out;
-  int dtype, m, n, r, c, rp, cp, steps, tall;
+  int m, n, r, c, rp, cp, steps, tall;
   float a, b, k, eps;
 };
 
-template <int TERMS>
+// SIDE: the products are formed in blocks of 16 x 16 (one instruction tile: the shortest chain, and enough blocks of A for the
+// waves up to 64 rows) or 32 x 32 (two fragments of each side for four tiles: half the LDS reads).  us for 5 steps: 17 x 300 f32
+// 20 at 16, 32 at 32; 64 x 400 bf16 35, 38; 128 x 128 bf16 40, 34.
+// COLUMN = 0: X has no more blocks than there are waves; a block is held over a barrier before it overwrites X.
+// COLUMN > 0: a wave takes columns of blocks, which depend on nothing but themselves: held, COLUMN of them at most, without a
+// barrier, their X^T fragments read once (64 x 400 bf16: blocks dealt out, held and written by straight code 51 us, half of
+// them its instruction fetches; by columns 35).
+template <typename V, int SIDE, int COLUMN>
 __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
   __shared__ double parts[kSmallWaves];
-  constexpr bool two = TERMS == 2;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ldx = a.cp + 8, ldr = a.rp + 8;  // X: rp rows of ldx; X^T: cp rows of ldr; A, B: rp rows of ldr
-  _Float16 *at = reinterpret_cast<_Float16 *>(lds);
-  auto take = [&](int values) {
-    Terms t;
-    t.hi = at;
-    t.lo = at + values;
-    at += TERMS * values;
-    return t;
+  // each array: its first terms, then its second ones
+  const int sx = a.rp * ldx, st = a.cp * ldr, sa = a.rp * ldr;
+  constexpr int TX = std::is_same<V, __bf16>::value ? 1 : 2;  // terms of X; A and B have two
+  using Two = std::integral_constant<int, 2>;
+  using OfX = std::integral_constant<int, TX>;
+  const int X = 0, XT = X + TX * sx, A = XT + TX * st, B = A + 2 * sa;
+  auto put1 = [&](int at, int size, float v) {
+    const _Float16 h = static_cast<_Float16>(v);
+    lds[at] = h;
+    if (TX == 2) lds[at + size] = static_cast<_Float16>(v - static_cast<float>(h));
   };
-  const Terms X = take(a.rp * ldx), XT = take(a.cp * ldr), A = take(a.rp * ldr), B = take(a.rp * ldr);
+  // four consecutive rows of a column: into the row of the transpose (`turned`) and, if wanted, into four rows (`at`, ld apart)
+  auto put4 = [&](auto terms, int turned, int turned_size, int at, int ld, int size, bool both, f32x4 v) {
+    constexpr bool two = decltype(terms)::value == 2;
+    f16x4 h, l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[k] = static_cast<_Float16>(v[k]);
+      l[k] = static_cast<_Float16>(v[k] - static_cast<float>(h[k]));
+    }
+    *reinterpret_cast<f16x4 *>(lds + turned) = h;
+    if (two) *reinterpret_cast<f16x4 *>(lds + turned + turned_size) = l;
+    if (both) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        lds[at + k * ld] = h[k];
+        if (two) lds[at + k * ld + size] = l[k];
+      }
+    }
+  };
   const int count = a.m * a.n;
-  const long long base = blockIdx.x * static_cast<long long>(count);
-  double s = 0;
-  for (int i = tid; i < count; i += kSmallWaves * 64) {
-    const double v = get_in(a.in, a.dtype, base + i);
-    s += v * v;
-  }
+  const V *in = static_cast<const V *>(a.in) + blockIdx.x * static_cast<long long>(count);
+  double s = sum_of_squares(in, count, tid, kSmallWaves * 64);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if (lane == 0) parts[wave] = s;
   __syncthreads();
   s = 0;
+#pragma unroll
   for (int i = 0; i < kSmallWaves; ++i) s += parts[i];
   const double factor = kScaleX / (sqrt(s) + a.eps);
-  for (int i = tid; i < a.rp * a.cp; i += kSmallWaves * 64) {
-    const int row = i / a.cp, col = i - row * a.cp;
-    float v = 0.f;
-    if (row < a.r && col < a.c) v = static_cast<float>(get_in(a.in, a.dtype, base + (a.tall ? col * a.n + row : row * a.n + col)) * factor);
-    put_terms(X, row * ldx + col, v, two);
-    put_terms(XT, col * ldr + row, v, two);
-  }
-  __syncthreads();
-  const int l15 = lane & 15, quad = lane >> 4;
-  // acc = P[16 rows from pm] Q[16 rows from qn]^T; accumulator e of a lane: row 4 (lane / 16) + e, column lane % 16
-  auto product = [&](const Terms &P, int ldp, int pm, const Terms &Q, int ldq, int qn, int K) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    const int po = (pm + l15) * ldp + quad * 8, qo = (qn + l15) * ldq + quad * 8;
-    for (int k = 0; k < K; k += 32) {
-      const f16x8 ph = *reinterpret_cast<const f16x8 *>(P.hi + po + k), qh = *reinterpret_cast<const f16x8 *>(Q.hi + qo + k);
-      if (two) {
-        const f16x8 pl = *reinterpret_cast<const f16x8 *>(P.lo + po + k), ql = *reinterpret_cast<const f16x8 *>(Q.lo + qo + k);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, acc, 0, 0, 0);
+  for (int row = wave; row < a.rp; row += kSmallWaves)  // a wave per row of X, 256 columns' loads at a time
+    for (int col0 = lane; col0 < a.cp; col0 += 256) {
+      V g[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int col = min(col0 + 64 * k, a.c - 1), from = min(row, a.r - 1);
+        g[k] = in[a.tall ? col * a.n + from : from * a.n + col];
       }
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int col = col0 + 64 * k;
+        if (col >= a.cp) continue;
+        const float v = row < a.r && col < a.c ? static_cast<float>(static_cast<float>(g[k]) * factor) : 0.f;
+        put1(X + row * ldx + col, sx, v);
+        put1(XT + col * ldr + row, st, v);
+      }
     }
-    return acc;
+  __syncthreads();
+  // acc[i] = rows SIDE i .. of P times SIDE rows of Q transposed, the first `count` of N blocks.  Accumulator e of a lane and
+  // 16 x 16 tile: row 4 (lane / 16) + e, column lane % 16
+  constexpr int F = SIDE / 16, kHeld = COLUMN > 0 ? COLUMN : 1;
+  struct Block { f32x4 v[F][F]; };
+  auto products = [&](auto pt, auto qt, auto &acc, int count, int P, int ldp, int sp, int Q, int ldq, int sq, int K) {
+    constexpr int N = sizeof(acc) / sizeof(Block);
+    constexpr bool p2 = decltype(pt)::value == 2, q2 = decltype(qt)::value == 2;
+    Block cross[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      acc[i] = Block{};
+      cross[i] = Block{};
+    }
+    const int po = P + l15 * ldp + quad * 8, qo = Q + l15 * ldq + quad * 8;
+#pragma unroll 1
+    for (int k = 0; k < K; k += 32) {
+      f16x8 qh[F], ql[F];
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        qh[f] = *reinterpret_cast<const f16x8 *>(lds + qo + f * 16 * ldq + k);
+        if (q2) ql[f] = *reinterpret_cast<const f16x8 *>(lds + qo + f * 16 * ldq + sq + k);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (N > 1 && i >= count) continue;
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const int at = po + (i * SIDE + f * 16) * ldp + k;
+          const f16x8 ph = *reinterpret_cast<const f16x8 *>(lds + at);
+          f16x8 pl;
+          if (p2) pl = *reinterpret_cast<const f16x8 *>(lds + at + sp);
+#pragma unroll
+          for (int g = 0; g < F; ++g) {
+            acc[i].v[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh[g], acc[i].v[f][g], 0, 0, 0);
+            f32x4 &c = cross[i].v[f][g];  // (a sum of its own: dependent instructions issue at half the rate)
+            if (p2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh[g], c, 0, 0, 0);
+            if (q2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql[g], c, 0, 0, 0);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int g = 0; g < F; ++g) acc[i].v[f][g] += cross[i].v[f][g];
   };
-  const int tr = a.rp / 16, tc = a.cp / 16;
+  const int tr = a.rp / SIDE, tc = a.cp / SIDE, upper = tr * (tr + 1) / 2;
+#pragma unroll 1
   for (int step = 0; step < a.steps; ++step) {
-    for (int half = 0; half < 2; ++half) {  // A = X X^T, then B = a I + b A + c A A: upper triangles, stored twice
-      for (int tile = wave; tile < tr * (tr + 1) / 2; tile += kSmallWaves) {
+    // A = X X^T, then B = a I + b A + c A A: their upper triangles, stored twice
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      const int to = half ? B : A;
+#pragma unroll 1
+      for (int tile = wave; tile < upper; tile += kSmallWaves) {
         int left = tile, row = 0;
         while (left >= tr - row) left -= tr - row++;
-        const int pm = row * 16, qn = (row + left) * 16;
-        const f32x4 acc = half ? product(A, ldr, pm, A, ldr, qn, a.rp) : product(X, ldx, pm, X, ldx, qn, a.cp);
-        const int m = pm + 4 * quad, n = qn + l15;
-        float v[4];
-        if (half) {
-          const f16x4 h = *reinterpret_cast<const f16x4 *>(A.hi + n * ldr + m);
-          f16x4 l = {0, 0, 0, 0};
-          if (two) l = *reinterpret_cast<const f16x4 *>(A.lo + n * ldr + m);
+        const int pm = row * SIDE, qn = (row + left) * SIDE;
+        Block acc[1];
+        if (half) products(Two{}, Two{}, acc, 1, A + pm * ldr, ldr, sa, A + qn * ldr, ldr, sa, a.rp);
+        else products(OfX{}, OfX{}, acc, 1, X + pm * ldx, ldx, sx, X + qn * ldx, ldx, sx, a.cp);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            v[k] = a.k * (acc[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(h[k]) + static_cast<float>(l[k])) + (m + k == n ? a.a * kScaleA : 0.f);
-        } else {
+        for (int f = 0; f < F; ++f)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = acc[k] * (kScaleA / (kScaleX * kScaleX));
-        }
-        const Terms &D = half ? B : A;
-        put_terms4(D, n * ldr + m, v, two);
-        if (pm != qn)
+          for (int g = 0; g < F; ++g) {
+            const int m = pm + f * 16 + 4 * quad, n = qn + g * 16 + l15;
+            f32x4 v = acc[0].v[f][g] * (half ? a.k / kScaleA : kScaleA / (kScaleX * kScaleX));
+            if (half) {
+              const f16x4 h = *reinterpret_cast<const f16x4 *>(lds + A + n * ldr + m);
+              const f16x4 l = *reinterpret_cast<const f16x4 *>(lds + A + n * ldr + m + sa);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) put_terms(D, (m + k) * ldr + n, v[k], two);
+              for (int k = 0; k < 4; ++k) v[k] += a.b * (static_cast<float>(h[k]) + static_cast<float>(l[k])) + (m + k == n ? a.a * kScaleA : 0.f);
+            }
+            put4(Two{}, to + n * ldr + m, sa, to + m * ldr + n, ldr, sa, pm != qn, v);
+          }
       }
       __syncthreads();
     }
-    f32x4 held[kSmallTiles];
-#pragma unroll
-    for (int i = 0; i < kSmallTiles; ++i) {
-      const int tile = wave + i * kSmallWaves;
-      if (tile < tr * tc) held[i] = product(B, ldr, tile % tr * 16, XT, ldr, tile / tr * 16, a.rp);
-    }
-    __syncthreads();
     const bool last = step + 1 == a.steps;
+    auto put_block = [&](int tm, int tn, const Block &b) {
 #pragma unroll
-    for (int i = 0; i < kSmallTiles; ++i) {
-      const int tile = wave + i * kSmallWaves;
-      if (tile >= tr * tc) continue;
-      const int m = tile % tr * 16 + 4 * quad, n = tile / tr * 16 + l15;
-      float v[4];
+      for (int f = 0; f < F; ++f)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = held[i][k] * (1.f / kScaleA);
-      if (last) {
+        for (int g = 0; g < F; ++g) {
+          const int m = tm * SIDE + f * 16 + 4 * quad, n = tn * SIDE + g * 16 + l15;
+          const f32x4 v = b.v[f][g] * (1.f / kScaleA);
+          if (!last) {
+            put4(OfX{}, XT + n * ldr + m, st, X + m * ldx + n, ldx, sx, true, v);
+          } else {
+            V *out = static_cast<V *>(a.out) + blockIdx.x * static_cast<long long>(count);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (m + k < a.r && n < a.c)
-            put_out(a.out, a.dtype, base + (a.tall ? n * a.n + m + k : (m + k) * a.n + n), v[k] * (1.f / kScaleX));
-      } else {
-        put_terms4(XT, n * ldr + m, v, two);
+            for (int k = 0; k < 4; ++k)
+              if (m + k < a.r && n < a.c) out[a.tall ? n * a.n + m + k : (m + k) * a.n + n] = static_cast<V>(v[k] * (1.f / kScaleX));
+          }
+        }
+    };
+    Block held[kHeld];
+    if constexpr (COLUMN == 0) {
+      if (wave < tr * tc) products(Two{}, OfX{}, held, 1, B + wave % tr * SIDE * ldr, ldr, sa, XT + wave / tr * SIDE * ldr, ldr, st, a.rp);
+      __syncthreads();
+      if (wave < tr * tc) put_block(wave % tr, wave / tr, held[0]);
+    } else {
+#pragma unroll 1
+      for (int tn = wave; tn < tc; tn += kSmallWaves) {
+        products(Two{}, OfX{}, held, tr, B, ldr, sa, XT + tn * SIDE * ldr, ldr, st, a.rp);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) put_terms(X, (m + k) * ldx + n, v[k], two);
+        for (int i = 0; i < COLUMN; ++i)
+          if (i < tr) put_block(i, tn, held[i]);
       }
     }
     __syncthreads();
   }
 }
 
+template <typename V, int SIDE, int COLUMN>
+int launch_small_as(const SmallArgs &q, int batch, int bytes, hipStream_t s) {
+  DX_LDS_OPT_IN((ns_small_kernel<V, SIDE, COLUMN>), kSmallLds);
+  hipLaunchKernelGGL((ns_small_kernel<V, SIDE, COLUMN>), dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
+  DX_LAUNCH_CHECK();
+  return DX_OK;
+}
+template <typename V>
+int launch_small(const SmallArgs &q, int batch, int bytes, hipStream_t s) {
+  const int blocks = q.rp / 32 * (q.cp / 32);
+  if (blocks * 4 <= kSmallWaves) return launch_small_as<V, 16, 0>(q, batch, bytes, s);
+  if (q.rp <= 32) return launch_small_as<V, 16, 2>(q, batch, bytes, s);
+  if (q.rp <= 64) return launch_small_as<V, 16, 4>(q, batch, bytes, s);
+  return launch_small_as<V, 32, 0>(q, batch, bytes, s);
+}
+
 struct Plan {
-  int r, c, rp, cp, terms, parts;
+  int r, c, rp, cp, tx, ta, parts;  // tx, ta: terms of X, of A and B
   long long x, sq;             // values of X and of A per matrix, padded
   long long bytes;
 };
@@ -654,13 +727,14 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   p.c = m < n ? n : m;
   p.rp = (p.r + kPad - 1) / kPad * kPad;
   p.cp = (p.c + kPad - 1) / kPad * kPad;
-  p.terms = dtype == DX_F32 ? 2 : 1;
+  p.tx = dtype == DX_BF16 ? 1 : 2;
+  p.ta = dtype == DX_BF16 && p.r > kOneTermRows ? 1 : 2;
   p.x = static_cast<long long>(p.rp) * p.cp;
   p.sq = static_cast<long long>(p.rp) * p.rp;
   // X, two copies of X^T, A, B, and the norm's partial sums
   const long long blocks = (static_cast<long long>(m) * n + 8191) / 8192;  // 8192 elements a workgroup at least
   p.parts = static_cast<int>(blocks < kNormParts ? blocks : kNormParts);
-  p.bytes = batch * (p.terms * 2 * (3 * p.x + 2 * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4LL * kSplitGroups * 64 * 64;
+  p.bytes = batch * (2 * (3 * p.tx * p.x + 2 * p.ta * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4LL * kSplitGroups * 64 * 64;
   return p;
 }
 int check_shape(int dtype, int batch, int m, int n) {
@@ -670,16 +744,16 @@ int check_shape(int dtype, int batch, int m, int n) {
   return DX_OK;
 }
 
-template <int TM, int WR, int WC, int TERMS, int RING, Epilogue EPI>
+template <int TM, int WR, int WC, int PT, int QT, int OT, int RING, Epilogue EPI>
 int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
-  constexpr int bytes = RING * 2 * TERMS * TM * kBK * 2;
-  DX_LDS_OPT_IN((ns_gemm_kernel<TM, WR, WC, TERMS, RING, EPI>), bytes);
+  constexpr int bytes = RING * (PT + QT) * TM * kBK * 2;
+  DX_LDS_OPT_IN((ns_gemm_kernel<TM, WR, WC, PT, QT, OT, RING, EPI>), bytes);
   a.tiles_m = cdiv(a.rows_p, TM);
   a.tiles_n = cdiv(a.rows_q, TM);
   const int tiles = EPI == GRAM || EPI == POLY ? a.tiles_m * (a.tiles_m + 1) / 2 : a.tiles_m * a.tiles_n;
   a.split_stages = cdiv(a.K / kBK, splits);
   a.splits = cdiv(a.K / kBK, a.split_stages);
-  hipLaunchKernelGGL((ns_gemm_kernel<TM, WR, WC, TERMS, RING, EPI>), dim3(tiles * a.splits, batch), dim3(WR * WC * 64), bytes, s, a);
+  hipLaunchKernelGGL((ns_gemm_kernel<TM, WR, WC, PT, QT, OT, RING, EPI>), dim3(tiles * a.splits, batch), dim3(WR * WC * 64), bytes, s, a);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
@@ -690,9 +764,9 @@ int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
 // X X^T of a wide matrix has few tiles and a long K: K is split until the CUs are busy, where that saves more than the 4 us
 // that the exchange of the sums takes: 512 x 3136 f32 (36 tiles, 49 stages of 0.45 us) 276 us in one piece, 224 in seven;
 // 128 x 1000 bf16 (3 tiles, 16 stages of 0.2 us) 85 against 89 in four.
-template <int TERMS, Epilogue EPI>
+template <int PT, int QT, int OT, Epilogue EPI>
 int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
-  constexpr bool half = EPI == GRAM || EPI == POLY;
+  constexpr bool half = EPI == GRAM || EPI == POLY, single = PT + QT + OT == 3;
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   auto tiles = [&](int tile) {
@@ -700,22 +774,23 @@ int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
     return (half ? m * (m + 1) / 2 : m * n) * batch;
   };
   int best = 64;
-  for (int tile = 128; tile <= (TERMS == 1 ? 256 : 128); tile += 64)
+  for (int tile = 128; tile <= (single ? 256 : 128); tile += 64)
     if ((tiles(tile) + cus - 1) / cus * tile < (tiles(best) + cus - 1) / cus * best) best = tile;
-  if constexpr (TERMS == 1) {
-    if (best == 256) return launch_tile<256, 2, 4, 1, 2, EPI>(a, batch, 1, s);
-    if (best == 192) return launch_tile<192, 2, 2, 1, 3, EPI>(a, batch, 1, s);
+  if constexpr (single) {
+    if (best == 256) return launch_tile<256, 2, 4, 1, 1, 1, 2, EPI>(a, batch, 1, s);
+    if (best == 192) return launch_tile<192, 2, 2, 1, 1, 1, 3, EPI>(a, batch, 1, s);
   }
-  if (best == 128) return launch_tile<128, 2, 2, TERMS, 2, EPI>(a, batch, 1, s);
+  if (best == 128) return launch_tile<128, 2, 2, PT, QT, OT, 2, EPI>(a, batch, 1, s);
   long long splits = 1;
-  if (EPI == GRAM && a.K / kBK >= (TERMS == 2 ? 16 : 32)) {
+  if (EPI == GRAM && a.K / kBK >= (PT == 2 ? 16 : 32)) {
     splits = (cus < kSplitGroups ? cus : kSplitGroups) / tiles(64);
     if (splits > a.K / kBK / 6) splits = a.K / kBK / 6;
     if (splits < 1) splits = 1;
   }
-  return launch_tile<64, 2, 2, TERMS, 4, EPI>(a, batch, static_cast<int>(splits), s);
+  return launch_tile<64, 2, 2, PT, QT, OT, 4, EPI>(a, batch, static_cast<int>(splits), s);
 }
-template <int TERMS>
+// TX: terms of X, TA: of A and B
+template <int TX, int TA>
 int run_steps(const Plan &p, int batch, int steps, NsArgs a, Terms X, Terms XT0, Terms XT1, Terms A, Terms B, hipStream_t s) {
   for (int k = 0; k < steps; ++k) {
     const Terms xt = k & 1 ? XT1 : XT0, next = k & 1 ? XT0 : XT1;
@@ -727,12 +802,12 @@ int run_steps(const Plan &p, int batch, int steps, NsArgs a, Terms X, Terms XT0,
     g.D = g.DT = A;
     g.d_stride = g.dt_stride = p.sq;
     g.ldd = g.lddt = p.rp;
-    if (int rc = launch_gemm<TERMS, GRAM>(g, batch, s)) return rc;
+    if (int rc = launch_gemm<TX, TX, TA, GRAM>(g, batch, s)) return rc;
     g.P = g.Q = A;
     g.p_stride = g.q_stride = p.sq;
     g.ldp = g.ldq = g.K = p.rp;
     g.D = g.DT = B;
-    if (int rc = launch_gemm<TERMS, POLY>(g, batch, s)) return rc;
+    if (int rc = launch_gemm<TA, TA, TA, POLY>(g, batch, s)) return rc;
     g.P = B;
     g.Q = xt;
     g.q_stride = p.x;
@@ -741,7 +816,7 @@ int run_steps(const Plan &p, int batch, int steps, NsArgs a, Terms X, Terms XT0,
     g.DT = next;
     g.d_stride = g.dt_stride = p.x;
     g.ldd = p.cp;
-    if (int rc = k + 1 < steps ? launch_gemm<TERMS, UPDATE>(g, batch, s) : launch_gemm<TERMS, FINAL>(g, batch, s)) return rc;
+    if (int rc = k + 1 < steps ? launch_gemm<TA, TX, TX, UPDATE>(g, batch, s) : launch_gemm<TA, TX, TX, FINAL>(g, batch, s)) return rc;
   }
   return DX_OK;
 }
@@ -768,29 +843,24 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   const Plan p = make_plan(dtype, batch, m, n);
   if (workspace_bytes < p.bytes) return fail(DX_EWS, "dx_orthogonalize: workspace of %lld bytes, %lld needed", workspace_bytes, p.bytes);
   hipStream_t s = as_stream(stream);
-  if (small_lds(p.rp, p.cp, p.terms) <= kSmallLds) {
-    const SmallArgs q{update, out, dtype, m, n, p.r, p.c, p.rp, p.cp, steps, m > n, a, b, c, eps};
-    const int bytes = static_cast<int>(small_lds(p.rp, p.cp, p.terms));
-    if (p.terms == 2) {
-      DX_LDS_OPT_IN(ns_small_kernel<2>, kSmallLds);
-      hipLaunchKernelGGL(ns_small_kernel<2>, dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
-    } else {
-      DX_LDS_OPT_IN(ns_small_kernel<1>, kSmallLds);
-      hipLaunchKernelGGL(ns_small_kernel<1>, dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
-    }
-    DX_LAUNCH_CHECK();
-    return DX_OK;
+  if (small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32, p.tx) <= kSmallLds) {
+    const int r32 = cdiv(p.r, 32) * 32, c32 = cdiv(p.c, 32) * 32;
+    const SmallArgs q{update, out, m, n, p.r, p.c, r32, c32, steps, m > n, a, b, c, eps};
+    const int bytes = static_cast<int>(small_lds(r32, c32, p.tx));
+    if (dtype == DX_F32) return launch_small<float>(q, batch, bytes, s);
+    if (dtype == DX_BF16) return launch_small<__bf16>(q, batch, bytes, s);
+    return launch_small<_Float16>(q, batch, bytes, s);
   }
   _Float16 *at = static_cast<_Float16 *>(workspace);
-  auto take = [&](long long values) {
+  auto take = [&](long long values, int terms) {
     Terms t;
     t.hi = at;
     at += values * batch;
     t.lo = at;
-    if (p.terms == 2) at += values * batch;
+    if (terms == 2) at += values * batch;
     return t;
   };
-  const Terms X = take(p.x), XT0 = take(p.x), XT1 = take(p.x), A = take(p.sq), B = take(p.sq);
+  const Terms X = take(p.x, p.tx), XT0 = take(p.x, p.tx), XT1 = take(p.x, p.tx), A = take(p.sq, p.ta), B = take(p.sq, p.ta);
   double *partials = reinterpret_cast<double *>(at);
   unsigned *arrivals = reinterpret_cast<unsigned *>(partials + static_cast<long long>(batch) * p.parts);
   float *split = reinterpret_cast<float *>(arrivals + kSplitGroups);
@@ -810,7 +880,7 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
     hipLaunchKernelGGL((ns_pack_kernel<__bf16, false>), grid, dim3(256), 0, s, static_cast<const __bf16 *>(update), m, n, partials, p.parts, eps,
                        same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   else
-    hipLaunchKernelGGL((ns_pack_kernel<_Float16, false>), grid, dim3(256), 0, s, static_cast<const _Float16 *>(update), m, n, partials, p.parts,
+    hipLaunchKernelGGL((ns_pack_kernel<_Float16, true>), grid, dim3(256), 0, s, static_cast<const _Float16 *>(update), m, n, partials, p.parts,
                        eps, same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   DX_LAUNCH_CHECK();
   NsArgs g{};
@@ -824,5 +894,6 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   g.r = p.r;
   g.cols = p.c;
   g.tall = tall;
-  return p.terms == 2 ? run_steps<2>(p, batch, steps, g, X, XT0, XT1, A, B, s) : run_steps<1>(p, batch, steps, g, X, XT0, XT1, A, B, s);
+  if (p.tx == 2) return run_steps<2, 2>(p, batch, steps, g, X, XT0, XT1, A, B, s);
+  return p.ta == 2 ? run_steps<1, 2>(p, batch, steps, g, X, XT0, XT1, A, B, s) : run_steps<1, 1>(p, batch, steps, g, X, XT0, XT1, A, B, s);
 }

@@ -21,11 +21,13 @@ typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.402823466e+38f;
+constexpr int kMaxPieces = 512;    // pieces of rows, where few rows are cut
 constexpr int kMaxWorkers = 2048;  // workgroups of a row kernel = rows of `partials` (8 doubles each)
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 struct ElemF32 {
+  static constexpr uint32_t kNegInf = 0;  // (unused: a word is an element)
   using Store = float;
   using Vec = u32x4_a4;
   static constexpr int E = 4;
@@ -46,6 +48,7 @@ struct ElemF32 {
   static __device__ __forceinline__ Store put(float x) { return x; }
 };
 struct ElemBF16 {
+  static constexpr uint32_t kNegInf = 0xff80u;
   using Store = __bf16;
   using Vec = u32x4_a2;
   static constexpr int E = 8;
@@ -71,6 +74,7 @@ struct ElemBF16 {
   static __device__ __forceinline__ Store put(float x) { return static_cast<__bf16>(x); }
 };
 struct ElemF16 {
+  static constexpr uint32_t kNegInf = 0xfc00u;
   using Store = _Float16;
   using Vec = u32x4_a2;
   static constexpr int E = 8;
@@ -97,20 +101,39 @@ struct ElemF16 {
   static __device__ __forceinline__ Store put(float x) { return static_cast<_Float16>(x); }
 };
 
-// E elements of a row from column `first` on; columns at or past V read as -inf
+// Rows are walked in chunks of T threads x E columns.  `at` is the chunk's address (uniform), t its thread, `first` the
+// thread's column; `ragged` (uniform): the chunk passes the row's end.  There a thread reads the row's LAST E columns instead
+// (one vector load as everywhere else: element loads would have to be waited for on the spot, and with them every load in
+// flight before them), and unpack_raw moves them to their places; columns past the end are -inf.
 template <class D>
-__device__ __forceinline__ u32x4 load_vec(const char *row, int first, int V) {
-  if (first + D::E <= V) return *reinterpret_cast<const typename D::Vec *>(row + static_cast<long long>(first) * sizeof(typename D::Store));
-  float x[D::E];
+__device__ __forceinline__ u32x4 load_raw(const char *row, const char *at, int t, int first, int V, bool ragged) {
+  using Store = typename D::Store;
+  if (!ragged) return *reinterpret_cast<const typename D::Vec *>(at + static_cast<uint32_t>(t) * 16);
+  if (V >= D::E) return *reinterpret_cast<const typename D::Vec *>(row + static_cast<long long>(min(first, V - D::E)) * sizeof(Store));
+  float x[D::E];  // rows shorter than a vector
 #pragma unroll
-  for (int k = 0; k < D::E; ++k)
-    x[k] = first + k < V ? D::get(reinterpret_cast<const typename D::Store *>(row)[first + k]) : -INFINITY;
+  for (int k = 0; k < D::E; ++k) x[k] = first + k < V ? D::get(reinterpret_cast<const Store *>(row)[first + k]) : -INFINITY;
   return D::pack(x);  // exact: the values came from this type
 }
 template <class D>
-__device__ __forceinline__ void store_vec(char *row, int first, int V, const float (&x)[D::E]) {
-  if (first + D::E <= V) {
-    *reinterpret_cast<typename D::Vec *>(row + static_cast<long long>(first) * sizeof(typename D::Store)) = D::pack(x);
+__device__ __forceinline__ void unpack_raw(u32x4 v, float (&x)[D::E], int first, int V, bool ragged) {
+  D::unpack(v, x);
+  if (!ragged || V < D::E) return;
+  const int shift = max(0, first - (V - D::E));
+#pragma unroll
+  for (int b = 1; b < D::E; b *= 2)
+#pragma unroll
+    for (int k = 0; k < D::E; ++k) {
+      const float other = k + b < D::E ? x[k + b] : -INFINITY;
+      x[k] = shift & b ? other : x[k];
+    }
+#pragma unroll
+  for (int k = 0; k < D::E; ++k) x[k] = shift < D::E ? x[k] : -INFINITY;
+}
+template <class D>
+__device__ __forceinline__ void store_chunk(char *row, char *at, int t, int first, int V, bool ragged, const float (&x)[D::E]) {
+  if (!ragged || first + D::E <= V) {
+    *reinterpret_cast<typename D::Vec *>(at + static_cast<uint32_t>(t) * 16) = D::pack(x);
     return;
   }
 #pragma unroll
@@ -147,16 +170,12 @@ __device__ __forceinline__ void raise_ref(RowStats &r, float x) {
 }
 
 template <class D, bool REF>
-__device__ __forceinline__ void add_vec(RowStats &r, u32x4 v, u32x4 w) {
-  float x[D::E];
-  D::unpack(v, x);
+__device__ __forceinline__ void add_vec(RowStats &r, const float (&x)[D::E], const float (&q)[D::E]) {
   float mx = x[0];
 #pragma unroll
   for (int k = 1; k < D::E; ++k) mx = fmaxf(mx, x[k]);
   if (mx > r.m) raise_max(r, mx);
-  float q[D::E];
   if constexpr (REF) {
-    D::unpack(w, q);
     float mq = q[0];
 #pragma unroll
     for (int k = 1; k < D::E; ++k) mq = fmaxf(mq, q[k]);
@@ -174,6 +193,99 @@ __device__ __forceinline__ void add_vec(RowStats &r, u32x4 v, u32x4 w) {
   }
 }
 
+// a column's terms, or a vector's, under maxima that are known already (r.m, r.mr)
+template <bool REF>
+__device__ __forceinline__ void add_term(RowStats &r, float x, float q) {
+  const float d = x - r.m, e = exp_of(d);
+  r.s += e;
+  r.ed += e * fmaxf(d, kLowest);
+  if constexpr (REF) {
+    r.sr += exp_of(q - r.mr);
+    r.gap += gap_term(e, x, q);
+  }
+}
+template <class D, bool REF>
+__device__ __forceinline__ void add_terms(RowStats &r, const float (&x)[D::E], const float (&q)[D::E]) {
+#pragma unroll
+  for (int k = 0; k < D::E; ++k) add_term<REF>(r, x[k], REF ? q[k] : 0.f);
+}
+
+// columns begin .. end of a row (begin and, but for the row's end, end are multiples of a chunk) added to this thread's statistics
+template <class D, int T, bool REF>
+__device__ __forceinline__ void add_columns(RowStats &r, const char *z, const char *q, int V, int begin, int end, int t) {
+  constexpr int C = T * D::E, U = 4;
+  int base = begin;
+  for (; base + U * C <= end; base += U * C) {
+    u32x4 v[U], u[REF ? U : 1];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const long long at = static_cast<long long>(base + k * C) * sizeof(typename D::Store);
+      v[k] = load_raw<D>(z, z + at, t, 0, V, false);
+      if constexpr (REF) u[k] = load_raw<D>(q, q + at, t, 0, V, false);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      float x[D::E], y[D::E];
+      D::unpack(v[k], x);
+      if constexpr (REF) D::unpack(u[k], y);
+      add_vec<D, REF>(r, x, y);
+    }
+  }
+  for (; base < end; base += C) {
+    const bool ragged = base + C > V;
+    const int first = base + t * D::E;
+    if (first >= V) break;
+    const long long at = static_cast<long long>(base) * sizeof(typename D::Store);
+    float x[D::E], y[D::E];
+    unpack_raw<D>(load_raw<D>(z, z + at, t, first, V, ragged), x, first, V, ragged);
+    if constexpr (REF) unpack_raw<D>(load_raw<D>(q, q + at, t, first, V, ragged), y, first, V, ragged);
+    add_vec<D, REF>(r, x, y);
+  }
+}
+// dz of columns begin .. end from `value(x, y, column)`; `read` false: zeros, nothing is read
+template <class D, int T, bool REF, class F>
+__device__ __forceinline__ void write_columns(const char *z, const char *q, char *dz, int V, int begin, int end, int t, bool read, F value) {
+  constexpr int C = T * D::E, U = 2;
+  int base = begin;
+  for (; base + U * C <= end; base += U * C) {
+    u32x4 v[U], u[REF ? U : 1];
+    if (read) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const long long at = static_cast<long long>(base + k * C) * sizeof(typename D::Store);
+        v[k] = load_raw<D>(z, z + at, t, 0, V, false);
+        if constexpr (REF) u[k] = load_raw<D>(q, q + at, t, 0, V, false);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int first = base + k * C + t * D::E;
+      float x[D::E] = {}, y[D::E];
+      if (read) {
+        D::unpack(v[k], x);
+        if constexpr (REF) D::unpack(u[k], y);
+#pragma unroll
+        for (int i = 0; i < D::E; ++i) x[i] = value(x[i], REF ? y[i] : 0.f, first + i);
+      }
+      store_chunk<D>(dz, dz + static_cast<long long>(base + k * C) * sizeof(typename D::Store), t, first, V, false, x);
+    }
+  }
+  for (; base < end; base += C) {
+    const bool ragged = base + C > V;
+    const int first = base + t * D::E;
+    if (first >= V) break;
+    const long long at = static_cast<long long>(base) * sizeof(typename D::Store);
+    float x[D::E] = {}, y[D::E];
+    if (read) {
+      unpack_raw<D>(load_raw<D>(z, z + at, t, first, V, ragged), x, first, V, ragged);
+      if constexpr (REF) unpack_raw<D>(load_raw<D>(q, q + at, t, first, V, ragged), y, first, V, ragged);
+#pragma unroll
+      for (int i = 0; i < D::E; ++i) x[i] = value(x[i], REF ? y[i] : 0.f, first + i);
+    }
+    store_chunk<D>(dz, dz + at, t, first, V, ragged, x);
+  }
+}
+
 // the statistics of all lanes of a wave joined, in every lane
 template <bool REF>
 __device__ __forceinline__ void join_wave(RowStats &r) {
@@ -184,6 +296,22 @@ __device__ __forceinline__ void join_wave(RowStats &r) {
     raise_ref(r, wave_max_all(r.mr));
     r.sr = wave_sum_all(r.sr);
     r.gap = wave_sum_all(r.gap);
+  }
+}
+constexpr RowStats kNothing = {kLowest, 0.f, 0.f, 0.f, kLowest, 0.f};
+
+// joined over the W waves that share a row; `parts`: two sets of W, used in turn (one barrier a row)
+template <int W, bool REF>
+__device__ __forceinline__ void join_row(RowStats &r, RowStats (&parts)[2][W], int &turn) {
+  join_wave<REF>(r);
+  if constexpr (W > 1) {
+    const int lane = threadIdx.x & 63;
+    if (lane == 0) parts[turn][threadIdx.x >> 6] = r;
+    __syncthreads();
+    r = kNothing;
+    if (lane < W) r = parts[turn][lane];
+    join_wave<REF>(r);
+    turn ^= 1;
   }
 }
 
@@ -202,141 +330,351 @@ struct RowArgs {
   double batch;         // > 0: what the gradient is divided by, else the unmasked rows
   float cliprange, kl_coef, ent_coef;
   double *partials;
+  // rows cut into `splits` pieces of `piece` columns (a multiple of 2048)
+  int splits, piece;
+  RowStats *piece_stats;
+  struct RowPlan *plans;
 };
 
 enum Mode { LOGP, STATS, POLICY };
 
-// T threads per row (64: one wave, four rows per workgroup).
-// POLICY: the policy loss and its gradient; LOGP: log-probability and entropy; STATS: what the preference loss keeps.
-template <class D, int T, Mode MODE, bool REF>
+// what a row's gradient is made of: dz_j = p_j (c0 + c1 (z_j - m) + c2 (z_j - q_j)) + at 1{j = action}
+struct RowPlan { float m, inv_s, c0, c1, c2, at; };
+
+template <class D, bool REF, bool ENT>
+__device__ __forceinline__ float grad_of(const RowPlan &g, float x, float y) {
+  const float d = x - g.m, p = exp_of(d) * g.inv_s;
+  float v = g.c0;
+  if constexpr (ENT) v += g.c1 * fmaxf(d, kLowest);
+  if constexpr (REF) return p == 0.f ? 0.f : p * (v + g.c2 * (x - y));
+  return p * v;
+}
+
+struct RowTerms { float policy, entropy, kl, outside, ratio, lp; };
+
+// the policy loss of a row from its statistics: the gradient's plan and the row's terms
+template <bool REF>
+__device__ __forceinline__ RowPlan policy_row(const RowArgs &a, const RowStats &r, float za, float old, float adv, float ref, float w,
+                                              RowTerms *terms) {
+  const float log_s = logf(r.s), lp = (za - r.m) - log_s, H = log_s - r.ed / r.s;
+  const float ratio = expf(lp - old), l1 = -ratio * adv;
+  float policy = l1;
+  bool active = true, outside = false;
+  if (a.cliprange >= 0.f) {
+    const float lo = 1.f - a.cliprange, hi = 1.f + a.cliprange;
+    const float l2 = -(ratio < lo ? lo : ratio > hi ? hi : ratio) * adv;
+    active = !(l2 > l1);  // inside the range the two are equal
+    policy = active ? l1 : l2;
+    outside = ratio < lo || ratio > hi;
+  }
+  float g = active ? l1 : 0.f;  // d policy / d lp
+  float kl = 0.f, shift = 0.f;
+  if (a.ref_lp) {  // e^d - 1 - d with d = log ref - log p >= 0, its expectation under p is the divergence
+    const float d = ref - lp, em = expm1f(d);
+    kl = em - d;
+    g -= a.kl_coef * em;
+  }
+  if constexpr (REF) {
+    shift = (r.m - r.mr) + logf(r.s / r.sr);  // difference of the two log-normalisers
+    kl = r.gap / r.s - shift;
+  }
+  *terms = {policy, H, kl, outside ? 1.f : 0.f, ratio, lp};
+  // dz_j = w [ g (1{j = a} - p_j) + c_H p_j (log p_j + H) + c_K p_j (log p_j - log q_j - KL) ]
+  const float c1 = w * a.ent_coef, c2 = REF ? w * a.kl_coef : 0.f;
+  return RowPlan{r.m, 1.f / r.s, w * (a.ent_coef * (H - log_s) - g) - c2 * (shift + kl), c1, c2, w * g};
+}
+
+__device__ __forceinline__ float row_weight(const RowArgs &a) {
+  return static_cast<float>(1.0 / (a.batch > 0 ? a.batch : a.mask ? *a.count : static_cast<double>(a.rows)));
+}
+
+template <class D>
+__device__ __forceinline__ float action_logit(const char *row, long long action, int V) {
+  return action >= 0 && action < V ? D::get(reinterpret_cast<const typename D::Store *>(row)[action]) : __builtin_nanf("");
+}
+
+// T threads per row (64: one wave, four rows per workgroup).  POLICY: the policy loss and its gradient; LOGP: log-probability
+// and entropy; STATS: what the preference loss keeps.
+//   NV > 0: a thread holds its NV vectors of the row in registers, so the row is read once; while the gradient leaves, the
+//           vectors are replaced by those of the workgroup's next row, which are then on their way during the whole store.
+//   NV = 0: rows too long for that: the row is read twice, the second time from the caches for the most part.
+// A workgroup takes rows b, b + grid, ...: 64 of them at a time have their masks, actions, scalars and chosen logits loaded
+// by the lanes of every wave at once, one latency for all.
+template <class D, int T, int NV, Mode MODE, bool REF, bool ENT>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const RowArgs a) {
   constexpr int kWaves = T / 64, kRows = T < 256 ? 256 / T : 1;  // waves per row, rows per workgroup
-  constexpr int E = D::E;
-  __shared__ RowStats parts[2][kWaves > 1 ? kWaves : 1];
+  constexpr int E = D::E, N = NV ? NV : 1;
+  __shared__ RowStats parts[2][kWaves];
   __shared__ double sums[kRows][8];
   const int t = threadIdx.x % T, slot = threadIdx.x / T, lane = threadIdx.x & 63;
-  const double weight = MODE == POLICY ? 1.0 / (a.batch > 0 ? a.batch : a.mask ? *a.count : static_cast<double>(a.rows)) : 0.0;
-  const float w = static_cast<float>(weight);
-  double sum[6] = {0, 0, 0, 0, 0, 0};
+  const float w = MODE == POLICY ? row_weight(a) : 0.f;
+  if (MODE == POLICY && t < 8) sums[slot][t] = 0.0;
   int turn = 0;
-  for (long long row = static_cast<long long>(blockIdx.x) * kRows + slot; row < a.rows; row += static_cast<long long>(gridDim.x) * kRows) {
-    const bool keep = !a.mask || a.mask[row];
-    const char *z = a.z + row * a.z_pitch;
-    char *dz = MODE == POLICY ? a.dz + row * a.dz_pitch : nullptr;
-    if (!keep) {  // (the same decision in every thread of the row)
-      if (t == 0) {
-        if (MODE != STATS) a.lp[row] = 0.f;
-        if (MODE == LOGP && a.entropy) a.entropy[row] = 0.f;
-        if (MODE == STATS) a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      if (MODE == POLICY) {
-        float none[E];
+  const long long step = static_cast<long long>(gridDim.x) * kRows;
+  u32x4 v[N], u[REF ? N : 1];
+  // NV > 0: `vectors` whole vectors of a row (vector k T + t is this thread's k-th), and `rest` columns behind them, one each
+  // for the first threads
+  const int vectors = a.V / E, rest = a.V % E;
+  typename D::Store vt = {}, ut = {};
+  auto load_row = [&](long long row) {
+    const char *z = a.z + row * a.z_pitch, *q = REF ? a.q + row * a.q_pitch : nullptr;
+    if (t < rest) {
+      vt = reinterpret_cast<const typename D::Store *>(z)[vectors * E + t];
+      if constexpr (REF) ut = reinterpret_cast<const typename D::Store *>(q)[vectors * E + t];
+    }
+  };
+  auto load_part = [&](int k, long long row) {  // (a thread past the end reads the last vector; see `own`)
+    int lane_at = t;
+    asm volatile("" : "+v"(lane_at));  // (opaque: sixteen addresses kept over the rows would spill)
+    if ((k + 1) * T > vectors) lane_at = min(lane_at, vectors - 1 - k * T);
+    const uint32_t at = static_cast<uint32_t>(lane_at) * 16;
+    v[k] = *reinterpret_cast<const typename D::Vec *>(a.z + row * a.z_pitch + k * T * 16 + at);
+    if constexpr (REF) u[k] = *reinterpret_cast<const typename D::Vec *>(a.q + row * a.q_pitch + k * T * 16 + at);
+  };
+  // nothing but -inf in the vectors that this thread does not have
+  auto own = [&](int k) {
+    if ((k + 1) * T <= vectors) return;
+    constexpr uint32_t kNone = sizeof(typename D::Store) == 4 ? 0xff800000u : D::kNegInf * 0x10001u;
 #pragma unroll
-        for (int k = 0; k < E; ++k) none[k] = 0.f;
-        for (int first = t * E; first < a.V; first += T * E) store_vec<D>(dz, first, a.V, none);
+    for (int i = 0; i < 4; ++i) {
+      v[k][i] = k * T + t < vectors ? v[k][i] : kNone;
+      if constexpr (REF) u[k][i] = k * T + t < vectors ? u[k][i] : kNone;
+    }
+  };
+  for (long long row0 = static_cast<long long>(blockIdx.x) * kRows + slot; row0 < a.rows; row0 += 64 * step) {
+    const long long mine = row0 + lane * step;
+    const bool exists = mine < a.rows, keep = exists && (!a.mask || a.mask[mine]);
+    float za = 0.f, old = 0.f, adv = 0.f, ref = 0.f;
+    RowTerms out = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // of this lane's row
+    int action = -1;
+    if (keep) {
+      const long long wanted = a.actions[mine];
+      za = action_logit<D>(a.z + mine * a.z_pitch, wanted, a.V);  // before any store of the row: dz may be z
+      if (wanted >= 0 && wanted < a.V) action = static_cast<int>(wanted);
+      if (MODE == POLICY) {
+        old = a.old_lp[mine];
+        adv = a.adv[mine];
+        if (a.ref_lp) ref = a.ref_lp[mine];
       }
-      continue;
     }
-    const char *q = REF ? a.q + row * a.q_pitch : nullptr;
-    const long long action = a.actions[row];
-    const bool valid = action >= 0 && action < a.V;
-    // read before any store of this row: dz may be z
-    const float za = valid ? D::get(reinterpret_cast<const typename D::Store *>(z)[action]) : __builtin_nanf("");
-    RowStats r = {kLowest, 0.f, 0.f, 0.f, kLowest, 0.f};
-    for (int first = t * E; first < a.V; first += T * E) {
-      const u32x4 v = load_vec<D>(z, first, a.V);
-      u32x4 u = v;
-      if constexpr (REF) u = load_vec<D>(q, first, a.V);
-      add_vec<D, REF>(r, v, u);
+    unsigned long long left = __ballot(keep);
+    if (MODE == POLICY) {
+      if constexpr (kWaves > 1) {
+        asm volatile("" ::"v"(za));  // the chosen logits have arrived in every wave before any wave stores
+        __syncthreads();
+      }
+      for (unsigned long long none = __ballot(exists && !keep); none; none &= none - 1) {
+        char *dz = a.dz + (row0 + __builtin_ctzll(none) * step) * a.dz_pitch;
+        write_columns<D, T, false>(nullptr, nullptr, dz, a.V, 0, a.V, t, false, [](float, float, int) { return 0.f; });
+      }
     }
-    join_wave<REF>(r);
-    if constexpr (kWaves > 1) {
-      if (lane == 0) parts[turn][threadIdx.x >> 6] = r;
-      asm volatile("" ::"v"(za));  // za has arrived in every wave before any wave stores
-      __syncthreads();
-      r = {kLowest, 0.f, 0.f, 0.f, kLowest, 0.f};
-      if (lane < kWaves) r = parts[turn][lane];
-      join_wave<REF>(r);
-      turn ^= 1;
+    if (NV && left) {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (k * T < vectors) load_part(k, row0 + __builtin_ctzll(left) * step);
+      load_row(row0 + __builtin_ctzll(left) * step);
     }
-    const float log_s = logf(r.s);
-    const float lp = (za - r.m) - log_s;
-    if (MODE == LOGP || MODE == STATS) {
-      if (t == 0) {
+    while (left) {
+      const int j = __builtin_ctzll(left);
+      left &= left - 1;
+      const long long row = row0 + j * step;
+      RowStats r = kNothing;
+      if constexpr (NV > 0) {
+        // (asm: opaque, else the compiler keeps the 16-bit values once it has widened them, and spills)
+        const float xt = t < rest ? D::get(vt) : -INFINITY, yt = REF && t < rest ? D::get(ut) : -INFINITY;
+        r.m = fmaxf(r.m, xt);
+        if constexpr (REF) r.mr = fmaxf(r.mr, yt);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          if (k * T >= vectors) continue;
+          own(k);
+          float x[E], y[E];
+          D::unpack(v[k], x);
+          if constexpr (REF) D::unpack(u[k], y);
+#pragma unroll
+          for (int i = 0; i < E; i += 2) {
+            r.m = fmaxf(r.m, fmaxf(x[i], x[i + 1]));
+            if constexpr (REF) r.mr = fmaxf(r.mr, fmaxf(y[i], y[i + 1]));
+          }
+          __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          if (k * T >= vectors) continue;
+          asm volatile("" : "+v"(v[k]));
+          if constexpr (REF) asm volatile("" : "+v"(u[k]));
+          float x[E], y[E];
+          D::unpack(v[k], x);
+          if constexpr (REF) D::unpack(u[k], y);
+          add_terms<D, REF>(r, x, y);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        add_term<REF>(r, xt, yt);
+      } else {
+        add_columns<D, T, REF>(r, a.z + row * a.z_pitch, REF ? a.q + row * a.q_pitch : nullptr, a.V, 0, a.V, t);
+      }
+      join_row<kWaves, REF>(r, parts, turn);
+      const float z_chosen = lane_value(za, j);
+      if constexpr (MODE != POLICY) {
+        const float log_s = logf(r.s), lp = (z_chosen - r.m) - log_s;
         if (MODE == LOGP) {
-          a.lp[row] = lp;
-          if (a.entropy) a.entropy[row] = log_s - r.ed / r.s;
-        } else {
+          if (lane == j) {
+            out.lp = lp;
+            out.entropy = log_s - r.ed / r.s;
+          }
+        } else if (t == 0) {
           a.stats[row] = make_float4(r.m, 1.f / r.s, lp, 0.f);
         }
-      }
-      continue;
-    }
-    if constexpr (MODE == POLICY) {
-      const float H = log_s - r.ed / r.s;
-      const float ratio = expf(lp - a.old_lp[row]), adv = a.adv[row];
-      const float l1 = -ratio * adv;
-      float policy = l1;
-      bool active = true, outside = false;
-      if (a.cliprange >= 0.f) {
-        const float lo = 1.f - a.cliprange, hi = 1.f + a.cliprange;
-        const float l2 = -(ratio < lo ? lo : ratio > hi ? hi : ratio) * adv;
-        active = !(l2 > l1);  // inside the range the two are equal
-        policy = active ? l1 : l2;
-        outside = ratio < lo || ratio > hi;
-      }
-      float g = active ? l1 : 0.f;  // d policy / d lp
-      float kl = 0.f, shift = 0.f;
-      if (a.ref_lp) {  // e^d - 1 - d with d = log ref - log p >= 0, its expectation under p is the divergence
-        const float d = a.ref_lp[row] - lp, em = expm1f(d);
-        kl = em - d;
-        g -= a.kl_coef * em;
-      }
-      if constexpr (REF) {
-        shift = (r.m - r.mr) + logf(r.s / r.sr);  // difference of the two log-normalisers
-        kl = r.gap / r.s - shift;
-      }
-      if (t == 0) {
-        a.lp[row] = lp;
-        sum[0] += policy;
-        sum[1] += H;
-        sum[2] += kl;
-        sum[3] += outside ? 1.0 : 0.0;
-        sum[4] += ratio;
-        sum[5] += lp;
-      }
-      // dz_j = w [ g (1{j = a} - p_j) + c_H p_j (log p_j + H) + c_K p_j (log p_j - log q_j - KL) ]
-      //      = p_j (c0 + c1 (z_j - m) + c2 (z_j - q_j)) + w g 1{j = a}
-      const float c1 = w * a.ent_coef, c2 = REF ? w * a.kl_coef : 0.f;
-      const float c0 = w * (a.ent_coef * (H - log_s) - g) - c2 * (shift + kl);
-      const float inv_s = 1.f / r.s;
-      auto grad = [&](float x, float y) {
-        const float d = x - r.m, p = exp_of(d) * inv_s;
-        float v = c0 + c1 * fmaxf(d, kLowest);
-        if constexpr (REF) return p == 0.f ? 0.f : p * (v + c2 * (x - y));
-        return p * v;
-      };
-      for (int first = t * E; first < a.V; first += T * E) {
-        float x[E], y[E];
-        D::unpack(load_vec<D>(z, first, a.V), x);
-        if constexpr (REF) D::unpack(load_vec<D>(q, first, a.V), y);
+        if (NV && left) {
 #pragma unroll
-        for (int k = 0; k < E; ++k) x[k] = grad(x[k], REF ? y[k] : 0.f) + (first + k == action ? w * g : 0.f);
-        store_vec<D>(dz, first, a.V, x);
+          for (int k = 0; k < N; ++k)
+            if (k * T < vectors) load_part(k, row0 + __builtin_ctzll(left) * step);
+          load_row(row0 + __builtin_ctzll(left) * step);
+        }
+      } else {
+        RowTerms terms;
+        const RowPlan g = policy_row<REF>(a, r, z_chosen, lane_value(old, j), lane_value(adv, j), lane_value(ref, j), w, &terms);
+        if (lane == j) out = terms;
+        const int chosen = __builtin_amdgcn_readlane(action, j);
+        char *dz = a.dz + row * a.dz_pitch;
+        const long long next = left ? row0 + __builtin_ctzll(left) * step : -1;
+        if constexpr (NV > 0) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            if (k * T >= vectors) continue;
+            float x[E], y[E];
+            asm volatile("" : "+v"(v[k]));
+            D::unpack(v[k], x);
+            if constexpr (REF) {
+              asm volatile("" : "+v"(u[k]));
+              D::unpack(u[k], y);
+            }
+            if (next >= 0) load_part(k, next);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = grad_of<D, REF, ENT>(g, x[i], REF ? y[i] : 0.f);
+            if ((k + 1) * T <= vectors || k * T + t < vectors)
+              *reinterpret_cast<typename D::Vec *>(dz + k * T * 16 + static_cast<uint32_t>(t) * 16) = D::pack(x);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (t < rest)
+            reinterpret_cast<typename D::Store *>(dz)[vectors * E + t] =
+                D::put(grad_of<D, REF, ENT>(g, D::get(vt), REF ? D::get(ut) : 0.f));
+          if (next >= 0) load_row(next);
+        } else {
+          write_columns<D, T, REF>(a.z + row * a.z_pitch, REF ? a.q + row * a.q_pitch : nullptr, dz, a.V, 0, a.V, t, true,
+                                   [&](float x, float y, int) { return grad_of<D, REF, ENT>(g, x, y); });
+        }
+        // the chosen column again, by the thread that has just stored it (a thread's stores to one address stay in order)
+        if (chosen >= 0 && (NV && chosen >= vectors * E ? chosen - vectors * E : chosen / E % T) == t) {
+          const float y = REF ? D::get(reinterpret_cast<const typename D::Store *>(a.q + row * a.q_pitch)[chosen]) : 0.f;
+          reinterpret_cast<typename D::Store *>(dz)[chosen] = D::put(grad_of<D, REF, ENT>(g, z_chosen, y) + g.at);
+        }
       }
+    }
+    if (t < 64) {  // the first wave of the row: 64 rows' results at once
+      if (MODE != STATS && exists) a.lp[mine] = out.lp;
+      if (MODE == LOGP && exists && a.entropy) a.entropy[mine] = out.entropy;
+      if (MODE == POLICY) {
+        const float all[6] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp};
+#pragma unroll
+        for (int k = 0; k < 6; ++k) {
+          double s = all[k];
+#pragma unroll
+          for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+          if (lane == 0) sums[slot][k] += s;
+        }
+      }
+      if (MODE == STATS && exists && !keep) a.stats[mine] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
   if constexpr (MODE == POLICY) {
-    if (t == 0)
-#pragma unroll
-      for (int k = 0; k < 6; ++k) sums[slot][k] = sum[k];
     __syncthreads();
     if (threadIdx.x < 8) {
       double s = 0;
-      for (int i = 0; i < kRows; ++i) s += threadIdx.x < 6 ? sums[i][threadIdx.x] : 0.0;
+      for (int i = 0; i < kRows; ++i) s += sums[i][threadIdx.x];
       a.partials[blockIdx.x * 8LL + threadIdx.x] = s;
     }
   }
+}
+
+// ---- few rows: every row cut into pieces, a workgroup each ----------------------------------------------------------
+template <class D, bool REF>
+__global__ __launch_bounds__(256) void token_pieces_kernel(const RowArgs a) {
+  __shared__ RowStats parts[2][4];
+  const long long row = blockIdx.y;
+  if (a.mask && !a.mask[row]) return;
+  const int begin = blockIdx.x * a.piece, end = min(a.V, begin + a.piece);
+  const char *z = a.z + row * a.z_pitch, *q = REF ? a.q + row * a.q_pitch : nullptr;
+  RowStats r = kNothing;
+  int turn = 0;
+  add_columns<D, 256, REF>(r, z, q, a.V, begin, end, threadIdx.x);
+  join_row<4, REF>(r, parts, turn);
+  if (threadIdx.x == 0) a.piece_stats[row * a.splits + blockIdx.x] = r;
+}
+
+// the pieces of a row joined, a wave per row, and the row's results
+template <class D, Mode MODE, bool REF>
+__global__ __launch_bounds__(64) void token_join_kernel(const RowArgs a) {
+  const int lane = threadIdx.x;
+  const long long row = blockIdx.x;
+  if (a.mask && !a.mask[row]) {
+    if (lane == 0) {
+      if (MODE != STATS) a.lp[row] = 0.f;
+      if (MODE == LOGP && a.entropy) a.entropy[row] = 0.f;
+      if (MODE == STATS) a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (MODE == POLICY) {
+        a.plans[row] = RowPlan{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 8; ++k) a.partials[row * 8 + k] = 0.0;
+      }
+    }
+    return;
+  }
+  RowStats r = kNothing;
+  for (int i = lane; i < a.splits; i += 64) {
+    const RowStats p = a.piece_stats[row * a.splits + i];
+    RowStats q = p;
+    raise_max(q, r.m);
+    raise_max(r, p.m);
+    r.s += q.s;
+    r.ed += q.ed;
+    if constexpr (REF) {
+      raise_ref(q, r.mr);
+      raise_ref(r, p.mr);
+      r.sr += q.sr;
+      r.gap += q.gap;
+    }
+  }
+  join_wave<REF>(r);
+  const float za = action_logit<D>(a.z + row * a.z_pitch, a.actions[row], a.V);
+  const float log_s = logf(r.s);
+  const float lp = (za - r.m) - log_s;
+  if constexpr (MODE == POLICY) {
+    RowTerms out;
+    const RowPlan g = policy_row<REF>(a, r, za, a.old_lp[row], a.adv[row], a.ref_lp ? a.ref_lp[row] : 0.f, row_weight(a), &out);
+    if (lane == 0) {
+      a.plans[row] = g;
+      const double all[8] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp, 0.0, 0.0};
+      for (int k = 0; k < 8; ++k) a.partials[row * 8 + k] = all[k];
+    }
+  }
+  if (lane == 0) {
+    if (MODE != STATS) a.lp[row] = lp;
+    if (MODE == LOGP && a.entropy) a.entropy[row] = log_s - r.ed / r.s;
+    if (MODE == STATS) a.stats[row] = make_float4(r.m, 1.f / r.s, lp, 0.f);
+  }
+}
+
+template <class D, bool REF>
+__global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a) {
+  const long long row = blockIdx.y;
+  const bool keep = !a.mask || a.mask[row];
+  const RowPlan g = a.plans[row];
+  const long long action = keep ? a.actions[row] : -1;
+  const int begin = blockIdx.x * a.piece, end = min(a.V, begin + a.piece);
+  const char *z = a.z + row * a.z_pitch, *q = REF ? a.q + row * a.q_pitch : nullptr;
+  char *dz = a.dz + row * a.dz_pitch;
+  write_columns<D, 256, REF>(z, q, dz, a.V, begin, end, threadIdx.x, keep,
+                             [&](float x, float y, int col) { return grad_of<D, REF, true>(g, x, y) + (col == action ? g.at : 0.f); });
 }
 
 __global__ __launch_bounds__(1024) void mask_count_kernel(const uint8_t *mask, long long n, double *count) {
@@ -353,15 +691,17 @@ __global__ __launch_bounds__(1024) void mask_count_kernel(const uint8_t *mask, l
   }
 }
 
-// sums of `n` rows of eight doubles, in one fixed order: thread (i, k) takes rows i, i + 128, ... of column k
+// sums of `n` rows of eight doubles, in one fixed order: thread (i, k) of the T takes rows i, i + T / 8, ... of column k
+template <int T>
 __device__ void sum_partials(const double *partials, int n, double (&total)[8]) {
-  __shared__ double acc[128][8];
+  constexpr int R = T / 8;
+  __shared__ double acc[R][8];
   const int k = threadIdx.x & 7, i = threadIdx.x >> 3;
   double s = 0;
-  for (int j = i; j < n; j += 128) s += partials[j * 8LL + k];
+  for (int j = i; j < n; j += R) s += partials[j * 8LL + k];
   acc[i][k] = s;
   __syncthreads();
-  for (int half = 64; half > 0; half >>= 1) {
+  for (int half = R / 2; half > 0; half >>= 1) {
     if (i < half) acc[i][k] += acc[i + half][k];
     __syncthreads();
   }
@@ -371,7 +711,7 @@ __device__ void sum_partials(const double *partials, int n, double (&total)[8]) 
 __global__ __launch_bounds__(1024) void policy_terms_kernel(const double *partials, int n, const double *count, long long rows,
                                                             float kl_coef, float ent_coef, float *loss_out) {
   double s[8];
-  sum_partials(partials, n, s);
+  sum_partials<1024>(partials, n, s);
   if (threadIdx.x == 0) {
     const double c = count ? *count : static_cast<double>(rows);
     const double inv = c > 0 ? 1.0 / c : 0.0;  // nothing unmasked: zeros
@@ -444,41 +784,32 @@ __global__ __launch_bounds__(256) void preference_pairs_kernel(const PairArgs a)
   }
 }
 
-__global__ __launch_bounds__(1024) void preference_terms_kernel(const double *partials, int n, int pairs, float *loss_out) {
-  double s[8];
-  sum_partials(partials, n, s);
-  if (threadIdx.x == 0) {
-    for (int k = 0; k < 7; ++k) loss_out[k] = static_cast<float>(s[k] / pairs);
-    loss_out[7] = static_cast<float>(pairs);
-  }
-}
-
-// dz_j = c (1{j = a} - p_j) of every row, c the coefficient of its sequence (0: no sequence's, or masked)
+// dz_j = c (1{j = a} - p_j) of every row, c the coefficient of its sequence (0: no sequence's, or masked).  T threads take a
+// piece of a row; also the loss's terms, by the first workgroup.
 template <class D, int T>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void preference_grad_kernel(const RowArgs a) {
-  constexpr int kRows = T < 256 ? 256 / T : 1, E = D::E;
+__global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, int pairs, int pair_groups, float *loss_out) {
+  constexpr int kRows = 256 / T;
   const int t = threadIdx.x % T, slot = threadIdx.x / T;
-  // from the last row down: the end of the logits is what the statistics pass has left in the last-level cache
-  for (long long i = static_cast<long long>(blockIdx.x) * kRows + slot; i < a.rows; i += static_cast<long long>(gridDim.x) * kRows) {
-    const long long row = a.rows - 1 - i;
-    const float4 st = a.stats[row];
-    char *dz = a.dz + row * a.dz_pitch;
-    const char *z = a.z + row * a.z_pitch;
-    const float c = st.w, k = -c * st.y;
-    const long long action = c != 0.f ? a.actions[row] : -1;
-    for (int first = t * E; first < a.V; first += T * E) {
-      float x[E];
-      if (c != 0.f) {
-        D::unpack(load_vec<D>(z, first, a.V), x);
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = k * exp_of(x[j] - st.x) + (first + j == action ? c : 0.f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = 0.f;
-      }
-      store_vec<D>(dz, first, a.V, x);
+  if (blockIdx.x == 0) {
+    double s[8];
+    sum_partials<256>(a.partials, pair_groups, s);
+    if (threadIdx.x == 0) {
+      for (int k = 0; k < 7; ++k) loss_out[k] = static_cast<float>(s[k] / pairs);
+      loss_out[7] = static_cast<float>(pairs);
     }
   }
+  // from the last row down: the end of the logits is what the statistics pass has left in the last-level cache
+  const long long i = (blockIdx.x / a.splits) * static_cast<long long>(kRows) + slot;
+  if (i >= a.rows) return;
+  const long long row = a.rows - 1 - i;
+  const int begin = blockIdx.x % a.splits * a.piece, end = min(a.V, begin + a.piece);
+  const float4 st = a.stats[row];
+  char *dz = a.dz + row * a.dz_pitch;
+  const char *z = a.z + row * a.z_pitch;
+  const float c = st.w, k = -c * st.y;
+  const long long action = c != 0.f ? a.actions[row] : -1;
+  write_columns<D, T, false>(z, nullptr, dz, a.V, begin, end, t, c != 0.f,
+                             [&](float x, float, int col) { return k * exp_of(x - st.x) + (col == action ? c : 0.f); });
 }
 
 // log-probabilities of sequences: a workgroup per sequence
@@ -498,49 +829,105 @@ template <class D>
 __global__ __launch_bounds__(256) void scale_rows_kernel(char *x, long long pitch, long long rows, int V, const float *factor) {
   const float f = *factor;
   if (f == 1.f) return;
-  constexpr int E = D::E;
   for (long long row = blockIdx.x; row < rows; row += gridDim.x)
-    for (int first = threadIdx.x * E; first < V; first += 256 * E) {
-      float v[E];
-      D::unpack(load_vec<D>(x + row * pitch, first, V), v);
-#pragma unroll
-      for (int k = 0; k < E; ++k) v[k] *= f;
-      store_vec<D>(x + row * pitch, first, V, v);
-    }
+    write_columns<D, 256, false>(x + row * pitch, nullptr, x + row * pitch, V, 0, V, threadIdx.x, true,
+                                 [&](float v, float, int) { return v * f; });
 }
 
-// threads per row, by its bytes
-inline int row_threads(int V, int dtype) {
-  const long long bytes = static_cast<long long>(V) * (dtype == DX_F32 ? 4 : 2);
-  return bytes <= 4096 ? 64 : bytes <= 32768 ? 256 : 1024;
-}
-inline int row_grid(long long rows, int T) {
-  const long long need = T == 64 ? (rows + 3) / 4 : rows;
-  const long long most = T == 1024 ? 512 : kMaxWorkers;
-  return static_cast<int>(need < most ? need : most);
+inline int elem_size(int dtype) { return dtype == DX_F32 ? 4 : 2; }
+
+// Threads per row T and vectors of 16 bytes a thread holds of it, NV (0: too many for the registers).
+struct RowShape { int T, NV; };
+RowShape row_shape(int V, int dtype, bool ref, bool once) {
+  const long long vectors = (static_cast<long long>(V) * elem_size(dtype) + 15) / 16;
+  const int most = ref ? 8 : 16;  // registers: two rows are held where there are reference logits
+  if (vectors <= 64 * 4) return {64, vectors <= 64 ? 1 : 4};
+  if (once) return {256, 0};  // read once anyway: the more waves, the more is on its way
+  if (vectors <= 256 * 4) return {256, 4};
+  if (vectors <= 256 * most) return {256, vectors <= 256 * 8 ? 8 : 16};
+  if (vectors <= 1024 * most) return {1024, vectors <= 1024 * 8 ? 8 : 16};
+  return {1024, 0};
 }
 
-template <class D, Mode MODE, bool REF>
-int launch_rows(const RowArgs &a, int T, int grid, hipStream_t s) {
-  if (T == 64) hipLaunchKernelGGL((token_rows_kernel<D, 64, MODE, REF>), dim3(grid), dim3(256), 0, s, a);
-  else if (T == 256) hipLaunchKernelGGL((token_rows_kernel<D, 256, MODE, REF>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((token_rows_kernel<D, 1024, MODE, REF>), dim3(grid), dim3(1024), 0, s, a);
-  DX_LAUNCH_CHECK();
-  return DX_OK;
-}
-template <Mode MODE, bool REF>
-int launch_rows_of(const RowArgs &a, int dtype, int T, int grid, hipStream_t s) {
-  if (dtype == DX_F32) return launch_rows<ElemF32, MODE, REF>(a, T, grid, s);
-  if (dtype == DX_BF16) return launch_rows<ElemBF16, MODE, REF>(a, T, grid, s);
-  return launch_rows<ElemF16, MODE, REF>(a, T, grid, s);
+template <class D, Mode MODE, bool REF, bool ENT>
+int launch_rows(const RowArgs &a, RowShape sh, int grid, hipStream_t s) {
+#define DX_ROWS(TT, NN)                                                                                                       \
+  if (sh.T == TT && sh.NV == NN) {                                                                                            \
+    hipLaunchKernelGGL((token_rows_kernel<D, TT, NN, MODE, REF, ENT>), dim3(grid), dim3(TT < 256 ? 256 : TT), 0, s, a);       \
+    DX_LAUNCH_CHECK();                                                                                                        \
+    return DX_OK;                                                                                                             \
+  }
+  DX_ROWS(64, 1)
+  DX_ROWS(64, 4)
+  if constexpr (MODE != POLICY) {
+    DX_ROWS(256, 0)
+  } else {
+    DX_ROWS(256, 4)
+    DX_ROWS(256, 8)
+    if constexpr (!REF) DX_ROWS(256, 16)
+    DX_ROWS(1024, 8)
+    if constexpr (!REF) DX_ROWS(1024, 16)
+    DX_ROWS(1024, 0)
+  }
+#undef DX_ROWS
+  return dx::fail(DX_ENOSUP, "token rows: no kernel for %d threads, %d vectors", sh.T, sh.NV);
 }
 template <class D>
-int launch_pref_grad(const RowArgs &a, int T, int grid, hipStream_t s) {
-  if (T == 64) hipLaunchKernelGGL((preference_grad_kernel<D, 64>), dim3(grid), dim3(256), 0, s, a);
-  else if (T == 256) hipLaunchKernelGGL((preference_grad_kernel<D, 256>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((preference_grad_kernel<D, 1024>), dim3(grid), dim3(1024), 0, s, a);
+int launch_pref_grad(const RowArgs &a, int T, int grid, int pairs, int pair_groups, float *loss_out, hipStream_t s) {
+  if (T == 64) hipLaunchKernelGGL((preference_grad_kernel<D, 64>), dim3(grid), dim3(256), 0, s, a, pairs, pair_groups, loss_out);
+  else hipLaunchKernelGGL((preference_grad_kernel<D, 256>), dim3(grid), dim3(256), 0, s, a, pairs, pair_groups, loss_out);
   DX_LAUNCH_CHECK();
   return DX_OK;
+}
+
+// Rows -> statistics (LOGP, STATS: results too) or the whole policy loss.  `*groups`: rows of `partials` that were written.
+// Few long rows are cut into pieces over the CUs and joined by a second launch.
+template <class D, Mode MODE, bool REF, bool ENT>
+int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
+  int cus = 0;
+  if (int rc = dx::device_cus(&cus)) return rc;
+  const long long bytes = static_cast<long long>(a.V) * elem_size(dtype);
+  if (a.rows <= kMaxPieces / 2 && bytes >= 32768 && a.rows * 2 <= cus) {
+    long long splits = cus / a.rows, most = (bytes + 8191) / 8192;
+    if (splits > most) splits = most;
+    if (splits * a.rows > kMaxPieces) splits = kMaxPieces / a.rows;
+    a.piece = static_cast<int>((a.V + splits - 1) / splits + 2047) / 2048 * 2048;
+    a.splits = (a.V + a.piece - 1) / a.piece;
+    if (a.splits > 1) {
+      const dim3 grid(a.splits, static_cast<unsigned>(a.rows));
+      hipLaunchKernelGGL((token_pieces_kernel<D, REF>), grid, dim3(256), 0, s, a);
+      DX_LAUNCH_CHECK();
+      hipLaunchKernelGGL((token_join_kernel<D, MODE, REF>), dim3(static_cast<unsigned>(a.rows)), dim3(64), 0, s, a);
+      DX_LAUNCH_CHECK();
+      if (MODE == POLICY) {
+        hipLaunchKernelGGL((token_pieces_grad_kernel<D, REF>), grid, dim3(256), 0, s, a);
+        DX_LAUNCH_CHECK();
+      }
+      *groups = static_cast<int>(a.rows);
+      return DX_OK;
+    }
+  }
+  const RowShape sh = row_shape(a.V, dtype, REF, MODE != POLICY);
+  const long long need = sh.T == 64 ? (a.rows + 3) / 4 : a.rows;
+  // resident workgroups: 1024 threads with 16 vectors each fill a CU
+  const long long most = MODE != POLICY ? 8LL * cus : sh.T == 1024 ? (sh.NV == 16 || REF ? cus : 2LL * cus) : 8LL * cus < kMaxWorkers ? 8LL * cus : kMaxWorkers;
+  const int grid = static_cast<int>(need < most ? need : most);
+  *groups = grid;
+  if (grid == 0) return DX_OK;
+  return launch_rows<D, MODE, REF, ENT>(a, sh, grid, s);
+}
+template <class D>
+int run_policy(const RowArgs &a, int dtype, int *groups, hipStream_t s) {
+  if (a.q) return run_rows<D, POLICY, true, true>(a, dtype, groups, s);
+  if (a.ent_coef != 0.f) return run_rows<D, POLICY, false, true>(a, dtype, groups, s);
+  return run_rows<D, POLICY, false, false>(a, dtype, groups, s);
+}
+template <Mode MODE>
+int run_stats(const RowArgs &a, int dtype, hipStream_t s) {
+  int groups = 0;
+  if (dtype == DX_F32) return run_rows<ElemF32, MODE, false, false>(a, dtype, &groups, s);
+  if (dtype == DX_BF16) return run_rows<ElemBF16, MODE, false, false>(a, dtype, &groups, s);
+  return run_rows<ElemF16, MODE, false, false>(a, dtype, &groups, s);
 }
 
 // what every entry point over logits checks
@@ -554,9 +941,19 @@ int check_logits(const char *who, const void *logits, int dtype, long long rows,
   return DX_OK;
 }
 
-RowArgs row_args(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions, const uint8_t *mask) {
+// workspace, in doubles: 8 for the count, 8 a workgroup for its sums, the pieces' statistics and the rows' plans
+constexpr int kPartialsAt = 8, kPiecesAt = 8 + 8 * kMaxWorkers, kPlansAt = kPiecesAt + kMaxPieces * 3;
+static_assert(sizeof(RowStats) == 24 && sizeof(RowPlan) == 24 && kPlansAt + kMaxPieces * 3 == DX_TOKEN_WORKSPACE, "workspace");
+
+RowArgs row_args(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions, const uint8_t *mask,
+                 double *workspace) {
   RowArgs a{};
-  const int size = dtype == DX_F32 ? 4 : 2;
+  a.splits = 1;
+  a.count = workspace;
+  a.partials = workspace + kPartialsAt;
+  a.piece_stats = reinterpret_cast<RowStats *>(workspace + kPiecesAt);
+  a.plans = reinterpret_cast<RowPlan *>(workspace + kPlansAt);
+  const int size = elem_size(dtype);
   a.z = static_cast<const char *>(logits);
   a.z_pitch = pitch * size;
   a.rows = rows;
@@ -569,16 +966,18 @@ RowArgs row_args(const void *logits, int dtype, long long rows, int vocab, long 
 }  // namespace
 
 extern "C" int dx_token_log_prob(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
-                                 const uint8_t *mask, float *log_prob, float *entropy, void *stream) {
+                                 const uint8_t *mask, float *log_prob, float *entropy, double *workspace, long long workspace_count,
+                                 void *stream) {
   DX_TRACE("dx_token_log_prob");
   if (int rc = check_logits("dx_token_log_prob", logits, dtype, rows, vocab, pitch, actions)) return rc;
   if (rows == 0) return DX_OK;
-  DX_REQUIRE(log_prob != nullptr, "dx_token_log_prob: null pointer");
-  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask);
+  DX_REQUIRE(log_prob != nullptr && workspace != nullptr, "dx_token_log_prob: null pointer");
+  if (workspace_count < DX_TOKEN_WORKSPACE)
+    return dx::fail(DX_EWS, "dx_token_log_prob: workspace of %lld doubles, %d needed", workspace_count, DX_TOKEN_WORKSPACE);
+  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask, workspace);
   a.lp = log_prob;
   a.entropy = entropy;
-  const int T = row_threads(vocab, dtype);
-  return launch_rows_of<LOGP, false>(a, dtype, T, row_grid(rows, T), dx::as_stream(stream));
+  return run_stats<LOGP>(a, dtype, dx::as_stream(stream));
 }
 
 extern "C" int dx_sequence_log_prob(const float *token_log_prob, const int32_t *offsets, long long rows, int sequences, float *out,
@@ -610,8 +1009,8 @@ extern "C" int dx_token_policy_loss(const void *logits, int dtype, long long row
   if (workspace_count < DX_TOKEN_WORKSPACE)
     return dx::fail(DX_EWS, "dx_token_policy_loss: workspace of %lld doubles, %d needed", workspace_count, DX_TOKEN_WORKSPACE);
   hipStream_t s = dx::as_stream(stream);
-  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask);
-  const int size = dtype == DX_F32 ? 4 : 2;
+  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask, workspace);
+  const int size = elem_size(dtype);
   a.q = static_cast<const char *>(ref_logits);
   a.q_pitch = ref_pitch * size;
   a.dz = static_cast<char *>(dlogits);
@@ -620,21 +1019,19 @@ extern "C" int dx_token_policy_loss(const void *logits, int dtype, long long row
   a.adv = advantages;
   a.ref_lp = ref_log_prob;
   a.lp = log_prob;
-  a.count = workspace;
   a.batch = global_batch > 0 ? static_cast<double>(global_batch) : 0.0;
   a.cliprange = cliprange;
   a.kl_coef = kl_coef;
   a.ent_coef = entropy_coef;
-  a.partials = workspace + 8;
   if (mask) {
     hipLaunchKernelGGL(mask_count_kernel, dim3(1), dim3(1024), 0, s, mask, rows, workspace);
     DX_LAUNCH_CHECK();
   }
-  const int T = row_threads(vocab, dtype), grid = row_grid(rows, T);
-  if (grid > 0) {
-    if (int rc = ref_logits ? launch_rows_of<POLICY, true>(a, dtype, T, grid, s) : launch_rows_of<POLICY, false>(a, dtype, T, grid, s)) return rc;
-  }
-  hipLaunchKernelGGL(policy_terms_kernel, dim3(1), dim3(1024), 0, s, a.partials, grid, mask ? workspace : nullptr, rows, kl_coef,
+  int groups = 0;
+  if (rows > 0)
+    if (int rc = dtype == DX_F32 ? run_policy<ElemF32>(a, dtype, &groups, s)
+                 : dtype == DX_BF16 ? run_policy<ElemBF16>(a, dtype, &groups, s) : run_policy<ElemF16>(a, dtype, &groups, s)) return rc;
+  hipLaunchKernelGGL(policy_terms_kernel, dim3(1), dim3(1024), 0, s, a.partials, groups, mask ? workspace : nullptr, rows, kl_coef,
                      entropy_coef, loss_out);
   DX_LAUNCH_CHECK();
   return DX_OK;
@@ -656,24 +1053,27 @@ extern "C" int dx_preference_loss(const void *logits, int dtype, long long rows,
   if (workspace_count < DX_TOKEN_WORKSPACE)
     return dx::fail(DX_EWS, "dx_preference_loss: workspace of %lld doubles, %d needed", workspace_count, DX_TOKEN_WORKSPACE);
   hipStream_t s = dx::as_stream(stream);
-  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask);
+  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask, workspace);
   a.stats = reinterpret_cast<float4 *>(row_stats);
   a.dz = static_cast<char *>(dlogits);
-  a.dz_pitch = dlogits_pitch * (dtype == DX_F32 ? 4 : 2);
-  const int T = row_threads(vocab, dtype), grid = row_grid(rows, T);
-  if (grid > 0)
-    if (int rc = launch_rows_of<STATS, false>(a, dtype, T, grid, s)) return rc;
+  a.dz_pitch = dlogits_pitch * elem_size(dtype);
+  if (rows > 0)
+    if (int rc = run_stats<STATS>(a, dtype, s)) return rc;
   PairArgs p{a.stats, offsets, ref_log_prob, mask, rows, pairs, global_pairs > 0 ? static_cast<double>(global_pairs) : 0.0, beta,
-             label_smoothing, sequence_log_prob, workspace + 8};
-  const int pair_grid = pairs < kMaxWorkers ? pairs : kMaxWorkers;
-  hipLaunchKernelGGL(preference_pairs_kernel, dim3(pair_grid), dim3(256), 0, s, p);
+             label_smoothing, sequence_log_prob, a.partials};
+  const int pair_groups = pairs < kMaxWorkers ? pairs : kMaxWorkers;
+  hipLaunchKernelGGL(preference_pairs_kernel, dim3(pair_groups), dim3(256), 0, s, p);
   DX_LAUNCH_CHECK();
-  hipLaunchKernelGGL(preference_terms_kernel, dim3(1), dim3(1024), 0, s, p.partials, pair_grid, pairs, loss_out);
-  DX_LAUNCH_CHECK();
-  if (grid == 0) return DX_OK;
-  if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, grid, s);
-  if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, grid, s);
-  return launch_pref_grad<ElemF16>(a, T, grid, s);
+  // gradient: a wave per short row, else a workgroup per piece of 32 KB of a row
+  const int T = static_cast<long long>(vocab) * elem_size(dtype) <= 4096 ? 64 : 256;
+  a.piece = T == 64 ? vocab : 32768 / elem_size(dtype);
+  a.splits = (vocab - 1) / a.piece + 1;
+  const long long blocks = (T == 64 ? (rows + 3) / 4 : rows) * a.splits;
+  DX_REQUIRE(blocks <= 0x7fffffffLL, "dx_preference_loss: %lld rows of %d logits are more than a launch takes", rows, vocab);
+  const int grid = blocks < 1 ? 1 : static_cast<int>(blocks);  // (the first workgroup also writes the terms)
+  if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, grid, pairs, pair_groups, loss_out, s);
+  if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, grid, pairs, pair_groups, loss_out, s);
+  return launch_pref_grad<ElemF16>(a, T, grid, pairs, pair_groups, loss_out, s);
 }
 
 extern "C" int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pitch, const float *factor, void *stream) {

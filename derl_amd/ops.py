@@ -249,7 +249,7 @@ _ELEMENT_TYPES = {torch.float32: _lib.DX_F32, torch.bfloat16: _lib.DX_BF16, torc
 def _call_on(device, name, *args):
   """One native call with ``device`` current (kernels launch on the current device)."""
   if device.index == torch.cuda.current_device():
-    _lib.call(name, *args)
+    _lib.check(getattr(_lib.load(), name)(*args), name)
   else:
     with torch.cuda.device(device):
       _lib.call(name, *args)
@@ -274,18 +274,19 @@ def _rows_of(t, name, like=None):
 
 
 def _vector(t, name, n, device, dtype):
-  """A contiguous vector of ``n`` on the logits' device; its pointer (None stays None)."""
+  """Address of a contiguous vector of ``n`` on the logits' device (None stays None)."""
   if t is None:
     return None
+  if (isinstance(t, torch.Tensor) and t.dtype in dtype and t.shape == (n,) and t.get_device() == device.index
+      and t.is_contiguous()):
+    return t.data_ptr()
   _dev(t, name)
   if t.dtype not in dtype:
     raise ValueError(f"{name} must have dtype {' or '.join(map(str, dtype))}, got {t.dtype}")
-  if tuple(t.shape) != (n,) or t.device != device:
-    raise ValueError(f"{name} must be ({n},) on {device}, got {tuple(t.shape)} on {t.device}")
-  return _lib.ptr(t)
+  raise ValueError(f"{name} must be ({n},) on {device}, got {tuple(t.shape)} on {t.device}")
 
 
-_INDEX, _FLAG, _FLOAT, _OFFSET = (torch.int64,), (torch.bool, torch.uint8), (torch.float32,), (torch.int32,)
+_INDEX, _FLAG, _FLOAT = (torch.int64,), (torch.bool, torch.uint8), (torch.float32,)
 
 
 def _span(t):
@@ -321,12 +322,13 @@ def token_log_prob(logits, actions, mask=None):
   single tokens of sequences being generated."""
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
-  out = torch.empty((2, rows), dtype=torch.float32, device=dev)
-  log_prob, entropy = out[0], out[1]
+  log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
+  entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
   act = _vector(actions, "actions", rows, dev, _INDEX)
   keep = _vector(mask, "mask", rows, dev, _FLAG)
-  _call_on(dev, "dx_token_log_prob", _lib.ptr(logits), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, keep,
-           _lib.ptr(log_prob), _lib.ptr(entropy), _lib.stream_ptr(dev))
+  _call_on(dev, "dx_token_log_prob", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, keep,
+           log_prob.data_ptr(), entropy.data_ptr(), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(dev))
   return log_prob, entropy
 
 
@@ -346,7 +348,7 @@ def sequence_log_prob(logits, actions, offsets, mask=None):
   sequences = _check_offsets(offsets, dev)
   log_prob, _ = token_log_prob(logits, actions, mask)
   out = torch.empty(sequences, dtype=torch.float32, device=dev)
-  _call_on(dev, "dx_sequence_log_prob", _lib.ptr(log_prob), _lib.ptr(offsets), rows, sequences, _lib.ptr(out),
+  _call_on(dev, "dx_sequence_log_prob", log_prob.data_ptr(), offsets.data_ptr(), rows, sequences, out.data_ptr(),
            _lib.stream_ptr(dev))
   return out
 
@@ -384,10 +386,10 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
   log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
   workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
-  _call_on(dev, "dx_token_policy_loss", _lib.ptr(logits), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, old, adv, ref,
-           _lib.ptr(ref_logits), ref_pitch, keep, -1.0 if cliprange is None else float(cliprange), float(kl_coef),
-           float(entropy_coef), int(global_batch), _lib.ptr(dlogits), dlogits.stride(0) if rows > 1 else vocab,
-           _lib.ptr(log_prob), _lib.ptr(workspace), workspace.numel(), _lib.ptr(loss_out), _lib.stream_ptr(dev))
+  _call_on(dev, "dx_token_policy_loss", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, old, adv, ref,
+           None if ref_logits is None else ref_logits.data_ptr(), ref_pitch, keep, -1.0 if cliprange is None else float(cliprange), float(kl_coef),
+           float(entropy_coef), int(global_batch), dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab,
+           log_prob.data_ptr(), workspace.data_ptr(), workspace.numel(), loss_out.data_ptr(), _lib.stream_ptr(dev))
   return loss_out, dlogits, log_prob
 
 
@@ -418,12 +420,12 @@ def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothin
   dlogits = _gradient_buffer(dlogits_out, logits)
   sequence = torch.empty(sequences, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
-  row_stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
-  _call_on(dev, "dx_preference_loss", _lib.ptr(logits), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act,
-           _lib.ptr(offsets), sequences // 2, ref, keep, float(beta), float(label_smoothing), int(global_pairs),
-           _lib.ptr(dlogits), dlogits.stride(0) if rows > 1 else vocab, _lib.ptr(sequence), _lib.ptr(row_stats),
-           _lib.ptr(workspace), workspace.numel(), _lib.ptr(loss_out), _lib.stream_ptr(dev))
+  # the library's scratch and behind it four floats a row
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE + 2 * rows, dtype=torch.float64, device=dev)
+  _call_on(dev, "dx_preference_loss", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act,
+           offsets.data_ptr(), sequences // 2, ref, keep, float(beta), float(label_smoothing), int(global_pairs),
+           dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, sequence.data_ptr(),
+           workspace.data_ptr() + 8 * _lib.DX_TOKEN_WORKSPACE, workspace.data_ptr(), _lib.DX_TOKEN_WORKSPACE, loss_out.data_ptr(), _lib.stream_ptr(dev))
   return loss_out, dlogits, sequence
 
 
@@ -433,7 +435,7 @@ def scale_rows(x, factor):
   _dev(factor, "factor", torch.float32)
   if factor.numel() != 1 or factor.device != x.device:
     raise ValueError(f"factor must be one float32 on {x.device}, got {tuple(factor.shape)} on {factor.device}")
-  _call_on(x.device, "dx_scale_rows", _lib.ptr(x), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, _lib.ptr(factor),
+  _call_on(x.device, "dx_scale_rows", x.data_ptr(), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, factor.data_ptr(),
            _lib.stream_ptr(x.device))
   return x
 
@@ -446,7 +448,7 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
   """Newton-Schulz orthogonalisation of (..., m, n) matrices: X = G / (|G|_F + eps), then ``steps`` times
   X <- a X + (b A + c A A) X with A = X X^T (of the shorter side).  The singular vectors stay, the singular
-  values approach 1.  float32 (fp32 accuracy throughout), bfloat16 or float16 (11-bit intermediates);
+  values approach 1.  float32 or float16 (fp32 accuracy throughout) or bfloat16 (11-bit intermediates);
   contiguous; the result has update's type and shape.  ``out`` may be ``update``.  A zero matrix gives zeros."""
   if not isinstance(update, torch.Tensor) or not update.is_cuda:
     raise ValueError("update must be a tensor on the GPU (derl_amd has no CPU path)")
@@ -476,8 +478,8 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
   need = _lib.load().dx_orthogonalize_workspace(kind, batch, m, n)
   _lib.check(min(need, 0), "dx_orthogonalize_workspace")
   workspace = torch.empty(need, dtype=torch.uint8, device=update.device)
-  _call_on(update.device, "dx_orthogonalize", _lib.ptr(update), kind, batch, m, n, int(steps), a, b, c, float(eps),
-           _lib.ptr(out), _lib.ptr(workspace), need, _lib.stream_ptr(update.device))
+  _call_on(update.device, "dx_orthogonalize", update.data_ptr(), kind, batch, m, n, int(steps), a, b, c, float(eps),
+           out.data_ptr(), workspace.data_ptr(), need, _lib.stream_ptr(update.device))
   return out
 
 

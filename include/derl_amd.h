@@ -219,10 +219,10 @@ int dx_reward_summary_f32(const float *rewards, const uint8_t *resets, int T, in
 #define DX_F32 0
 #define DX_BF16 1
 #define DX_F16 2
-#define DX_TOKEN_WORKSPACE 16392
+#define DX_TOKEN_WORKSPACE 19464
 int dx_token_log_prob(const void *logits, int dtype, long long rows, int vocab, long long pitch,
                       const int64_t *actions, const uint8_t *mask, float *log_prob, float *entropy,
-                      void *stream);
+                      double *workspace, long long workspace_count, void *stream);
 int dx_sequence_log_prob(const float *token_log_prob, const int32_t *offsets, long long rows,
                          int sequences, float *out, void *stream);
 int dx_token_policy_loss(const void *logits, int dtype, long long rows, int vocab, long long pitch,
@@ -244,8 +244,9 @@ int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pit
 /* ---------------------------------------------------------------------------------
  * Orthogonalised update of a matrix optimizer: `batch` contiguous (m, n) matrices of `dtype`, each
  *   X = G / (|G|_F + eps);  `steps` times: A = X X^T (of the shorter side), X <- a X + (b A + c A^2) X
- * and `out` = X in the same type (out may be update).  Products on the fp16 matrix cores: fp32 input as
- * two fp16 terms per operand and three products (22 bits, fp32 accuracy), bf16 / fp16 input as one.
+ * and `out` = X in the same type (out may be update).  Products on the fp16 matrix cores: two fp16 terms per
+ * operand and three products (22 bits, fp32 accuracy); bf16: one term of X, of A and B too where the shorter
+ * side passes 640.
  * Intermediate entries are held scaled: |X| < 16 and |b A + c A^2 + a| < 256 must hold, which any
  * coefficients whose iteration keeps singular values near 1 do.
  * dx_orthogonalize_workspace: bytes of `workspace` (256-byte aligned), negative DX_E* on bad shapes.

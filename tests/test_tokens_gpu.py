@@ -434,7 +434,7 @@ def check_orthogonal(got, g, steps, dtype):
   """Each step rounds X, A and B (two fp16 terms: 2^-22 each, one: 2^-12; fp32 accumulation: 2^-24 sqrt(K) each) and
   passes the error on multiplied by the polynomial's slope, a at most.  In Frobenius norm."""
   want, norms = newton_schulz64(g, steps)
-  unit = (3 * 2.0 ** -22 if dtype == F32 else 3 * 2.0 ** -12) + 3 * 2.0 ** -24 * max(g.shape) ** 0.5
+  unit = (3 * 2.0 ** -12 if dtype == BF16 else 3 * 2.0 ** -22) + 3 * 2.0 ** -24 * max(g.shape) ** 0.5
   bound = 2 * unit * sum(A ** (steps - k) * n for k, n in enumerate(norms)) + torch.finfo(dtype).eps / 2 * norms[-1]
   assert got.dtype == dtype and got.shape == g.shape
   assert float((got.double() - want).norm()) <= bound, (float((got.double() - want).norm()), bound)
