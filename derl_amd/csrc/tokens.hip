@@ -836,37 +836,39 @@ __global__ __launch_bounds__(256) void scale_rows_kernel(char *x, long long pitc
 
 inline int elem_size(int dtype) { return dtype == DX_F32 ? 4 : 2; }
 
-// Threads per row T and vectors of 16 bytes a thread holds of it, NV (0: too many for the registers).
+// Threads per row T and vectors of 16 bytes a thread holds of it, NV (0: none, or too many for the registers).
 struct RowShape { int T, NV; };
 RowShape row_shape(int V, int dtype, bool ref, bool once) {
   const long long vectors = (static_cast<long long>(V) * elem_size(dtype) + 15) / 16;
-  const int most = ref ? 8 : 16;  // registers: two rows are held where there are reference logits
-  if (vectors <= 64 * 4) return {64, vectors <= 64 ? 1 : 4};
+  if (vectors <= 64) return {64, 1};
+  if (vectors <= 64 * 8) return {64, vectors <= 64 * 4 ? 4 : 8};
   if (once) return {256, 0};  // read once anyway: the more waves, the more is on its way
-  if (vectors <= 256 * 4) return {256, 4};
-  if (vectors <= 256 * most) return {256, vectors <= 256 * 8 ? 8 : 16};
-  if (vectors <= 1024 * most) return {1024, vectors <= 1024 * 8 ? 8 : 16};
+  const int most = ref ? 8 : 16;  // two rows are held where there are reference logits
+  if (vectors <= 256 * most) return {256, vectors <= 256 * 4 ? 4 : vectors <= 256 * 8 ? 8 : 16};
+  if (vectors <= 512 * most) return {512, most};
+  if (vectors <= 1024 * most) return {1024, most};
   return {1024, 0};
 }
 
 template <class D, Mode MODE, bool REF, bool ENT>
 int launch_rows(const RowArgs &a, RowShape sh, int grid, hipStream_t s) {
 #define DX_ROWS(TT, NN)                                                                                                       \
-  if (sh.T == TT && sh.NV == NN) {                                                                                            \
-    hipLaunchKernelGGL((token_rows_kernel<D, TT, NN, MODE, REF, ENT>), dim3(grid), dim3(TT < 256 ? 256 : TT), 0, s, a);       \
+  if (sh.T == (TT) && sh.NV == (NN)) {                                                                                            \
+    hipLaunchKernelGGL((token_rows_kernel<D, (TT), (NN), MODE, REF, ENT>), dim3(grid), dim3((TT) < 256 ? 256 : (TT)), 0, s, a);   \
     DX_LAUNCH_CHECK();                                                                                                        \
     return DX_OK;                                                                                                             \
   }
   DX_ROWS(64, 1)
   DX_ROWS(64, 4)
+  DX_ROWS(64, 8)
   if constexpr (MODE != POLICY) {
     DX_ROWS(256, 0)
   } else {
     DX_ROWS(256, 4)
     DX_ROWS(256, 8)
     if constexpr (!REF) DX_ROWS(256, 16)
-    DX_ROWS(1024, 8)
-    if constexpr (!REF) DX_ROWS(1024, 16)
+    DX_ROWS(512, REF ? 8 : 16)
+    DX_ROWS(1024, REF ? 8 : 16)
     DX_ROWS(1024, 0)
   }
 #undef DX_ROWS
@@ -909,8 +911,10 @@ int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
   }
   const RowShape sh = row_shape(a.V, dtype, REF, MODE != POLICY);
   const long long need = sh.T == 64 ? (a.rows + 3) / 4 : a.rows;
-  // resident workgroups: 1024 threads with 16 vectors each fill a CU
-  const long long most = MODE != POLICY ? 8LL * cus : sh.T == 1024 ? (sh.NV == 16 || REF ? cus : 2LL * cus) : 8LL * cus < kMaxWorkers ? 8LL * cus : kMaxWorkers;
+  // POLICY: resident workgroups, which prefetch their next row (1024 threads fill a CU).  Read once: as many as there are 64 KB
+  // pieces, as masked rows would leave resident ones with unequal shares (8192 rows of 64 KB, a fifth masked: 96 us, 81 so).
+  long long most = sh.T == 1024 ? cus : sh.T == 512 ? 2LL * cus : 8LL * cus < kMaxWorkers ? 8LL * cus : kMaxWorkers;
+  if (MODE != POLICY && most < a.rows * bytes / 65536) most = a.rows * bytes / 65536;
   const int grid = static_cast<int>(need < most ? need : most);
   *groups = grid;
   if (grid == 0) return DX_OK;
