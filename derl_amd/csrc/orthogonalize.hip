@@ -32,26 +32,33 @@ using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 constexpr float kScaleX = 4096.f, kScaleA = 256.f;
 constexpr int kOneTermRows = 640;  // bf16: with more rows A and B are held as one fp16 term too
-constexpr int kPad = 64, kBK = 64, kNormParts = 512;
-constexpr int kSplitGroups = 256;  // workgroups of a product that is split over K, at most; its tiles are half as many
+constexpr int kPad = 64, kNormParts = 512;
+constexpr int kSplitGroups = 512;  // workgroups of a product that is split over K, at most
 
 enum Epilogue { GRAM, POLY, UPDATE, FINAL };
 
-struct Terms { _Float16 *hi, *lo; };  // lo: unused with one term
+// A matrix of one term: rows of `ld` values.  Of two: rows of 2 ld, each 32 values' first terms followed by their second ones, so
+// that a cache line holds both terms of 32 k.
+template <int T>
+__device__ __forceinline__ long long place(long long row, int col, int ld) {
+  return T == 2 ? row * 2 * ld + (col >> 5) * 64 + (col & 31) : row * ld + col;
+}
+constexpr int kSecond = 32;  // from a value's first term to its second
 
 struct NsArgs {
-  Terms P, Q;             // operands: rows of K contiguous values
-  long long p_stride, q_stride;  // values from one matrix of the batch to the next
+  const _Float16 *P, *Q;  // operands: rows of K values
+  long long p_stride, q_stride;  // halves from one matrix of the batch to the next
   int ldp, ldq, K;
   int rows_p, rows_q;     // rows of P / Q, multiples of kPad
   int tiles_m, tiles_n;   // tiles of TM rows of them
-  Terms D, DT;            // [m][n] and its transpose [n][m]
+  _Float16 *D, *DT;       // [m][n] and its transpose [n][m]
   long long d_stride, dt_stride;
   int ldd, lddt;
   float a, b, c;
   // split K: `splits` workgroups a tile, each over `split_stages` stages; their sums, and a count of arrivals per tile
   int splits, split_stages;
   float *partials;
+  long long split_floats;  // of `partials`
   unsigned *arrivals;
   // FINAL
   void *out;
@@ -132,10 +139,12 @@ template <int TM, int WR, int WC, int PT, int QT, int OT, int RING, Epilogue EPI
 __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
   constexpr int kWaves = WR * WC, FM = TM / WR / 32, FN = TM / WC / 32;
-  constexpr int kArray = TM * kBK * 2;           // bytes of one operand term of a stage
-  constexpr int kStage = (PT + QT) * kArray;
+  // a stage: 64 k, or 32 where both operands have two terms; 128-byte lines of it per row of P and Q
+  constexpr int kStageK = PT + QT == 4 ? 32 : 64, kParts = kStageK / 16, PL = PT * kStageK / 64, QL = QT * kStageK / 64;
+  constexpr int kArray = TM * 128;               // bytes of a line of every row
+  constexpr int kStage = (PL + QL) * kArray;
   constexpr int NP = TM / 8 / kWaves;            // 1 KiB pieces (8 rows) of an array that a wave copies
-  constexpr int kPieces = (PT + QT) * NP;
+  constexpr int kPieces = (PL + QL) * NP;
   static_assert(NP * 8 * kWaves == TM && FM * 32 * WR == TM && FN * 32 * WC == TM, "tile");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -143,7 +152,7 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   int bm, bn, split;
   {
     // consecutive workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles
-    const int splits = EPI == GRAM && TM == 64 ? a.splits : 1, total = gridDim.x / splits, per = (total + 7) / 8, full = total - 8 * (per - 1);  // XCDs 0 .. full - 1 hold `per` tiles
+    const int splits = (EPI == GRAM || EPI == POLY) && TM <= 128 ? a.splits : 1, total = gridDim.x / splits, per = (total + 7) / 8, full = total - 8 * (per - 1);  // XCDs 0 .. full - 1 hold `per` tiles
     const int id = blockIdx.x / splits, xcd = id & 7, k = id >> 3;
     split = blockIdx.x - id * splits;
     int left = xcd * per - (xcd > full ? xcd - full : 0) + k;
@@ -159,29 +168,25 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
       bm = 4 * band + left % rows;
     }
   }
-  const _Float16 *src[PT + QT];
-  const long long p_at = z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp, q_at = z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq;
-  src[0] = a.P.hi + p_at;
-  if (PT == 2) src[PT - 1] = a.P.lo + p_at;
-  src[PT] = a.Q.hi + q_at;
-  if (QT == 2) src[PT + QT - 1] = a.Q.lo + q_at;
   uint32_t off[2][NP];
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
     const int R = (wave * NP + p) * 8 + (lane >> 3);
     const int chunk = (lane & 7) ^ ((R >> 1) & 7);
-    off[0][p] = static_cast<uint32_t>(min(R, a.rows_p - 1 - bm * TM)) * a.ldp * 2 + chunk * 16;
-    off[1][p] = static_cast<uint32_t>(min(R, a.rows_q - 1 - bn * TM)) * a.ldq * 2 + chunk * 16;
+    off[0][p] = static_cast<uint32_t>(min(R, a.rows_p - 1 - bm * TM)) * a.ldp * (2 * PT) + chunk * 16;
+    off[1][p] = static_cast<uint32_t>(min(R, a.rows_q - 1 - bn * TM)) * a.ldq * (2 * QT) + chunk * 16;
   }
-  const int first = split * a.split_stages, stages = min(a.split_stages, a.K / kBK - first);
-  const char *from[PT + QT];
+  const int first = split * a.split_stages, stages = min(a.split_stages, a.K / kStageK - first);
+  const char *from[PL + QL];
 #pragma unroll
-  for (int s = 0; s < PT + QT; ++s) from[s] = reinterpret_cast<const char *>(src[s] + static_cast<long long>(first) * kBK);
-  // piece k of the next stage to copy, into `slot`; the last one moves on
+  for (int s = 0; s < PL + QL; ++s)
+    from[s] = s < PL ? reinterpret_cast<const char *>(a.P + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp * PT) + first * (PL * 128LL) + s * 128
+                     : reinterpret_cast<const char *>(a.Q + z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq * QT) + first * (QL * 128LL) + (s - PL) * 128;
+  // piece k of the next stage to copy, into `slot`; an array's last one moves on
   auto copy = [&](int k, int slot) {
     const int s = k / NP, p = k % NP;
-    dma_piece(from[s], off[s < PT ? 0 : 1][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
-    if (p == NP - 1) from[s] += kBK * 2;
+    dma_piece(from[s], off[s < PL ? 0 : 1][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
+    if (p == NP - 1) from[s] += (s < PL ? PL : QL) * 128;
   };
   // a wave of one tile keeps a sum for each product and 16 k of a stage: dependent instructions issue at half the rate
   constexpr int kPairs = PT + QT - 1;  // products of terms: hi hi | lo hi, hi hi | lo hi, hi lo, hi hi
@@ -198,19 +203,26 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   }
   const int wm = wave / WC, wn = wave % WC, hi = lane >> 5, l31 = lane & 31;
   const unsigned x = (l31 >> 1) & 7;
+  // lane addresses in a line's array: of one term, 16 k of four; of two, 16 k of two and the term
   unsigned prow[4], qrow[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    prow[k] = (wm * FM * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
-    qrow[k] = PT * kArray + (wn * FN * 32 + l31) * 128 + ((2 * k + hi) ^ x) * 16;
+    const int pc = PT == 2 ? (k & 1) * 4 + (k >> 1) * 2 + hi : 2 * k + hi, qc = QT == 2 ? (k & 1) * 4 + (k >> 1) * 2 + hi : 2 * k + hi;
+    prow[k] = (wm * FM * 32 + l31) * 128 + (pc ^ x) * 16;
+    qrow[k] = PL * kArray + (wn * FN * 32 + l31) * 128 + (qc ^ x) * 16;
   }
   f16x8 p[2][PT][FM], q[2][QT][FN];
   // fragment k (of kReads) of 16 k of a slot
   constexpr int kReads = PT * FM + QT * FN, kProducts = kPairs * FM * FN;
   auto fetch = [&](int set, int slot, int part, int k) {
     const char *base = reinterpret_cast<const char *>(smem) + slot * kStage;
-    if (k < PT * FM) p[set][k / FM][k % FM] = *reinterpret_cast<const f16x8 *>(base + prow[part] + k / FM * kArray + k % FM * 4096);
-    else q[set][(k - PT * FM) / FN][(k - PT * FM) % FN] = *reinterpret_cast<const f16x8 *>(base + qrow[part] + (k - PT * FM) / FN * kArray + (k - PT * FM) % FN * 4096);
+    if (k < PT * FM) {
+      const int t = k / FM, i = k % FM;
+      p[set][t][i] = *reinterpret_cast<const f16x8 *>(base + (PT == 2 ? prow[(part & 1) * 2 + t] + part / 2 * kArray : prow[part]) + i * 4096);
+    } else {
+      const int t = (k - PT * FM) / FN, j = (k - PT * FM) % FN;
+      q[set][t][j] = *reinterpret_cast<const f16x8 *>(base + (QT == 2 ? qrow[(part & 1) * 2 + t] + part / 2 * kArray : qrow[part]) + j * 4096);
+    }
   };
   auto multiply = [&](int set, int k) {  // the small products first
     const int t = k / (FM * FN), i = k / FN % FM, j = k % FN;
@@ -246,8 +258,10 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   for (int s = 0; s < stages; ++s) {
     const int next = slot + 1 == RING ? 0 : slot + 1;
     part(0, slot, 1, 0, false, std::false_type{});
-    part(1, slot, 2, 0, false, std::false_type{});
-    part(0, slot, 3, 0, false, std::false_type{});
+    if constexpr (kParts == 4) {
+      part(1, slot, 2, 0, false, std::false_type{});
+      part(0, slot, 3, 0, false, std::false_type{});
+    }
     // this wave's copies of stage s + 1 have landed and all its reads of stage s are done; behind the barrier every wave's
     if (s + RING <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * kPieces) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -266,7 +280,7 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
       acc[0][0][e] = v;
     }
   }
-  if (EPI == GRAM && TM == 64 && a.splits > 1) {
+  if ((EPI == GRAM || EPI == POLY) && TM <= 128 && a.splits > 1) {
     // The last of the tile's workgroups to arrive adds all of them up in the order of their numbers (its own among them: the
     // result does not depend on who is last) and leaves the count at zero for the next launch.  The sums are exchanged by
     // relaxed agent-scope accesses, which pass the XCDs' own L2s by; a store has completed when vmcnt says so, and the count
@@ -317,13 +331,7 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   // per lane by a transposition within quads (8 bytes a lane, 64 a row), the transposed copy of eight rows per lane by
   // exchanging with the lane of the other half (16 bytes).
   constexpr bool two = OT == 2;
-  Terms D = a.D, DT = a.DT;
-  D.hi += z * a.d_stride;
-  DT.hi += z * a.dt_stride;
-  if (two) {
-    D.lo += z * a.d_stride;
-    DT.lo += z * a.dt_stride;
-  }
+  _Float16 *D = a.D + z * a.d_stride, *DT = a.DT + z * a.dt_stride;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -342,10 +350,10 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
         } else if constexpr (EPI == POLY) {
-          const long long at = z * a.p_stride + static_cast<long long>(n) * a.ldp + m;  // A[n][m] = A[m][n]
-          const f16x4 ah = *reinterpret_cast<const f16x4 *>(a.P.hi + at);
+          const _Float16 *at = a.P + z * a.p_stride + place<PT>(n, m, a.ldp);  // A[n][m] = A[m][n]
+          const f16x4 ah = *reinterpret_cast<const f16x4 *>(at);
           f16x4 al = {0, 0, 0, 0};
-          if (PT == 2) al = *reinterpret_cast<const f16x4 *>(a.P.lo + at);
+          if (PT == 2) al = *reinterpret_cast<const f16x4 *>(at + kSecond);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             v[k] = a.c * (v[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(ah[k]) + static_cast<float>(al[k])) +
@@ -371,26 +379,26 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
         l[g][0] = bl.x;
         l[g][1] = bl.y;
         if (EPI == UPDATE || bm != bn) {
-          const long long at = static_cast<long long>(m + (lane & 3)) * a.ldd + n0 + (l31 & ~3);
+          _Float16 *at = D + place<OT>(m + (lane & 3), n0 + (l31 & ~3), a.ldd);
           const Pair2 th = quad_transpose(bh.x, bh.y, lane);
-          *reinterpret_cast<u32x2 *>(D.hi + at) = u32x2{th.x, th.y};
+          *reinterpret_cast<u32x2 *>(at) = u32x2{th.x, th.y};
           if (two) {
             const Pair2 tl = quad_transpose(bl.x, bl.y, lane);
-            *reinterpret_cast<u32x2 *>(D.lo + at) = u32x2{tl.x, tl.y};
+            *reinterpret_cast<u32x2 *>(at + kSecond) = u32x2{tl.x, tl.y};
           }
         }
       }
       if constexpr (EPI != FINAL) {
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {  // groups g (kept by the lower half) and g + 1 (by the upper one): eight rows each
-          const long long at = static_cast<long long>(n) * a.lddt + m0 + 8 * (g + hi);
+          _Float16 *at = DT + place<OT>(n, m0 + 8 * (g + hi), a.lddt);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             swap_halves(h[g][k], h[g + 1][k]);
             if (two) swap_halves(l[g][k], l[g + 1][k]);
           }
-          *reinterpret_cast<u32x4 *>(DT.hi + at) = u32x4{h[g][0], h[g][1], h[g + 1][0], h[g + 1][1]};
-          if (two) *reinterpret_cast<u32x4 *>(DT.lo + at) = u32x4{l[g][0], l[g][1], l[g + 1][0], l[g + 1][1]};
+          *reinterpret_cast<u32x4 *>(at) = u32x4{h[g][0], h[g][1], h[g + 1][0], h[g + 1][1]};
+          if (two) *reinterpret_cast<u32x4 *>(at + kSecond) = u32x4{l[g][0], l[g][1], l[g + 1][0], l[g + 1][1]};
         }
       }
     }
@@ -435,8 +443,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long cou
 // X0 and its transpose from a 64 x 64 tile of G: `same` has G's orientation (ld_same), `turned` the other.  Also clears the
 // arrival counts of the split products.
 template <typename V, bool TWO>
-__global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n, const double *partials, int parts, float eps, Terms same,
-                                                      int ld_same, Terms turned, int ld_turned, long long stride, unsigned *arrivals, int counts) {
+__global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n, const double *partials, int parts, float eps, _Float16 *same,
+                                                      int ld_same, _Float16 *turned, int ld_turned, long long stride, unsigned *arrivals, int counts) {
   constexpr int E = 16 / sizeof(V);
   using Vec = __attribute__((ext_vector_type(E))) V;
   typedef Vec Loose __attribute__((aligned(sizeof(V))));
@@ -471,7 +479,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n,
   __syncthreads();
   const double factor = kScaleX / (sqrt(total[0] + total[1] + total[2] + total[3]) + eps);  // double: the norm may exceed fp32's range
   const int mp = (m + kPad - 1) / kPad * kPad, np = (n + kPad - 1) / kPad * kPad;
-  auto put8 = [&](const Terms &t, long long at, auto value) {
+  auto put8 = [&](_Float16 *at, auto value) {
     f16x8 h, l;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -479,14 +487,14 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n,
       h[i] = static_cast<_Float16>(v);
       l[i] = static_cast<_Float16>(v - static_cast<float>(h[i]));
     }
-    *reinterpret_cast<f16x8 *>(t.hi + at) = h;
-    if (TWO) *reinterpret_cast<f16x8 *>(t.lo + at) = l;
+    *reinterpret_cast<f16x8 *>(at) = h;
+    if (TWO) *reinterpret_cast<f16x8 *>(at + kSecond) = l;
   };
 #pragma unroll
   for (int k = 0; k < 2; ++k) {  // 64 rows of 8 x 8 values; the sides are multiples of 64: a row of 8 is whole or outside
     const int at = k * 256 + threadIdx.x, row = at >> 3, col = (at & 7) * 8;
-    if (r0 + row < mp && c0 + col < np) put8(same, z * stride + static_cast<long long>(r0 + row) * ld_same + c0 + col, [&](int i) { return tile[row][col + i]; });
-    if (c0 + row < np && r0 + col < mp) put8(turned, z * stride + static_cast<long long>(c0 + row) * ld_turned + r0 + col, [&](int i) { return tile[col + i][row]; });
+    if (r0 + row < mp && c0 + col < np) put8(same + z * stride + place<TWO ? 2 : 1>(r0 + row, c0 + col, ld_same), [&](int i) { return tile[row][col + i]; });
+    if (c0 + row < np && r0 + col < mp) put8(turned + z * stride + place<TWO ? 2 : 1>(c0 + row, r0 + col, ld_turned), [&](int i) { return tile[col + i][row]; });
   }
 }
 
@@ -718,8 +726,8 @@ int launch_small(const SmallArgs &q, int batch, int bytes, hipStream_t s) {
 
 struct Plan {
   int r, c, rp, cp, tx, ta, parts;  // tx, ta: terms of X, of A and B
-  long long x, sq;             // values of X and of A per matrix, padded
-  long long bytes;
+  long long x, sq;             // halves of X and of A per matrix, padded
+  long long split_floats, bytes;
 };
 Plan make_plan(int dtype, int batch, int m, int n) {
   Plan p;
@@ -729,12 +737,14 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   p.cp = (p.c + kPad - 1) / kPad * kPad;
   p.tx = dtype == DX_BF16 ? 1 : 2;
   p.ta = dtype == DX_BF16 && p.r > kOneTermRows ? 1 : 2;
-  p.x = static_cast<long long>(p.rp) * p.cp;
-  p.sq = static_cast<long long>(p.rp) * p.rp;
+  p.x = static_cast<long long>(p.rp) * p.cp * p.tx;
+  p.sq = static_cast<long long>(p.rp) * p.rp * p.ta;
+
   // X, two copies of X^T, A, B, and the norm's partial sums
   const long long blocks = (static_cast<long long>(m) * n + 8191) / 8192;  // 8192 elements a workgroup at least
   p.parts = static_cast<int>(blocks < kNormParts ? blocks : kNormParts);
-  p.bytes = batch * (2 * (3 * p.tx * p.x + 2 * p.ta * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4LL * kSplitGroups * 64 * 64;
+  p.split_floats = static_cast<long long>(kSplitGroups) * (p.r > 1024 ? 128 * 128 : 64 * 64);  // (128 x 128 tiles are split where there are many)
+  p.bytes = batch * (2 * (3 * p.x + 2 * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4 * p.split_floats;
   return p;
 }
 int check_shape(int dtype, int batch, int m, int n) {
@@ -746,54 +756,62 @@ int check_shape(int dtype, int batch, int m, int n) {
 
 template <int TM, int WR, int WC, int PT, int QT, int OT, int RING, Epilogue EPI>
 int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
-  constexpr int bytes = RING * (PT + QT) * TM * kBK * 2;
+  constexpr int kStageK = PT + QT == 4 ? 32 : 64, bytes = RING * (PT + QT) * kStageK / 64 * TM * 128;
   DX_LDS_OPT_IN((ns_gemm_kernel<TM, WR, WC, PT, QT, OT, RING, EPI>), bytes);
   a.tiles_m = cdiv(a.rows_p, TM);
   a.tiles_n = cdiv(a.rows_q, TM);
   const int tiles = EPI == GRAM || EPI == POLY ? a.tiles_m * (a.tiles_m + 1) / 2 : a.tiles_m * a.tiles_n;
-  a.split_stages = cdiv(a.K / kBK, splits);
-  a.splits = cdiv(a.K / kBK, a.split_stages);
+  a.split_stages = cdiv(a.K / kStageK, splits);
+  a.splits = cdiv(a.K / kStageK, a.split_stages);
   hipLaunchKernelGGL((ns_gemm_kernel<TM, WR, WC, PT, QT, OT, RING, EPI>), dim3(tiles * a.splits, batch), dim3(WR * WC * 64), bytes, s, a);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
-// The tile whose rounds over the CUs take the shortest: a stage's time is its copies' (about 28 bytes a cycle and CU), so a
-// round's goes with the tile's SIDE.  Measured (us for the whole operator, this product's tile changed): 4096^2 bf16 gram 1475
-// at 192 (253 tiles, one round), 1555 at 256, 1600 at 128; 3 x 1023 x 769 bf16 gram 227 at 64, 251 at 128, update 252 at 128,
-// 260 at 64; 2001 x 5003 f32 gram 1528 at 128, 1623 at 64.  Ties go to the smaller tile (its epilogue is shorter).
-// X X^T of a wide matrix has few tiles and a long K: K is split until the CUs are busy, where that saves more than the 4 us
-// that the exchange of the sums takes: 512 x 3136 f32 (36 tiles, 49 stages of 0.45 us) 276 us in one piece, 224 in seven;
-// 128 x 1000 bf16 (3 tiles, 16 stages of 0.2 us) 85 against 89 in four.
+// Tile side and parts of K for a product of `stages` stages, by the time that these constants give it (fitted to measured
+// products; us a stage of 128-byte lines).  A CU's copies bound the small tiles (28 bytes a cycle): a 64 or 128 tile costs 0.30
+// or 0.78 alone on a CU, 0.52 or 1.10 for two at a time (their ring lets two workgroups on a CU); 192 and 256 run alone, 1.2 and
+// 1.9 with the chip full, where the package's power bounds them.  Split parts exchange their sums: 8 us and 8 bytes a value.
+// Measured, us a product: 2001 x 5003 f32 X X^T at 128 one part 126, three parts 94; 64, 192, 256: 127, 170, 258; its
+// update 178, 147, 177, 139 at 64, 128, 192, 256.  512 x 3136 f32 X X^T at 64: one part 23, seven 14; its update 14.6, 22, 35, 52.
+struct Choice { int tile, splits; };
+Choice choose(long long batch, int rows_p, int rows_q, bool half, bool mixed, bool may_split, int stages, int cus, long long split_floats) {
+  Choice best{64, 1};
+  double best_time = 1e300;
+  for (int tile = 64; tile <= (mixed ? 128 : 256); tile += 64) {
+    const long long m = cdiv(rows_p, tile), n = cdiv(rows_q, tile), tiles = (half ? m * (m + 1) / 2 : m * n) * batch;
+    const double alone = tile == 64 ? 0.30 : tile == 128 ? 0.78 : tile == 192 ? 1.2 : 1.9, two = tile == 64 ? 0.52 : 1.10;
+    for (int splits = 1; splits <= (may_split && tile <= 128 ? 8 : 1); ++splits) {
+      const long long groups = tiles * splits;
+      if (splits > 1 && (stages / splits < 12 || groups > kSplitGroups || groups * tile * tile > split_floats)) break;
+      const long long slots = tile <= 128 ? 2LL * cus : cus, rest = groups % slots;
+      const double rounds = tile <= 128 ? groups / slots * two + (rest > cus ? two : rest ? alone : 0.0) : (groups / slots + (rest ? 1 : 0)) * alone;
+      const double time = rounds * cdiv(stages, splits) + (splits > 1 ? 8.0 + groups * tile * tile * 2e-6 : 0.0);
+      if (time < best_time * 0.97) {
+        best_time = time;
+        best = {tile, splits};
+      }
+    }
+  }
+  return best;
+}
 template <int PT, int QT, int OT, Epilogue EPI>
 int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
-  constexpr bool half = EPI == GRAM || EPI == POLY, single = PT + QT + OT == 3;
+  constexpr bool half = EPI == GRAM || EPI == POLY, mixed = PT + QT + OT == 4;
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
-  auto tiles = [&](int tile) {
-    const long long m = cdiv(a.rows_p, tile), n = cdiv(a.rows_q, tile);
-    return (half ? m * (m + 1) / 2 : m * n) * batch;
-  };
-  int best = 64;
-  for (int tile = 128; tile <= (single ? 256 : 128); tile += 64)
-    if ((tiles(tile) + cus - 1) / cus * tile < (tiles(best) + cus - 1) / cus * best) best = tile;
-  if constexpr (single) {
-    if (best == 256) return launch_tile<256, 2, 4, 1, 1, 1, 2, EPI>(a, batch, 1, s);
-    if (best == 192) return launch_tile<192, 2, 2, 1, 1, 1, 3, EPI>(a, batch, 1, s);
+  const Choice c = choose(batch, a.rows_p, a.rows_q, half, mixed, half, a.K / (PT + QT == 4 ? 32 : 64), cus, a.split_floats);
+  if constexpr (!mixed) {
+    if (c.tile == 256) return launch_tile<256, 2, 4, PT, QT, OT, 2, EPI>(a, batch, 1, s);
+    if (c.tile == 192) return launch_tile<192, 2, 2, PT, QT, OT, 3, EPI>(a, batch, 1, s);
   }
-  if (best == 128) return launch_tile<128, 2, 2, PT, QT, OT, 2, EPI>(a, batch, 1, s);
-  long long splits = 1;
-  if (EPI == GRAM && a.K / kBK >= (PT == 2 ? 16 : 32)) {
-    splits = (cus < kSplitGroups ? cus : kSplitGroups) / tiles(64);
-    if (splits > a.K / kBK / 6) splits = a.K / kBK / 6;
-    if (splits < 1) splits = 1;
-  }
-  return launch_tile<64, 2, 2, PT, QT, OT, 4, EPI>(a, batch, static_cast<int>(splits), s);
+  if (c.tile == 128) return launch_tile<128, 2, 2, PT, QT, OT, 2, EPI>(a, batch, c.splits, s);
+  return launch_tile<64, 2, 2, PT, QT, OT, mixed ? 3 : 4, EPI>(a, batch, c.splits, s);
 }
 // TX: terms of X, TA: of A and B
 template <int TX, int TA>
-int run_steps(const Plan &p, int batch, int steps, NsArgs a, Terms X, Terms XT0, Terms XT1, Terms A, Terms B, hipStream_t s) {
+int run_steps(const Plan &p, int batch, int steps, NsArgs a, _Float16 *X, _Float16 *XT0, _Float16 *XT1, _Float16 *A, _Float16 *B, hipStream_t s) {
   for (int k = 0; k < steps; ++k) {
-    const Terms xt = k & 1 ? XT1 : XT0, next = k & 1 ? XT0 : XT1;
+    _Float16 *xt = k & 1 ? XT1 : XT0, *next = k & 1 ? XT0 : XT1;
     NsArgs g = a;
     g.P = g.Q = X;
     g.p_stride = g.q_stride = p.x;
@@ -852,15 +870,12 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
     return launch_small<_Float16>(q, batch, bytes, s);
   }
   _Float16 *at = static_cast<_Float16 *>(workspace);
-  auto take = [&](long long values, int terms) {
-    Terms t;
-    t.hi = at;
-    at += values * batch;
-    t.lo = at;
-    if (terms == 2) at += values * batch;
+  auto take = [&](long long halves) {
+    _Float16 *t = at;
+    at += halves * batch;
     return t;
   };
-  const Terms X = take(p.x, p.tx), XT0 = take(p.x, p.tx), XT1 = take(p.x, p.tx), A = take(p.sq, p.ta), B = take(p.sq, p.ta);
+  _Float16 *X = take(p.x), *XT0 = take(p.x), *XT1 = take(p.x), *A = take(p.sq), *B = take(p.sq);
   double *partials = reinterpret_cast<double *>(at);
   unsigned *arrivals = reinterpret_cast<unsigned *>(partials + static_cast<long long>(batch) * p.parts);
   float *split = reinterpret_cast<float *>(arrivals + kSplitGroups);
@@ -871,7 +886,7 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   DX_LAUNCH_CHECK();
   const bool tall = m > n;
   const dim3 grid(cdiv(tall ? p.rp : p.cp, 64), cdiv(tall ? p.cp : p.rp, 64), batch);
-  const Terms same = tall ? XT0 : X, turned = tall ? X : XT0;
+  _Float16 *same = tall ? XT0 : X, *turned = tall ? X : XT0;
   const int ld_same = tall ? p.rp : p.cp, ld_turned = tall ? p.cp : p.rp;
   if (dtype == DX_F32)
     hipLaunchKernelGGL((ns_pack_kernel<float, true>), grid, dim3(256), 0, s, static_cast<const float *>(update), m, n, partials, p.parts, eps,
@@ -886,6 +901,7 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   NsArgs g{};
   g.arrivals = arrivals;
   g.partials = split;
+  g.split_floats = p.split_floats;
   g.a = a;
   g.b = b;
   g.c = c;
