@@ -130,10 +130,12 @@ __device__ __forceinline__ void unpack_raw(u32x4 v, float (&x)[D::E], int first,
 #pragma unroll
   for (int k = 0; k < D::E; ++k) x[k] = shift < D::E ? x[k] : -INFINITY;
 }
+// (gradients leave past the caches, which then keep logits for a pass that reads them again: preference loss of 512 MB of
+// logits 5.2 -> 5.8 TB/s over its three passes)
 template <class D>
 __device__ __forceinline__ void store_chunk(char *row, char *at, int t, int first, int V, bool ragged, const float (&x)[D::E]) {
   if (!ragged || first + D::E <= V) {
-    *reinterpret_cast<typename D::Vec *>(at + static_cast<uint32_t>(t) * 16) = D::pack(x);
+    __builtin_nontemporal_store(D::pack(x), reinterpret_cast<typename D::Vec *>(at + static_cast<uint32_t>(t) * 16));
     return;
   }
 #pragma unroll
@@ -346,7 +348,7 @@ __device__ __forceinline__ float grad_of(const RowPlan &g, float x, float y) {
   const float d = x - g.m, p = exp_of(d) * g.inv_s;
   float v = g.c0;
   if constexpr (ENT) v += g.c1 * fmaxf(d, kLowest);
-  if constexpr (REF) return p == 0.f ? 0.f : p * (v + g.c2 * (x - y));
+  if constexpr (REF) return p == 0.f ? 0.f : p * (g.c2 != 0.f ? v + g.c2 * (x - y) : v);  // (x - y may be infinite)
   return p * v;
 }
 
@@ -372,7 +374,7 @@ __device__ __forceinline__ RowPlan policy_row(const RowArgs &a, const RowStats &
   if (a.ref_lp) {  // e^d - 1 - d with d = log ref - log p >= 0, its expectation under p is the divergence
     const float d = ref - lp, em = expm1f(d);
     kl = em - d;
-    g -= a.kl_coef * em;
+    if (a.kl_coef != 0.f) g -= a.kl_coef * em;  // (0: the divergence, which may be infinite, is reported only)
   }
   if constexpr (REF) {
     shift = (r.m - r.mr) + logf(r.s / r.sr);  // difference of the two log-normalisers
@@ -381,7 +383,8 @@ __device__ __forceinline__ RowPlan policy_row(const RowArgs &a, const RowStats &
   *terms = {policy, H, kl, outside ? 1.f : 0.f, ratio, lp};
   // dz_j = w [ g (1{j = a} - p_j) + c_H p_j (log p_j + H) + c_K p_j (log p_j - log q_j - KL) ]
   const float c1 = w * a.ent_coef, c2 = REF ? w * a.kl_coef : 0.f;
-  return RowPlan{r.m, 1.f / r.s, w * (a.ent_coef * (H - log_s) - g) - c2 * (shift + kl), c1, c2, w * g};
+  const float c0 = w * (a.ent_coef * (H - log_s) - g);
+  return RowPlan{r.m, 1.f / r.s, c2 != 0.f ? c0 - c2 * (shift + kl) : c0, c1, c2, w * g};
 }
 
 __device__ __forceinline__ float row_weight(const RowArgs &a) {
@@ -428,7 +431,9 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const Row
     asm volatile("" : "+v"(lane_at));  // (opaque: sixteen addresses kept over the rows would spill)
     if ((k + 1) * T > vectors) lane_at = min(lane_at, vectors - 1 - k * T);
     const uint32_t at = static_cast<uint32_t>(lane_at) * 16;
-    v[k] = *reinterpret_cast<const typename D::Vec *>(a.z + row * a.z_pitch + k * T * 16 + at);
+    const auto *from = reinterpret_cast<const typename D::Vec *>(a.z + row * a.z_pitch + k * T * 16 + at);
+    // (the policy loss has no other use for them; 1001 x 32768 f32 4.9 -> 5.1 TB/s)
+    v[k] = MODE == POLICY ? __builtin_nontemporal_load(from) : *from;
     if constexpr (REF) u[k] = *reinterpret_cast<const typename D::Vec *>(a.q + row * a.q_pitch + k * T * 16 + at);
   };
   // nothing but -inf in the vectors that this thread does not have
@@ -553,7 +558,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const Row
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = grad_of<D, REF, ENT>(g, x[i], REF ? y[i] : 0.f);
             if ((k + 1) * T <= vectors || k * T + t < vectors)
-              *reinterpret_cast<typename D::Vec *>(dz + k * T * 16 + static_cast<uint32_t>(t) * 16) = D::pack(x);
+              __builtin_nontemporal_store(D::pack(x), reinterpret_cast<typename D::Vec *>(dz + k * T * 16 + static_cast<uint32_t>(t) * 16));
             __builtin_amdgcn_sched_barrier(0);
           }
           if (t < rest)
@@ -677,10 +682,19 @@ __global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a)
                              [&](float x, float y, int col) { return grad_of<D, REF, true>(g, x, y) + (col == action ? g.at : 0.f); });
 }
 
+// unmasked rows: 16 bytes of the mask at a time, a bit for each byte that is not 0
 __global__ __launch_bounds__(1024) void mask_count_kernel(const uint8_t *mask, long long n, double *count) {
+  typedef u32x4 Loose __attribute__((aligned(1)));
   __shared__ long long parts[16];
   long long c = 0;
-  for (long long i = threadIdx.x; i < n; i += 1024) c += mask[i] != 0;
+  const long long vectors = n / 16;
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < vectors; i += 1024) {
+    const u32x4 v = *reinterpret_cast<const Loose *>(mask + i * 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c += __popc((((v[k] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v[k]) & 0x80808080u);
+  }
+  if (vectors * 16 + threadIdx.x < n) c += mask[vectors * 16 + threadIdx.x] != 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
   if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = c;
@@ -715,7 +729,7 @@ __global__ __launch_bounds__(1024) void policy_terms_kernel(const double *partia
   if (threadIdx.x == 0) {
     const double c = count ? *count : static_cast<double>(rows);
     const double inv = c > 0 ? 1.0 / c : 0.0;  // nothing unmasked: zeros
-    loss_out[0] = static_cast<float>((s[0] - ent_coef * s[1] + kl_coef * s[2]) * inv);
+    loss_out[0] = static_cast<float>((s[0] - ent_coef * s[1] + (kl_coef != 0.f ? kl_coef * s[2] : 0.0)) * inv);
     for (int k = 0; k < 6; ++k) loss_out[k + 1] = static_cast<float>(s[k] * inv);
     loss_out[7] = static_cast<float>(c);
   }
@@ -787,7 +801,7 @@ __global__ __launch_bounds__(256) void preference_pairs_kernel(const PairArgs a)
 // dz_j = c (1{j = a} - p_j) of every row, c the coefficient of its sequence (0: no sequence's, or masked).  T threads take a
 // piece of a row; also the loss's terms, by the first workgroup.
 template <class D, int T>
-__global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, int pairs, int pair_groups, float *loss_out) {
+__global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, long long blocks, int pairs, int pair_groups, float *loss_out) {
   constexpr int kRows = 256 / T;
   const int t = threadIdx.x % T, slot = threadIdx.x / T;
   if (blockIdx.x == 0) {
@@ -798,18 +812,20 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, i
       loss_out[7] = static_cast<float>(pairs);
     }
   }
-  // from the last row down: the end of the logits is what the statistics pass has left in the last-level cache
-  const long long i = (blockIdx.x / a.splits) * static_cast<long long>(kRows) + slot;
-  if (i >= a.rows) return;
-  const long long row = a.rows - 1 - i;
-  const int begin = blockIdx.x % a.splits * a.piece, end = min(a.V, begin + a.piece);
-  const float4 st = a.stats[row];
-  char *dz = a.dz + row * a.dz_pitch;
-  const char *z = a.z + row * a.z_pitch;
-  const float c = st.w, k = -c * st.y;
-  const long long action = c != 0.f ? a.actions[row] : -1;
-  write_columns<D, T, false>(z, nullptr, dz, a.V, begin, end, t, c != 0.f,
-                             [&](float x, float, int col) { return k * exp_of(x - st.x) + (col == action ? c : 0.f); });
+  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
+    // from the last row down: the end of the logits is what the statistics pass has left in the last-level cache
+    const long long i = (block / a.splits) * kRows + slot;
+    if (i >= a.rows) return;
+    const long long row = a.rows - 1 - i;
+    const int begin = static_cast<int>(block % a.splits) * a.piece, end = min(a.V, begin + a.piece);
+    const float4 st = a.stats[row];
+    char *dz = a.dz + row * a.dz_pitch;
+    const char *z = a.z + row * a.z_pitch;
+    const float c = st.w, k = -c * st.y;
+    const long long action = c != 0.f ? a.actions[row] : -1;
+    write_columns<D, T, false>(z, nullptr, dz, a.V, begin, end, t, c != 0.f,
+                               [&](float x, float, int col) { return k * exp_of(x - st.x) + (col == action ? c : 0.f); });
+  }
 }
 
 // log-probabilities of sequences: a workgroup per sequence
@@ -875,9 +891,11 @@ int launch_rows(const RowArgs &a, RowShape sh, int grid, hipStream_t s) {
   return dx::fail(DX_ENOSUP, "token rows: no kernel for %d threads, %d vectors", sh.T, sh.NV);
 }
 template <class D>
-int launch_pref_grad(const RowArgs &a, int T, int grid, int pairs, int pair_groups, float *loss_out, hipStream_t s) {
-  if (T == 64) hipLaunchKernelGGL((preference_grad_kernel<D, 64>), dim3(grid), dim3(256), 0, s, a, pairs, pair_groups, loss_out);
-  else hipLaunchKernelGGL((preference_grad_kernel<D, 256>), dim3(grid), dim3(256), 0, s, a, pairs, pair_groups, loss_out);
+int launch_pref_grad(const RowArgs &a, int T, long long blocks, int pairs, int pair_groups, float *loss_out, hipStream_t s) {
+  // one workgroup at least, which writes the terms; fewer than 2^32 threads, the most of a launch
+  const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : blocks < (1 << 23) ? blocks : 1 << 23));
+  if (T == 64) hipLaunchKernelGGL((preference_grad_kernel<D, 64>), grid, dim3(256), 0, s, a, blocks, pairs, pair_groups, loss_out);
+  else hipLaunchKernelGGL((preference_grad_kernel<D, 256>), grid, dim3(256), 0, s, a, blocks, pairs, pair_groups, loss_out);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
@@ -1073,11 +1091,9 @@ extern "C" int dx_preference_loss(const void *logits, int dtype, long long rows,
   a.piece = T == 64 ? vocab : 32768 / elem_size(dtype);
   a.splits = (vocab - 1) / a.piece + 1;
   const long long blocks = (T == 64 ? (rows + 3) / 4 : rows) * a.splits;
-  DX_REQUIRE(blocks <= 0x7fffffffLL, "dx_preference_loss: %lld rows of %d logits are more than a launch takes", rows, vocab);
-  const int grid = blocks < 1 ? 1 : static_cast<int>(blocks);  // (the first workgroup also writes the terms)
-  if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, grid, pairs, pair_groups, loss_out, s);
-  if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, grid, pairs, pair_groups, loss_out, s);
-  return launch_pref_grad<ElemF16>(a, T, grid, pairs, pair_groups, loss_out, s);
+  if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, blocks, pairs, pair_groups, loss_out, s);
+  if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
+  return launch_pref_grad<ElemF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
 }
 
 extern "C" int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pitch, const float *factor, void *stream) {

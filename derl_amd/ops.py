@@ -360,8 +360,8 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
   Per unmasked row: ratio = exp(log p(action) - old_log_prob); ``-min(ratio A, clip(ratio, 1 - cliprange,
   1 + cliprange) A) - entropy_coef H + kl_coef KL`` (cliprange None: not clipped).  The divergence from
   the reference policy is estimated from the action alone, ``e^d - 1 - d`` with ``d = ref_log_prob - log p``,
-  or summed over the vocabulary where ``ref_logits`` are given (at most one of the two).  The loss is the
-  mean over the unmasked rows; ``global_batch`` > 0 divides the gradient by that instead (shards add up).
+  or summed over the vocabulary where ``ref_logits`` are given (at most one of the two); with kl_coef 0 it is
+  reported and takes no part, also where it is infinite.  The loss is the mean over the unmasked rows; ``global_batch`` > 0 divides the gradient by that instead (shards add up).
 
   logits (N, V) float32 / bfloat16 / float16 (rows contiguous, any row stride), actions (N,) int64,
   old_log_prob / advantages / ref_log_prob (N,) float32, ref_logits like logits, mask (N,) bool / uint8.
@@ -374,6 +374,8 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
     raise ValueError("give ref_log_prob or ref_logits, not both")
   if cliprange is not None and not cliprange >= 0:
     raise ValueError(f"cliprange must be None or >= 0, got {cliprange}")
+  if global_batch < 0:
+    raise ValueError(f"global_batch must be >= 0, got {global_batch}")
   ref_pitch = vocab
   if ref_logits is not None:
     _, _, ref_pitch = _rows_of(ref_logits, "ref_logits", like=logits)
@@ -414,6 +416,8 @@ def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothin
     raise ValueError(f"offsets must have 2 pairs + 1 entries, got {offsets.numel()}")
   if not 0 <= label_smoothing <= 1:
     raise ValueError(f"label_smoothing must lie in [0, 1], got {label_smoothing}")
+  if global_pairs < 0:
+    raise ValueError(f"global_pairs must be >= 0, got {global_pairs}")
   act = _vector(actions, "actions", rows, dev, _INDEX)
   ref = _vector(ref_log_prob, "ref_log_prob", sequences, dev, _FLOAT)
   keep = _vector(mask, "mask", rows, dev, _FLAG)
@@ -449,7 +453,9 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
   """Newton-Schulz orthogonalisation of (..., m, n) matrices: X = G / (|G|_F + eps), then ``steps`` times
   X <- a X + (b A + c A A) X with A = X X^T (of the shorter side).  The singular vectors stay, the singular
   values approach 1.  float32 or float16 (fp32 accuracy throughout) or bfloat16 (11-bit intermediates);
-  contiguous; the result has update's type and shape.  ``out`` may be ``update``.  A zero matrix gives zeros."""
+  contiguous; the result has update's type and shape.  ``out`` may be ``update``.  With eps > 0 a zero matrix gives
+  zeros; a matrix with a NaN or an infinity gives NaN.  Coefficients that let a singular value pass 8 on the way
+  leave fp16's range."""
   if not isinstance(update, torch.Tensor) or not update.is_cuda:
     raise ValueError("update must be a tensor on the GPU (derl_amd has no CPU path)")
   if update.dtype not in _ELEMENT_TYPES:
@@ -490,10 +496,10 @@ def muon_momentum(grads, momentum, update, partials, max_norm, mu, nesterov=True
     _dev(t, name, torch.float32)
     if t.numel() != grads.numel():
       raise ValueError(f"{name} must have {grads.numel()} elements, got {t.numel()}")
-  _lib.call("dx_muon_momentum_f32", _lib.ptr(grads), _lib.ptr(momentum), _lib.ptr(update), grads.numel(),
-            _lib.ptr(partials), 0 if partials is None else partials.numel(),
-            float(max_norm) if max_norm is not None else 0.0, float(mu), int(bool(nesterov)), _lib.ptr(norm_out),
-            _lib.stream_ptr(grads.device))
+  _call_on(grads.device, "dx_muon_momentum_f32", _lib.ptr(grads), _lib.ptr(momentum), _lib.ptr(update), grads.numel(),
+           _lib.ptr(partials), 0 if partials is None else partials.numel(),
+           float(max_norm) if max_norm is not None else 0.0, float(mu), int(bool(nesterov)), _lib.ptr(norm_out),
+           _lib.stream_ptr(grads.device))
 
 
 def muon_apply(params, update, decay, step):
@@ -502,5 +508,5 @@ def muon_apply(params, update, decay, step):
     _dev(t, name, torch.float32)
   if params.numel() != update.numel():
     raise ValueError(f"update must have {params.numel()} elements, got {update.numel()}")
-  _lib.call("dx_muon_apply_f32", _lib.ptr(params), _lib.ptr(update), params.numel(), float(decay), float(step),
-            _lib.stream_ptr(params.device))
+  _call_on(params.device, "dx_muon_apply_f32", _lib.ptr(params), _lib.ptr(update), params.numel(), float(decay), float(step),
+           _lib.stream_ptr(params.device))

@@ -410,6 +410,151 @@ def test_long_rows_past_32_bits():
     assert torch.equal(a, b)
 
 
+# more rows than a launch has workgroups for them, of every length that is held in registers, and longer ones
+MANY = [(2100, 4096), (2100, 8191), (2100, 16001), (600, 20011), (600, 32768), (300, 40003), (300, 65536), (300, 70001), (270, 131072),
+        (140, 140001)]
+
+
+@pytest.mark.parametrize("ref", ["none", "log_prob", "logits"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,vocab", MANY)
+def test_many_long_rows(rows, vocab, dtype, ref):
+  """The policy loss and the log-probabilities against 64 bits; the same bits in place and on rows at an odd distance; a
+  row that is NaN leaves the others alone."""
+  from derl_amd import ops
+  z, actions, old, adv, ref_lp, ref_z = policy_inputs(rows, vocab, dtype, rows + vocab)
+  ref_lp = ref_lp if ref == "log_prob" else None
+  ref_z = ref_z if ref == "logits" else None
+  mask = mask_of(rows, "some", rows)
+  ch = 0.01 if ref == "none" else 0.0
+  args = dict(kl_coef=0.1, entropy_coef=ch, ref_log_prob=ref_lp, ref_logits=ref_z, mask=mask)
+  got = ops.token_policy_loss(z, actions, old, adv, 0.2, **args)
+  want = policy_oracle(z, actions, old, adv, 0.2, 0.1, ch, ref_lp, ref_z, mask)
+  check_policy(got, want, vocab, dtype)
+  lp, entropy = ops.token_log_prob(z, actions, mask)
+  within(lp, want[3], slack(vocab) + 2.0 ** -23 * (want[3].abs() + 16), "log_prob")
+  h64 = torch.where(mask, rows64(z, actions)[2], 0.0)
+  within(entropy, h64, 2 * slack(vocab) * (1 + math.log(vocab + 1)) + 2.0 ** -22 * (h64 + 1), "entropy")
+  del want, h64
+  wide = torch.full((rows, vocab + 3), 7.0, dtype=dtype, device=DEV)
+  view = wide[:, 1:1 + vocab]
+  view.copy_(z)
+  again = ops.token_policy_loss(view, actions, old, adv, 0.2, dlogits_out=view, **args)
+  for a, b in zip(again, got):
+    assert torch.equal(a, b)
+  assert (wide[:, 0] == 7).all() and (wide[:, 1 + vocab:] == 7).all()
+  keep = torch.nonzero(mask)[:, 0]
+  bad = keep[[1, len(keep) // 2, len(keep) - 1]]
+  z[bad, vocab // 2] = float("nan")
+  again = ops.token_policy_loss(z, actions, old, adv, 0.2, **args)
+  assert torch.isnan(again[1][bad]).any(1).all() and torch.isnan(again[2][bad]).all()
+  rest = torch.ones(rows, dtype=torch.bool, device=DEV)
+  rest[bad] = False
+  assert torch.equal(again[1][rest], got[1][rest]) and torch.equal(again[2][rest], got[2][rest])
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(600_000, 5, F32), (540_000, 18, BF16), (140_000, 4100, BF16)])
+def test_more_than_64_rows_for_a_workgroup(rows, vocab, dtype):
+  """The same bits as when the rows come in parts (a global batch of the whole), and the sums of the parts' terms."""
+  from derl_amd import ops
+  z, actions = logits_of(rows, vocab, dtype, 5, banned=False)
+  old = -math.log(vocab) + 0.1 * torch.randn(rows, generator=gen(6), device=DEV)
+  adv = torch.randn(rows, generator=gen(7), device=DEV)
+  mask = mask_of(rows, "some", 8)
+  count = int(mask.sum())
+  loss, dz, lp = ops.token_policy_loss(z, actions, old, adv, 0.2, kl_coef=0.1, entropy_coef=0.01, ref_log_prob=old, mask=mask)
+  assert loss[7].item() == count
+  full, entropy = ops.token_log_prob(z, actions, mask)
+  # (rows that are read once are summed in another order than rows that are kept: each of the two is within its own error)
+  within(full, lp, 2 * (slack(vocab) + 2.0 ** -23 * (lp.abs() + 16)), "log_prob")
+  sums, parts = torch.zeros(7, dtype=torch.float64, device=DEV), 50_000 if vocab < 100 else 10_000
+  for at in range(0, rows, parts):
+    s = slice(at, at + parts)
+    l, d, p = ops.token_policy_loss(z[s], actions[s], old[s], adv[s], 0.2, kl_coef=0.1, entropy_coef=0.01, ref_log_prob=old[s], mask=mask[s],
+                                    global_batch=count)
+    assert torch.equal(d, dz[s]) and torch.equal(p, lp[s])
+    assert torch.equal(ops.token_log_prob(z[s], actions[s], mask[s])[1], entropy[s])
+    sums += l[:7].double() * l[7].double()
+  # the parts' means are rounded to fp32 each (2^-24 of values below 16), and so is the whole's
+  within(loss[:7], sums / count, torch.full((7,), 2.0 ** -19, dtype=torch.float64, device=DEV), "terms")
+
+
+def test_more_rows_than_threads_of_a_launch():
+  """70 million rows: the preference loss's gradient takes several blocks a workgroup."""
+  from derl_amd import ops
+  rows = 70_000_000
+  if torch.cuda.mem_get_info()[0] < 12e9:
+    pytest.skip("needs 8 GB of device memory")
+  z = torch.randn(rows, 2, generator=gen(1), device=DEV, dtype=F32).to(BF16)
+  actions = torch.randint(0, 2, (rows,), generator=gen(2), device=DEV)
+  mask = torch.ones(rows, dtype=torch.uint8, device=DEV)
+  mask[::3] = 0
+  offsets = torch.tensor([0, 5, 9, rows - 4, rows], dtype=torch.int32, device=DEV)
+  loss, dz, seq = ops.preference_loss(z, actions, offsets, None, 1e-6, mask=mask)
+  lp, _ = ops.token_log_prob(z, actions, mask)
+  want = torch.stack([lp[a:b].double().sum() for a, b in ((0, 5), (5, 9), (9, rows - 4), (rows - 4, rows))])
+  within(seq, want, 2.0 ** -23 * want.abs(), "sequences")
+  # a row's gradient: c (1 - p) and -c (1 - p), p the action's probability, c = -+ sigmoid(-h) 1e-6 / 2
+  h = 1e-6 * (want[0::2] - want[1::2])
+  c = torch.sigmoid(-h) * 1e-6 / 2
+  row = torch.cat([-c[0].expand(5), c[0].expand(4), -c[1].expand(rows - 13), c[1].expand(4)]) * (mask != 0)
+  for at in range(0, rows, 10_000_000):
+    s = slice(at, at + 10_000_000)
+    first = row[s] * (1 - torch.softmax(z[s].double(), 1).gather(1, actions[s, None])[:, 0])
+    got = dz[s].double().gather(1, actions[s, None])[:, 0]
+    within(got, first, half_step(first, BF16) + 2.0 ** -18 * row[s].abs(), "dlogits")
+    assert torch.equal(dz[s].gather(1, actions[s, None]), -dz[s].gather(1, 1 - actions[s, None])) or \
+        float((dz[s].double().sum(1).abs() / (row[s].abs() + 1e-30)).max()) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("kind", ["log_prob", "logits"])
+@pytest.mark.parametrize("vocab", [40, 5000, 40000])
+def test_a_divergence_that_is_only_reported(vocab, kind):
+  """kl_coef = 0: the divergence is reported, and where it is infinite neither the loss nor the gradient holds any of it."""
+  from derl_amd import ops
+  z, actions, old, adv, ref_lp, ref_z = policy_inputs(8, vocab, F32, 3)
+  want = ops.token_policy_loss(z, actions, old, adv, 0.2, entropy_coef=0.01)
+  ref_lp[2] = 1000.0
+  ref_z[2, 5::8] = -INF
+  args = dict(ref_log_prob=ref_lp) if kind == "log_prob" else dict(ref_logits=ref_z)
+  got = ops.token_policy_loss(z, actions, old, adv, 0.2, entropy_coef=0.01, **args)
+  assert got[0][3].item() == INF
+  within(got[0][[0, 1, 2, 4, 5, 6, 7]], want[0][[0, 1, 2, 4, 5, 6, 7]], 16 * slack(vocab) * (1 + math.log(vocab)), "terms")
+  _, dz, size, lp = policy_oracle(z, actions, old, adv, 0.2, 0.0, 0.01, None, None, None)
+  within(got[1], dz, 8 * slack(vocab) * size + half_step(dz, F32), "dlogits")
+
+
+@pytest.mark.parametrize("rows", [1, 15, 16, 17, 4099, 100_003])
+def test_mask_of_any_bytes_and_any_start(rows):
+  """A uint8 mask counts what is not 0, wherever it begins."""
+  from derl_amd import ops
+  z = torch.zeros(rows, 2, device=DEV)
+  actions = torch.zeros(rows, dtype=torch.int64, device=DEV)
+  one = torch.zeros(rows, device=DEV)
+  store = torch.randint(0, 256, (rows + 5,), generator=gen(rows), device=DEV, dtype=torch.uint8)
+  store[torch.rand(rows + 5, generator=gen(rows + 1), device=DEV) < 0.4] = 0
+  for start in (0, 1, 5):
+    mask = store[start:start + rows]
+    loss, dz, _ = ops.token_policy_loss(z, actions, one, one, 0.2, mask=mask)
+    assert loss[7].item() == int((mask != 0).sum())
+    assert not dz[mask == 0].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_the_same_index_twice_and_every_action(dtype):
+  """Rows that share an action, and each action of a vocabulary once, at widths around a wave's and a vector's."""
+  from derl_amd import ops
+  for vocab in (1, 7, 8, 9, 63, 64, 65, 515, 2051):
+    z, _, old, adv, ref_lp, _ = policy_inputs(vocab, vocab, dtype, vocab, clip=None)
+    z = logits_of(vocab, vocab, dtype, vocab, banned=False)[0]
+    for actions in (torch.arange(vocab, device=DEV), torch.full((vocab,), vocab - 1, device=DEV)):
+      got = ops.token_policy_loss(z, actions, old, adv, None, kl_coef=0.1, entropy_coef=0.01, ref_log_prob=ref_lp)
+      dz = policy_oracle(z, actions, old, adv, None, 0.1, 0.01, ref_lp, None, None)
+      s = slack(vocab)
+      within(got[2], dz[3], s + 2.0 ** -23 * (dz[3].abs() + 16), "log_prob")
+      within(got[1], dz[1], 8 * s * (dz[2] + 0.1 / vocab) + half_step(dz[1], dtype), "dlogits")
+
+
 # ---- orthogonalisation ---------------------------------------------------------------------------
 
 A, B, C = 3.4445, -4.7750, 2.0315
@@ -499,6 +644,25 @@ def test_orthogonalize_values():
   assert ops.orthogonalize(torch.zeros(4, 0, device=DEV)).shape == (4, 0)
 
 
+# every tile side, split and number of terms: one matrix and batches of them, sides that end inside a tile
+BATCHES = [(40, 318, 319), (40, 575, 570), (30, 700, 703), (16, 703, 700), (8, 704, 2111), (3, 700, 1500), (16, 959, 950), (40, 511, 127),
+           (16, 384, 1535), (40, 190, 1530), (1, 190, 1530), (1, 701, 5632), (1, 2001, 2100), (1, 4600, 1150), (1, 1150, 9200),
+           (1, 2900, 1300), (2, 3600, 3585)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("batch,m,n", BATCHES)
+def test_orthogonalize_batches(batch, m, n, dtype):
+  from derl_amd import ops
+  g = (torch.randn(batch, m, n, generator=gen(batch + m + n), device=DEV) * 0.02).to(dtype)
+  got = ops.orthogonalize(g, steps=3)
+  for k in {0, batch // 2, batch - 1}:
+    check_orthogonal(got[k], g[k], 3, dtype)
+  assert torch.equal(ops.orthogonalize(g, steps=3), got)  # split sums are added in one order
+  ops.orthogonalize(g, steps=3, out=g)
+  assert torch.equal(g, got)
+
+
 # ---- together ------------------------------------------------------------------------------------
 
 def test_refusals():
@@ -530,6 +694,17 @@ def test_refusals():
     ops.orthogonalize(g, out=torch.zeros(4, 5, device=DEV))
   with pytest.raises(ValueError):
     ops.orthogonalize(big[:6], out=big[1:])
+
+
+def test_negative_shares_and_too_many_matrices_are_refused():
+  from derl_amd import ops
+  z, actions, old, adv, _, _ = policy_inputs(6, 40, F32, 1)
+  with pytest.raises(ValueError, match="global_batch"):
+    ops.token_policy_loss(z, actions, old, adv, 0.2, global_batch=-1)
+  with pytest.raises(ValueError, match="global_pairs"):
+    ops.preference_loss(z, actions, torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV), None, 0.1, global_pairs=-1)
+  with pytest.raises(RuntimeError, match="batch"):
+    ops.orthogonalize(torch.zeros(65536, 2, 2, device=DEV))
 
 
 def test_no_rows():
