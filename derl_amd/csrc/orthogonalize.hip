@@ -428,6 +428,19 @@ __device__ __forceinline__ double sum_of_squares(const V *g, long long count, lo
   return s;
 }
 
+// kScaleX / (|G| + eps) as a fraction in [1/2, 1) and a power of two: the norm may lie outside fp32's range.  (A product in
+// double that goes on to fp16 is converted by 30 integer instructions: packing 512 x 3136 f32 took 14.4 us, 9.8 so.)
+struct Scale {
+  float fraction;
+  int power;
+};
+__device__ __forceinline__ Scale scale_of(double squares, float eps) {
+  Scale s;
+  s.fraction = static_cast<float>(frexp(kScaleX / (sqrt(squares) + eps), &s.power));
+  return s;
+}
+__device__ __forceinline__ float scaled(float x, const Scale &s) { return ldexpf(x * s.fraction, s.power); }
+
 // sums of squares, gridDim.x partial sums per matrix
 template <typename V>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long count, double *partials) {
@@ -455,35 +468,49 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n,
   const V *g = in + z * m * n;
   if (blockIdx.x == 0 && blockIdx.y == 0 && z == 0)
     for (int i = threadIdx.x; i < counts; i += 256) arrivals[i] = 0;
-  // 64 rows of 64 / E vectors
+  // 64 rows of 64 / E vectors, all on their way before the first is waited for
+  constexpr int kVecs = 64 * 64 / E / 256;
+  Vec v[kVecs];
+  if (r0 + 64 <= m && c0 + 64 <= n) {
 #pragma unroll
-  for (int k = 0; k < 64 * 64 / E / 256; ++k) {
-    const int at = k * 256 + threadIdx.x, row = at / (64 / E), col = at % (64 / E) * E;
-    Vec v = {};
-    if (r0 + row < m) {
-      const V *from = g + static_cast<long long>(r0 + row) * n + c0 + col;
-      if (c0 + col + E <= n) v = *reinterpret_cast<const Loose *>(from);
-      else
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (c0 + col + i < n) v[i] = from[i];
+    for (int k = 0; k < kVecs; ++k) {
+      const int at = k * 256 + threadIdx.x;
+      v[k] = *reinterpret_cast<const Loose *>(g + static_cast<long long>(r0 + at / (64 / E)) * n + c0 + at % (64 / E) * E);
     }
+  } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) tile[row][col + i] = static_cast<float>(v[i]);
+    for (int k = 0; k < kVecs; ++k) {
+      const int at = k * 256 + threadIdx.x, row = at / (64 / E), col = at % (64 / E) * E;
+      v[k] = Vec{};
+      if (r0 + row < m) {
+        const V *from = g + static_cast<long long>(r0 + row) * n + c0 + col;
+        if (c0 + col + E <= n) v[k] = *reinterpret_cast<const Loose *>(from);
+        else
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if (c0 + col + i < n) v[k][i] = from[i];
+      }
+    }
   }
   double s = 0;
   for (int i = threadIdx.x; i < parts; i += 256) s += partials[z * parts + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = s;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int at = k * 256 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < E; ++i) tile[at / (64 / E)][at % (64 / E) * E + i] = static_cast<float>(v[k][i]);
+  }
   __syncthreads();
-  const double factor = kScaleX / (sqrt(total[0] + total[1] + total[2] + total[3]) + eps);  // double: the norm may exceed fp32's range
+  const Scale scale = scale_of(total[0] + total[1] + total[2] + total[3], eps);
   const int mp = (m + kPad - 1) / kPad * kPad, np = (n + kPad - 1) / kPad * kPad;
   auto put8 = [&](_Float16 *at, auto value) {
     f16x8 h, l;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float v = static_cast<float>(value(i) * factor);
+      const float v = scaled(value(i), scale);
       h[i] = static_cast<_Float16>(v);
       l[i] = static_cast<_Float16>(v - static_cast<float>(h[i]));
     }
@@ -573,7 +600,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
   s = 0;
 #pragma unroll
   for (int i = 0; i < kSmallWaves; ++i) s += parts[i];
-  const double factor = kScaleX / (sqrt(s) + a.eps);
+  const Scale scale = scale_of(s, a.eps);
   for (int row = wave; row < a.rp; row += kSmallWaves)  // a wave per row of X, 256 columns' loads at a time
     for (int col0 = lane; col0 < a.cp; col0 += 256) {
       V g[4];
@@ -586,7 +613,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
       for (int k = 0; k < 4; ++k) {
         const int col = col0 + 64 * k;
         if (col >= a.cp) continue;
-        const float v = row < a.r && col < a.c ? static_cast<float>(static_cast<float>(g[k]) * factor) : 0.f;
+        const float v = row < a.r && col < a.c ? scaled(static_cast<float>(g[k]), scale) : 0.f;
         put1(X + row * ldx + col, sx, v);
         put1(XT + col * ldr + row, st, v);
       }
