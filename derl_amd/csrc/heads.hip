@@ -982,9 +982,9 @@ __global__ __launch_bounds__(kFbThreads) void tail_loss_bwd_kernel(const TailLos
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31;
   const int A = a.A;
   const LossParams lparams{a.A, a.mode, a.stats != nullptr, a.cliprange, a.value_loss_coef, a.entropy_coef, a.inv_batch};
-  // Up to six outputs: in PAIRS (2 jp, 2 jp + 1) -- one v_pk_fma_f32 multiplies a y2 element by both rows' weights (and, in
-  // the backward half, adds both rows' dL/dout x y2 to G): the fp32 vector peak needs the packed form; every element's own
-  // fma chain is the one the unpacked code forms.  An odd NJ carries a zero row.  Seven and eight outputs stay unpacked
+  // Up to six outputs: in PAIRS (2 jp, 2 jp + 1) -- a y2 element meets both rows' weights (and, in the backward half, both
+  // rows' dL/dout x y2 are added to G) side by side; packed fp32 instructions are off for this build, so a pair is two fmas,
+  // and every element's own fma chain is the one the unpacked code forms.  An odd NJ carries a zero row.  Seven and eight outputs stay unpacked
   // (the aligned register pairs spill there).
   constexpr bool PACK = NJ <= 6;
   constexpr int NP = (NJ + 1) / 2, NR = PACK ? NP : NJ;  // register rows of wc / g
