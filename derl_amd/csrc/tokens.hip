@@ -874,11 +874,13 @@ inline int elem_size(int dtype) { return dtype == DX_F32 ? 4 : 2; }
 
 // Threads per row T and vectors of 16 bytes a thread holds of it, NV (0: none, or too many for the registers).
 struct RowShape { int T, NV; };
-RowShape row_shape(int V, int dtype, bool ref, bool once) {
+RowShape row_shape(int V, int dtype, bool ref, bool once, bool few) {
   const long long vectors = (static_cast<long long>(V) * elem_size(dtype) + 15) / 16;
   if (vectors <= 64) return {64, 1};
   if (vectors <= 64 * 8) return {64, vectors <= 64 * 4 ? 4 : 8};
-  if (once) return {256, 0};  // read once anyway: the more waves, the more is on its way
+  // read once anyway: many rows to a CU, or, where there are no more rows than CUs, many threads to a row (32 x 32768 f32 log-
+  // probabilities: 6.0 us with 1024 threads, 7.6 with 256; 32 x 12000 bf16 4.7, 5.0; shorter ones alike)
+  if (once) return {few && vectors > 1024 ? 1024 : 256, 0};
   const int most = ref ? 8 : 16;  // two rows are held where there are reference logits
   if (vectors <= 256 * most) return {256, vectors <= 256 * 4 ? 4 : vectors <= 256 * 8 ? 8 : 16};
   if (vectors <= 512 * most) return {512, most};
@@ -899,6 +901,7 @@ int launch_rows(const RowArgs &a, RowShape sh, int grid, hipStream_t s) {
   DX_ROWS(64, 8)
   if constexpr (MODE != POLICY) {
     DX_ROWS(256, 0)
+    DX_ROWS(1024, 0)
   } else {
     DX_ROWS(256, 4)
     DX_ROWS(256, 8)
@@ -921,13 +924,16 @@ int launch_pref_grad(const RowArgs &a, int T, long long blocks, int pairs, int p
 }
 
 // Rows -> statistics (LOGP, STATS: results too) or the whole policy loss.  `*groups`: rows of `partials` that were written.
-// Few long rows are cut into pieces over the CUs and joined by a second launch.
+// Few long rows are cut into pieces over the CUs and joined by a second launch: long is what a CU takes longer for than the
+// launches cost (its exponentials bound it, so columns count, not bytes).  32 rows of bf16, GPU us / us with the host's part,
+// whole and in pieces: log-probabilities of 32768 columns 5.8 / 10.5, 6.0 / 13.1; of 65536 8.0 / 9.9, 6.1 / 13.0; of 131072
+// 12.3 / 12.7, 6.9 / 13.3; policy loss of 16384 11.2 / 17.3, 10.6 / 22.3; of 32768 14.7 / 17.6, 10.7 / 22.1; of 131072 26 / 26, 13 / 23.
 template <class D, Mode MODE, bool REF, bool ENT>
 int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
   int cus = 0;
   if (int rc = dx::device_cus(&cus)) return rc;
   const long long bytes = static_cast<long long>(a.V) * elem_size(dtype);
-  if (a.rows <= kMaxPieces / 2 && bytes >= 32768 && a.rows * 2 <= cus) {
+  if (a.rows <= kMaxPieces / 2 && a.V > (MODE == POLICY ? 16384 : 32768) && a.rows * 2 <= cus) {
     long long splits = cus / a.rows, most = (bytes + 8191) / 8192;
     if (splits > most) splits = most;
     if (splits * a.rows > kMaxPieces) splits = kMaxPieces / a.rows;
@@ -947,7 +953,7 @@ int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
       return DX_OK;
     }
   }
-  const RowShape sh = row_shape(a.V, dtype, REF, MODE != POLICY);
+  const RowShape sh = row_shape(a.V, dtype, REF, MODE != POLICY, a.rows <= cus);
   const long long need = sh.T == 64 ? (a.rows + 3) / 4 : a.rows;
   // POLICY: resident workgroups, which prefetch their next row (1024 threads fill a CU).  Read once: as many as there are 64 KB
   // pieces, as masked rows would leave resident ones with unequal shares (8192 rows of 64 KB, a fifth masked: 96 us, 81 so).
