@@ -135,7 +135,7 @@ class NativeError(RuntimeError):
 DX_EINVAL, DX_EHIP, DX_ENOSUP, DX_EWS, DX_ETIMEOUT = -1, -2, -3, -4, -5
 # element types and the scratch of the token losses (doubles), include/derl_amd.h
 DX_F32, DX_BF16, DX_F16 = 0, 1, 2
-DX_TOKEN_WORKSPACE = 19464
+DX_TOKEN_WORKSPACE = 18056
 
 
 def load():

@@ -338,7 +338,7 @@ struct RowArgs {
   // rows cut into `splits` pieces of `piece` columns (a multiple of 2048)
   int splits, piece;
   RowStats *piece_stats;
-  struct RowPlan *plans;
+  float *chosen;  // POLICY: the action's logit of each row
 };
 
 enum Mode { LOGP, STATS, POLICY };
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const Row
 }
 
 // ---- few rows: every row cut into pieces, a workgroup each ----------------------------------------------------------
-template <class D, bool REF>
+template <class D, Mode MODE, bool REF>
 __global__ __launch_bounds__(256) void token_pieces_kernel(const RowArgs a) {
   __shared__ RowStats parts[2][4];
   const long long row = blockIdx.y;
@@ -652,28 +652,17 @@ __global__ __launch_bounds__(256) void token_pieces_kernel(const RowArgs a) {
   int turn = 0;
   add_columns<D, 256, REF>(r, z, q, a.V, begin, end, threadIdx.x);
   join_row<4, REF>(r, parts, turn);
-  if (threadIdx.x == 0) a.piece_stats[row * a.splits + blockIdx.x] = r;
+  if (threadIdx.x == 0) {
+    a.piece_stats[row * a.splits + blockIdx.x] = r;
+    if (MODE == POLICY && blockIdx.x == 0) a.chosen[row] = action_logit<D>(z, a.actions[row], a.V);  // (the gradient may overwrite it)
+  }
 }
 
-// the pieces of a row joined, a wave per row, and the row's results
-template <class D, Mode MODE, bool REF>
-__global__ __launch_bounds__(64) void token_join_kernel(const RowArgs a) {
-  const int lane = threadIdx.x;
-  const long long row = blockIdx.x;
-  if (a.mask && !a.mask[row]) {
-    if (lane == 0) {
-      if (MODE != STATS) a.lp[row] = 0.f;
-      if (MODE == LOGP && a.entropy) a.entropy[row] = 0.f;
-      if (MODE == STATS) a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (MODE == POLICY) {
-        a.plans[row] = RowPlan{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < 8; ++k) a.partials[row * 8 + k] = 0.0;
-      }
-    }
-    return;
-  }
+// the pieces of a row joined, in every lane of a wave
+template <bool REF>
+__device__ __forceinline__ RowStats join_pieces(const RowArgs &a, long long row) {
   RowStats r = kNothing;
-  for (int i = lane; i < a.splits; i += 64) {
+  for (int i = threadIdx.x & 63; i < a.splits; i += 64) {
     const RowStats p = a.piece_stats[row * a.splits + i];
     RowStats q = p;
     raise_max(q, r.m);
@@ -688,31 +677,51 @@ __global__ __launch_bounds__(64) void token_join_kernel(const RowArgs a) {
     }
   }
   join_wave<REF>(r);
-  const float za = action_logit<D>(a.z + row * a.z_pitch, a.actions[row], a.V);
-  const float log_s = logf(r.s);
-  const float lp = (za - r.m) - log_s;
-  if constexpr (MODE == POLICY) {
-    RowTerms out;
-    const RowPlan g = policy_row<REF>(a, r, za, a.old_lp[row], a.adv[row], a.ref_lp ? a.ref_lp[row] : 0.f, row_weight<1>(a), &out);
-    if (lane == 0) {
-      a.plans[row] = g;
-      const double all[8] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp, 0.0, 0.0};
-      for (int k = 0; k < 8; ++k) a.partials[row * 8 + k] = all[k];
-    }
+  return r;
+}
+
+// the results of the rows, a wave per row
+template <class D, Mode MODE>
+__global__ __launch_bounds__(64) void token_join_kernel(const RowArgs a) {
+  const int lane = threadIdx.x;
+  const long long row = blockIdx.x;
+  const bool keep = !a.mask || a.mask[row];
+  float lp = 0.f, entropy = 0.f;
+  float4 stats = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (keep) {
+    const RowStats r = join_pieces<false>(a, row);
+    const float log_s = logf(r.s);
+    lp = (action_logit<D>(a.z + row * a.z_pitch, a.actions[row], a.V) - r.m) - log_s;
+    entropy = log_s - r.ed / r.s;
+    stats = make_float4(r.m, 1.f / r.s, lp, 0.f);
   }
   if (lane == 0) {
-    if (MODE != STATS) a.lp[row] = lp;
-    if (MODE == LOGP && a.entropy) a.entropy[row] = log_s - r.ed / r.s;
-    if (MODE == STATS) a.stats[row] = make_float4(r.m, 1.f / r.s, lp, 0.f);
+    if (MODE == LOGP) a.lp[row] = lp;
+    if (MODE == LOGP && a.entropy) a.entropy[row] = entropy;
+    if (MODE == STATS) a.stats[row] = stats;
   }
 }
 
+// the gradient of a piece; every workgroup joins its row's pieces itself (another launch would take longer), the first one of
+// a row writes its results
 template <class D, bool REF>
 __global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a) {
   const long long row = blockIdx.y;
   const bool keep = !a.mask || a.mask[row];
-  const RowPlan g = a.plans[row];
-  const long long action = keep ? a.actions[row] : -1;
+  RowTerms out = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  RowPlan g = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  long long action = -1;
+  if (keep) {
+    const float w = row_weight<4>(a);
+    const RowStats r = join_pieces<REF>(a, row);
+    g = policy_row<REF>(a, r, a.chosen[row], a.old_lp[row], a.adv[row], a.ref_lp ? a.ref_lp[row] : 0.f, w, &out);
+    action = a.actions[row];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.lp[row] = out.lp;
+    const double all[8] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp, 0.0, 0.0};
+    for (int k = 0; k < 8; ++k) a.partials[row * 8 + k] = all[k];
+  }
   const int begin = blockIdx.x * a.piece, end = min(a.V, begin + a.piece);
   const char *z = a.z + row * a.z_pitch, *q = REF ? a.q + row * a.q_pitch : nullptr;
   char *dz = a.dz + row * a.dz_pitch;
@@ -927,7 +936,7 @@ int launch_pref_grad(const RowArgs &a, int T, long long blocks, int pairs, int p
 // Few long rows are cut into pieces over the CUs and joined by a second launch: long is what a CU takes longer for than the
 // launches cost (its exponentials bound it, so columns count, not bytes).  32 rows of bf16, GPU us / us with the host's part,
 // whole and in pieces: log-probabilities of 32768 columns 5.8 / 10.5, 6.0 / 13.1; of 65536 8.0 / 9.9, 6.1 / 13.0; of 131072
-// 12.3 / 12.7, 6.9 / 13.3; policy loss of 16384 11.2 / 17.3, 10.6 / 22.3; of 32768 14.7 / 17.6, 10.7 / 22.1; of 131072 26 / 26, 13 / 23.
+// 12.3 / 12.7, 6.9 / 13.3; policy loss of 16384 11.3 / 17.3, 9 / 19.5; of 32768 14.7 / 17.6, 9.2 / 19.6; of 131072 26 / 26, 12 / 19.6.
 template <class D, Mode MODE, bool REF, bool ENT>
 int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
   int cus = 0;
@@ -941,14 +950,11 @@ int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
     a.splits = (a.V + a.piece - 1) / a.piece;
     if (a.splits > 1) {
       const dim3 grid(a.splits, static_cast<unsigned>(a.rows));
-      hipLaunchKernelGGL((token_pieces_kernel<D, REF>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((token_pieces_kernel<D, MODE, REF>), grid, dim3(256), 0, s, a);
       DX_LAUNCH_CHECK();
-      hipLaunchKernelGGL((token_join_kernel<D, MODE, REF>), dim3(static_cast<unsigned>(a.rows)), dim3(64), 0, s, a);
+      if constexpr (MODE == POLICY) hipLaunchKernelGGL((token_pieces_grad_kernel<D, REF>), grid, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((token_join_kernel<D, MODE>), dim3(static_cast<unsigned>(a.rows)), dim3(64), 0, s, a);
       DX_LAUNCH_CHECK();
-      if (MODE == POLICY) {
-        hipLaunchKernelGGL((token_pieces_grad_kernel<D, REF>), grid, dim3(256), 0, s, a);
-        DX_LAUNCH_CHECK();
-      }
       *groups = static_cast<int>(a.rows);
       return DX_OK;
     }
@@ -989,9 +995,9 @@ int check_logits(const char *who, const void *logits, int dtype, long long rows,
   return DX_OK;
 }
 
-// workspace, in doubles: 8 for the count, 8 a workgroup for its sums, the pieces' statistics and the rows' plans
-constexpr int kPartialsAt = 8, kPiecesAt = 8 + 8 * kMaxWorkers, kPlansAt = kPiecesAt + kMaxPieces * 3;
-static_assert(sizeof(RowStats) == 24 && sizeof(RowPlan) == 24 && kPlansAt + kMaxPieces * 3 == DX_TOKEN_WORKSPACE, "workspace");
+// workspace, in doubles: 8 for the count, 8 a workgroup for its sums, the pieces' statistics and their rows' chosen logits
+constexpr int kPartialsAt = 8, kPiecesAt = 8 + 8 * kMaxWorkers, kChosenAt = kPiecesAt + kMaxPieces * 3;
+static_assert(sizeof(RowStats) == 24 && kChosenAt + kMaxPieces / 4 == DX_TOKEN_WORKSPACE, "workspace");
 
 RowArgs row_args(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions, const uint8_t *mask,
                  double *workspace) {
@@ -1000,7 +1006,7 @@ RowArgs row_args(const void *logits, int dtype, long long rows, int vocab, long 
   a.count = workspace;
   a.partials = workspace + kPartialsAt;
   a.piece_stats = reinterpret_cast<RowStats *>(workspace + kPiecesAt);
-  a.plans = reinterpret_cast<RowPlan *>(workspace + kPlansAt);
+  a.chosen = reinterpret_cast<float *>(workspace + kChosenAt);
   const int size = elem_size(dtype);
   a.z = static_cast<const char *>(logits);
   a.z_pitch = pitch * size;

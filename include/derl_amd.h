@@ -219,7 +219,7 @@ int dx_reward_summary_f32(const float *rewards, const uint8_t *resets, int T, in
 #define DX_F32 0
 #define DX_BF16 1
 #define DX_F16 2
-#define DX_TOKEN_WORKSPACE 19464
+#define DX_TOKEN_WORKSPACE 18056
 int dx_token_log_prob(const void *logits, int dtype, long long rows, int vocab, long long pitch,
                       const int64_t *actions, const uint8_t *mask, float *log_prob, float *entropy,
                       double *workspace, long long workspace_count, void *stream);
