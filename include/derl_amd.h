@@ -201,6 +201,7 @@ int dx_reward_summary_f32(const float *rewards, const uint8_t *resets, int T, in
  *        -min(ratio A, clip(ratio, 1 - cliprange, 1 + cliprange) A) (cliprange < 0: no clipping)
  *        - entropy_coef H + kl_coef KL, with KL = e^d - 1 - d, d = ref_log_prob - lp, or with
  *        ref_logits (same dtype, rows ref_pitch apart) the divergence sum_j p_j (log p_j - log q_j).
+ *        kl_coef 0: the divergence is reported and takes no part, also where it is infinite.
  *        dlogits = gradient of the mean over the unmasked rows (global_batch > 0: of the sum divided
  *        by global_batch, so that shards add up); dlogits may be logits (in place).
  *        loss_out[8] = {loss, policy loss, entropy, KL, share of clipped ratios, mean ratio, mean lp,

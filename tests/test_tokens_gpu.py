@@ -555,6 +555,42 @@ def test_the_same_index_twice_and_every_action(dtype):
       within(got[1], dz[1], 8 * s * (dz[2] + 0.1 / vocab) + half_step(dz[1], dtype), "dlogits")
 
 
+def test_the_longest_rows():
+  """Two rows of 2^30 - 3 columns, nearly 4 GB each.  A thread adds at most 2^15 columns to its sum (128 pieces of 256
+  threads a row): 2^15 roundings of 2^-24 each, and the joins' 60."""
+  from derl_amd import ops
+  rows, vocab = 2, 2 ** 30 - 3
+  if torch.cuda.mem_get_info()[0] < 40e9:
+    pytest.skip("needs 40 GB of device memory")
+  z = torch.empty(rows, vocab, device=DEV)
+  z.normal_(generator=gen(1))
+  actions = torch.tensor([vocab - 1, vocab // 2 + 5], device=DEV)
+  z[0, vocab - 1], z[1, vocab // 2 + 5] = 24.0, 21.0
+  total = torch.zeros(rows, dtype=torch.float64, device=DEV)
+  for at in range(0, vocab, 1 << 27):
+    total += z[:, at:at + (1 << 27)].double().exp().sum(1)
+  want = z.gather(1, actions[:, None])[:, 0].double() - total.log()
+  s = (2 ** 15 + 60) * 2.0 ** -24
+  lp, _ = ops.token_log_prob(z, actions)
+  within(lp, want, s + 2.0 ** -23 * (want.abs() + 32), "log_prob")
+  old, adv = want.float() - 0.05, torch.tensor([1.0, -2.0], device=DEV)
+  _, dz, lp = ops.token_policy_loss(z, actions, old, adv, 0.2)
+  within(lp, want, s + 2.0 ** -23 * (want.abs() + 32), "log_prob")
+  g = -(want - old.double()).exp() * adv.double() / 2
+  offsets = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+  _, dz2, seq = ops.preference_loss(z, actions, offsets, None, 0.5)
+  slope = -0.5 * torch.sigmoid(-0.5 * (want[0] - want[1]))
+  c = torch.stack([slope, -slope])
+  for first in (0, vocab // 2 - 500, vocab - 1000):
+    at = torch.arange(first, first + 1000, device=DEV)
+    p = z[:, first:first + 1000].double().exp() / total[:, None]
+    onehot = (at[None] == actions[:, None]).double()
+    for got, k in ((dz, g), (dz2, c)):
+      size = k.abs()[:, None] * (onehot + p)
+      exact = k[:, None] * (onehot - p)
+      within(got[:, first:first + 1000], exact, 8 * s * size + half_step(exact, F32), "dlogits")
+
+
 # ---- orthogonalisation ---------------------------------------------------------------------------
 
 A, B, C = 3.4445, -4.7750, 2.0315
@@ -642,6 +678,23 @@ def test_orthogonalize_values():
       assert torch.equal(got[i, j], ops.orthogonalize(nested[i, j].contiguous()))
   assert ops.orthogonalize(torch.zeros(0, 4, 5, device=DEV)).shape == (0, 4, 5)
   assert ops.orthogonalize(torch.zeros(4, 0, device=DEV)).shape == (4, 0)
+
+
+@pytest.mark.parametrize("shape", [(40, 60), (130, 500)])
+def test_orthogonalize_at_the_ends_of_the_range(shape):
+  """Powers of two change nothing but the smallest entries, which may round to multiples of 2^-149 (2^-29 of entries of
+  2^-120); an infinity, like a NaN, leaves nothing."""
+  from derl_amd import ops
+  g = torch.randn(shape, generator=gen(7), device=DEV)
+  base = ops.orthogonalize(g, eps=0.0)
+  for scale in (2.0 ** 120, 2.0 ** -120, -1.0):
+    got = ops.orthogonalize(g * scale, eps=0.0)
+    assert float((got * math.copysign(1.0, scale) - base).abs().max()) <= 2.0 ** -18, scale
+  for bad in (INF, -INF, float("nan")):
+    broken = g.clone()
+    broken[3, 5] = bad
+    assert torch.isnan(ops.orthogonalize(broken)).all()
+  assert torch.isnan(ops.orthogonalize(torch.zeros(shape, device=DEV), eps=0.0)).all()
 
 
 # every tile side, split and number of terms: one matrix and batches of them, sides that end inside a tile
