@@ -832,6 +832,54 @@ def test_losses_train_a_module_and_muon_steps_its_matrix():
     loss_fn({k: v for k, v in data.items() if k != "log_prob"})
 
 
+def test_a_captured_training_step():
+  """Loss, backward and the orthogonalised update of a policy captured as one graph: every replay, with the inputs
+  changed in place and eager work in between, gives what the eager step gives."""
+  import derl_amd as derl
+  from derl_amd import ops
+  hidden, vocab, rows = 64, 3001, 24
+  model = torch.nn.Linear(hidden, vocab, bias=False).to(DEV)
+  obs = torch.randn(rows, hidden, generator=gen(1), device=DEV)
+  actions = torch.randint(0, vocab, (rows,), generator=gen(2), device=DEV)
+  mask = torch.rand(rows, generator=gen(3), device=DEV) < 0.8
+  old = torch.full((rows,), -8.0, device=DEV)
+  adv = torch.randn(rows, generator=gen(4), device=DEV)
+  offsets = torch.tensor([0, 5, 11, 20, 24], dtype=torch.int32, device=DEV)
+  policy, preference = derl.TokenPolicyLoss(model, kl_coef=0.1, entropy_coef=0.01), derl.PreferenceLoss(model, beta=0.2)
+  data = dict(observations=obs, actions=actions, log_prob=old, advantages=adv, ref_log_prob=old, mask=mask)
+  pairs = dict(observations=obs, actions=actions, offsets=offsets, mask=mask)
+
+  def step():
+    model.weight.grad = None
+    loss = policy(data) + 0.5 * preference(pairs)
+    loss.backward()
+    return loss.detach(), model.weight.grad, ops.orthogonalize(model.weight.grad)
+
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    for _ in range(2):
+      step()
+  torch.cuda.current_stream().wait_stream(side)
+  model.weight.grad = None
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    captured = step()
+  kept = model.weight.grad
+  for k in range(4):
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in captured]
+    want = [t.clone() for t in step()]
+    for a, b in zip(got, want):
+      assert torch.equal(a, b), k
+    obs.mul_(-0.9)
+    adv.add_(0.1)
+    actions.copy_((actions * 7 + 1) % vocab)
+    torch.cuda.synchronize()
+  assert kept is captured[1]
+
+
 def muon_reference(params, grads, state, spans, matrices, step, lr, max_norm, mu=0.95, betas=(0.9, 0.999), eps=1e-8, decay=0.0):
   """One step of the flat optimizer in 64 bits; returns the new parameters."""
   norm = float(np.sqrt((grads ** 2).sum()))
