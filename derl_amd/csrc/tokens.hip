@@ -778,18 +778,42 @@ struct PairArgs {
   double *partials;
 };
 
-__device__ double block_sum_256(double v, double *scratch) {
+// the sum over a workgroup of T threads, in every thread
+template <int T>
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double scratch[T / 64];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
-  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  v = 0;
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) v += scratch[i];
+  return v;
+}
+
+// this thread's share of a sum over rows begin .. end, eight of its rows on their way at a time (a row a round trip made one pair
+// of two sequences of 131072 rows take 340 us)
+template <int T, class F>
+__device__ __forceinline__ double sum_rows(long long begin, long long end, F value) {
+  constexpr int U = 8;
+  double s = 0;
+  long long i = begin + threadIdx.x;
+  for (; i + (U - 1) * T < end; i += U * T) {
+    float v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = value(i + k * T);
+#pragma unroll
+    for (int k = 0; k < U; ++k) s += v[k];
+  }
+  for (; i < end; i += T) s += value(i);
+  return s;
 }
 
 // a workgroup per pair: the two sequences' log-probabilities, the pair's loss, and the coefficient of each of its rows
-__global__ __launch_bounds__(256) void preference_pairs_kernel(const PairArgs a) {
-  __shared__ double scratch[4];
+template <int T>
+__global__ __launch_bounds__(T) void preference_pairs_kernel(const PairArgs a) {
   double sum[7] = {0, 0, 0, 0, 0, 0, 0};
   for (int pair = blockIdx.x; pair < a.pairs; pair += gridDim.x) {
     double lp[2];
@@ -798,9 +822,7 @@ __global__ __launch_bounds__(256) void preference_pairs_kernel(const PairArgs a)
       const long long b = a.offsets[2LL * pair + side], e = a.offsets[2LL * pair + side + 1];
       begin[side] = b < 0 ? 0 : b;
       end[side] = e > a.rows ? a.rows : e;
-      double s = 0;
-      for (long long i = begin[side] + threadIdx.x; i < end[side]; i += 256) s += a.stats[i].z;
-      lp[side] = block_sum_256(s, scratch);
+      lp[side] = block_sum<T>(sum_rows<T>(begin[side], end[side], [&](long long i) { return a.stats[i].z; }));
     }
     const double chosen = a.beta * (lp[0] - (a.ref_lp ? a.ref_lp[2LL * pair] : 0.f));
     const double rejected = a.beta * (lp[1] - (a.ref_lp ? a.ref_lp[2LL * pair + 1] : 0.f));
@@ -810,8 +832,11 @@ __global__ __launch_bounds__(256) void preference_pairs_kernel(const PairArgs a)
     const double slope = (a.smoothing / (1.0 + exp(-h)) - (1.0 - a.smoothing) / (1.0 + exp(h))) * a.beta / (a.batch > 0 ? a.batch : a.pairs);
     for (int side = 0; side < 2; ++side) {
       const float c = static_cast<float>(side ? -slope : slope);
-      for (long long i = begin[side] + threadIdx.x; i < end[side]; i += 256)
-        if (!a.mask || a.mask[i]) a.stats[i].w = c;
+#pragma unroll 4
+      for (long long i = begin[side] + threadIdx.x; i < end[side]; i += T) {
+        const bool keep = !a.mask || a.mask[i];
+        a.stats[i].w = keep ? c : 0.f;
+      }
     }
     if (threadIdx.x == 0) {
       a.seq_lp[2LL * pair] = static_cast<float>(lp[0]);
@@ -858,13 +883,11 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, l
 }
 
 // log-probabilities of sequences: a workgroup per sequence
-__global__ __launch_bounds__(256) void sequence_sum_kernel(const float *lp, const int32_t *offsets, long long rows, int sequences, float *out) {
-  __shared__ double scratch[4];
+template <int T>
+__global__ __launch_bounds__(T) void sequence_sum_kernel(const float *lp, const int32_t *offsets, long long rows, int sequences, float *out) {
   for (int q = blockIdx.x; q < sequences; q += gridDim.x) {
     const long long b = offsets[q] < 0 ? 0 : offsets[q], e = offsets[q + 1] > rows ? rows : offsets[q + 1];
-    double s = 0;
-    for (long long i = b + threadIdx.x; i < e; i += 256) s += lp[i];
-    s = block_sum_256(s, scratch);
+    const double s = block_sum<T>(sum_rows<T>(b, e, [&](long long i) { return lp[i]; }));
     if (threadIdx.x == 0) out[q] = static_cast<float>(s);
   }
 }
@@ -878,6 +901,10 @@ __global__ __launch_bounds__(256) void scale_rows_kernel(char *x, long long pitc
     write_columns<D, 256, false>(x + row * pitch, nullptr, x + row * pitch, V, 0, V, threadIdx.x, true,
                                  [&](float v, float, int) { return v * f; });
 }
+
+// sequences that are worth 1024 threads each instead of 256 (a masked preference loss of 18 columns, us with 256 / 1024 threads: one
+// pair of 8192 rows each 32.8 / 27.7, of 131072 466 / 270; four of 2048 21.4 / 22.2, 1024 of 8 23.3 / 45.7)
+inline bool long_sequences(long long rows, long long sequences) { return rows / sequences >= 8192; }
 
 inline int elem_size(int dtype) { return dtype == DX_F32 ? 4 : 2; }
 
@@ -1040,8 +1067,10 @@ extern "C" int dx_sequence_log_prob(const float *token_log_prob, const int32_t *
   DX_REQUIRE(rows >= 0 && sequences >= 0, "dx_sequence_log_prob: negative shape");
   if (sequences == 0) return DX_OK;
   DX_REQUIRE((token_log_prob || rows == 0) && offsets && out, "dx_sequence_log_prob: null pointer");
-  hipLaunchKernelGGL(sequence_sum_kernel, dim3(sequences < kMaxWorkers ? sequences : kMaxWorkers), dim3(256), 0, dx::as_stream(stream),
-                     token_log_prob, offsets, rows, sequences, out);
+  const dim3 grid(sequences < kMaxWorkers ? sequences : kMaxWorkers);
+  hipStream_t s = dx::as_stream(stream);
+  if (long_sequences(rows, sequences)) hipLaunchKernelGGL(sequence_sum_kernel<1024>, grid, dim3(1024), 0, s, token_log_prob, offsets, rows, sequences, out);
+  else hipLaunchKernelGGL(sequence_sum_kernel<256>, grid, dim3(256), 0, s, token_log_prob, offsets, rows, sequences, out);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
@@ -1117,7 +1146,8 @@ extern "C" int dx_preference_loss(const void *logits, int dtype, long long rows,
   PairArgs p{a.stats, offsets, ref_log_prob, mask, rows, pairs, global_pairs > 0 ? static_cast<double>(global_pairs) : 0.0, beta,
              label_smoothing, sequence_log_prob, a.partials};
   const int pair_groups = pairs < kMaxWorkers ? pairs : kMaxWorkers;
-  hipLaunchKernelGGL(preference_pairs_kernel, dim3(pair_groups), dim3(256), 0, s, p);
+  if (long_sequences(rows, 2LL * pairs)) hipLaunchKernelGGL(preference_pairs_kernel<1024>, dim3(pair_groups), dim3(1024), 0, s, p);
+  else hipLaunchKernelGGL(preference_pairs_kernel<256>, dim3(pair_groups), dim3(256), 0, s, p);
   DX_LAUNCH_CHECK();
   // gradient: a wave per short row, else a workgroup per piece of 32 KB of a row
   const int T = static_cast<long long>(vocab) * elem_size(dtype) <= 4096 ? 64 : 256;

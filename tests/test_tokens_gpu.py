@@ -331,6 +331,21 @@ def test_many_pairs_and_extreme_margins():
   check_preference(got, want, vocab, 8, F32, 0.5)
 
 
+@pytest.mark.parametrize("borders", [[0, 20000, 40000], [3, 17001, 17001, 17050, 39000], [0, 40000, 40000]])
+def test_long_sequences(borders):
+  """Sequences of tens of thousands of rows, which more threads add up."""
+  from derl_amd import ops
+  rows, vocab, beta = 40000, 9, 2.0 ** -8
+  z, actions = logits_of(rows, vocab, F32, 12, banned=False)
+  mask = mask_of(rows, "some", 2)
+  offsets = torch.tensor(borders, dtype=torch.int32, device=DEV)
+  got = ops.preference_loss(z, actions, offsets, None, beta, mask=mask)
+  check_preference(got, preference_oracle(z, actions, offsets, None, beta, 0.0, mask), vocab, rows, F32, beta)
+  assert torch.equal(ops.sequence_log_prob(z, actions, offsets, mask), got[2])
+  got = ops.preference_loss(z, actions, offsets, None, beta)
+  check_preference(got, preference_oracle(z, actions, offsets, None, beta, 0.0, None), vocab, rows, F32, beta)
+
+
 def test_gradients_against_differences():
   """<dL/dz, v> = (L(z + h v) - L(z - h v)) / 2 h up to h^2 |L'''| / 6 (third derivatives of these losses along a
   direction of length 1 are below 8 here) and the fp32 rounding of L, 2^-22 (1 + |L|) / h."""
