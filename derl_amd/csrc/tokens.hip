@@ -640,6 +640,140 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const Row
   }
 }
 
+// ---- rows of up to 1 KB: 16 lanes a row -----------------------------------------------------------------------------
+// A row of a small vocabulary costs a wave as many instructions as a long one's first vector, most of them the row's own scalars
+// and sums over lanes: four rows share them here.  262144 x 18 f32: log-probabilities 74 us, policy loss 138 us a call with a wave a
+// row, 18 and 42 so; of 250 columns 73 and 160, 44 and 115; 256 rows alike.  The next row is on its way during this one; the action's
+// logit is picked from the registers.
+template <int ROR>
+__device__ __forceinline__ float rotated16(float v) {  // within the 16 lanes of a row
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + ROR, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += rotated16<8>(v);
+  v += rotated16<4>(v);
+  v += rotated16<2>(v);
+  return v + rotated16<1>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, rotated16<8>(v));
+  v = fmaxf(v, rotated16<4>(v));
+  v = fmaxf(v, rotated16<2>(v));
+  return fmaxf(v, rotated16<1>(v));
+}
+
+template <class D, int NV, Mode MODE, bool REF, bool ENT>
+__global__ __launch_bounds__(256) void token_short_kernel(const RowArgs a) {
+  constexpr int E = D::E;
+  __shared__ double sums[16][8];
+  const int t = threadIdx.x & 15, slot = threadIdx.x >> 4;
+  const float w = MODE == POLICY ? row_weight<4>(a) : 0.f;
+  const long long step = gridDim.x * 16LL;
+  struct Row {
+    bool keep;
+    long long action;
+    float old, adv, ref;
+    u32x4 v[NV], u[REF ? NV : 1];
+  };
+  auto load = [&](long long row) {  // (a row past the last: the last one again)
+    if (row >= a.rows) row = a.rows - 1;
+    Row r{};
+    r.keep = !a.mask || a.mask[row];
+    if (!r.keep) return r;
+    r.action = a.actions[row];
+    if constexpr (MODE == POLICY) {
+      r.old = a.old_lp[row];
+      r.adv = a.adv[row];
+      if (a.ref_lp) r.ref = a.ref_lp[row];
+    }
+    const char *z = a.z + row * a.z_pitch, *q = REF ? a.q + row * a.q_pitch : nullptr;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (k * 16 * E >= a.V) continue;
+      const bool ragged = (k + 1) * 16 * E > a.V;
+      r.v[k] = load_raw<D>(z, z + k * 256, t, (k * 16 + t) * E, a.V, ragged);
+      if constexpr (REF) r.u[k] = load_raw<D>(q, q + k * 256, t, (k * 16 + t) * E, a.V, ragged);
+    }
+    return r;
+  };
+  double sum[6] = {0, 0, 0, 0, 0, 0};
+  long long row = blockIdx.x * 16LL + slot;
+  Row now = load(row);
+  for (; row < a.rows; row += step) {
+    const Row next = load(row + step);
+    RowStats r = kNothing;
+    float x[NV][E], y[REF ? NV : 1][E], za = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (k * 16 * E >= a.V) continue;
+      const int first = (k * 16 + t) * E;
+      const bool ragged = (k + 1) * 16 * E > a.V;
+      unpack_raw<D>(now.v[k], x[k], first, a.V, ragged);
+      if constexpr (REF) unpack_raw<D>(now.u[k], y[k], first, a.V, ragged);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        r.m = fmaxf(r.m, x[k][i]);
+        if constexpr (REF) r.mr = fmaxf(r.mr, y[k][i]);
+        za += first + i == now.action ? x[k][i] : 0.f;
+      }
+    }
+    r.m = max16(r.m);
+    if constexpr (REF) r.mr = max16(r.mr);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (k * 16 * E < a.V) add_terms<D, REF>(r, x[k], y[REF ? k : 0]);
+    r.s = sum16(r.s);
+    r.ed = sum16(r.ed);
+    if constexpr (REF) {
+      r.sr = sum16(r.sr);
+      r.gap = sum16(r.gap);
+    }
+    za = sum16(za);  // (one lane's)
+    if (now.action < 0 || now.action >= a.V) za = __builtin_nanf("");
+    RowTerms out = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if constexpr (MODE == POLICY) {
+      RowPlan g = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (now.keep) g = policy_row<REF>(a, r, za, now.old, now.adv, now.ref, w, &out);
+      char *dz = a.dz + row * a.dz_pitch;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if (k * 16 * E >= a.V) continue;
+        const int first = (k * 16 + t) * E;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          x[k][i] = now.keep ? grad_of<D, REF, ENT>(g, x[k][i], REF ? y[k][i] : 0.f) + (first + i == now.action ? g.at : 0.f) : 0.f;
+        if (first < a.V) store_chunk<D>(dz, dz + k * 256, t, first, a.V, (k + 1) * 16 * E > a.V, x[k]);
+      }
+      if (t == 0) {
+        const float all[6] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp};
+#pragma unroll
+        for (int k = 0; k < 6; ++k) sum[k] += all[k];
+      }
+    } else {
+      const float log_s = logf(r.s);
+      out.lp = now.keep ? (za - r.m) - log_s : 0.f;
+      out.entropy = now.keep ? log_s - r.ed / r.s : 0.f;
+    }
+    if (t == 0) {
+      if (MODE != STATS) a.lp[row] = out.lp;
+      if (MODE == LOGP && a.entropy) a.entropy[row] = out.entropy;
+      if (MODE == STATS) a.stats[row] = now.keep ? make_float4(r.m, 1.f / r.s, out.lp, 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    now = next;
+  }
+  if constexpr (MODE == POLICY) {
+    if (t == 0)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums[slot][k] = k < 6 ? sum[k] : 0.0;
+    __syncthreads();
+    if (threadIdx.x < 8) {
+      double s = 0;
+      for (int i = 0; i < 16; ++i) s += sums[i][threadIdx.x];
+      a.partials[blockIdx.x * 8LL + threadIdx.x] = s;
+    }
+  }
+}
+
 // ---- few rows: every row cut into pieces, a workgroup each ----------------------------------------------------------
 template <class D, Mode MODE, bool REF>
 __global__ __launch_bounds__(256) void token_pieces_kernel(const RowArgs a) {
@@ -912,7 +1046,7 @@ inline int elem_size(int dtype) { return dtype == DX_F32 ? 4 : 2; }
 struct RowShape { int T, NV; };
 RowShape row_shape(int V, int dtype, bool ref, bool once, bool few) {
   const long long vectors = (static_cast<long long>(V) * elem_size(dtype) + 15) / 16;
-  if (vectors <= 64) return {64, 1};
+  if (vectors <= 64) return {16, vectors <= 16 ? 1 : 4};
   if (vectors <= 64 * 8) return {64, vectors <= 64 * 4 ? 4 : 8};
   // read once anyway: many rows to a CU, or, where there are no more rows than CUs, many threads to a row (32 x 32768 f32 log-
   // probabilities: 6.0 us with 1024 threads, 7.6 with 256; 32 x 12000 bf16 4.7, 5.0; shorter ones alike)
@@ -932,7 +1066,12 @@ int launch_rows(const RowArgs &a, RowShape sh, int grid, hipStream_t s) {
     DX_LAUNCH_CHECK();                                                                                                        \
     return DX_OK;                                                                                                             \
   }
-  DX_ROWS(64, 1)
+  if (sh.T == 16) {
+    if (sh.NV == 1) hipLaunchKernelGGL((token_short_kernel<D, 1, MODE, REF, ENT>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((token_short_kernel<D, 4, MODE, REF, ENT>), dim3(grid), dim3(256), 0, s, a);
+    DX_LAUNCH_CHECK();
+    return DX_OK;
+  }
   DX_ROWS(64, 4)
   DX_ROWS(64, 8)
   if constexpr (MODE != POLICY) {
@@ -953,7 +1092,8 @@ template <class D>
 int launch_pref_grad(const RowArgs &a, int T, long long blocks, int pairs, int pair_groups, float *loss_out, hipStream_t s) {
   // one workgroup at least, which writes the terms; fewer than 2^32 threads, the most of a launch
   const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : blocks < (1 << 23) ? blocks : 1 << 23));
-  if (T == 64) hipLaunchKernelGGL((preference_grad_kernel<D, 64>), grid, dim3(256), 0, s, a, blocks, pairs, pair_groups, loss_out);
+  if (T == 16) hipLaunchKernelGGL((preference_grad_kernel<D, 16>), grid, dim3(256), 0, s, a, blocks, pairs, pair_groups, loss_out);
+  else if (T == 64) hipLaunchKernelGGL((preference_grad_kernel<D, 64>), grid, dim3(256), 0, s, a, blocks, pairs, pair_groups, loss_out);
   else hipLaunchKernelGGL((preference_grad_kernel<D, 256>), grid, dim3(256), 0, s, a, blocks, pairs, pair_groups, loss_out);
   DX_LAUNCH_CHECK();
   return DX_OK;
@@ -987,7 +1127,7 @@ int run_rows(RowArgs a, int dtype, int *groups, hipStream_t s) {
     }
   }
   const RowShape sh = row_shape(a.V, dtype, REF, MODE != POLICY, a.rows <= cus);
-  const long long need = sh.T == 64 ? (a.rows + 3) / 4 : a.rows;
+  const long long need = sh.T < 256 ? (a.rows + 256 / sh.T - 1) / (256 / sh.T) : a.rows;
   // POLICY: resident workgroups, which prefetch their next row (1024 threads fill a CU).  Read once: as many as there are 64 KB
   // pieces, as masked rows would leave resident ones with unequal shares (8192 rows of 64 KB, a fifth masked: 96 us, 81 so).
   long long most = sh.T == 1024 ? cus : sh.T == 512 ? 2LL * cus : 8LL * cus < kMaxWorkers ? 8LL * cus : kMaxWorkers;
@@ -1149,11 +1289,13 @@ extern "C" int dx_preference_loss(const void *logits, int dtype, long long rows,
   if (long_sequences(rows, 2LL * pairs)) hipLaunchKernelGGL(preference_pairs_kernel<1024>, dim3(pair_groups), dim3(1024), 0, s, p);
   else hipLaunchKernelGGL(preference_pairs_kernel<256>, dim3(pair_groups), dim3(256), 0, s, p);
   DX_LAUNCH_CHECK();
-  // gradient: a wave per short row, else a workgroup per piece of 32 KB of a row
-  const int T = static_cast<long long>(vocab) * elem_size(dtype) <= 4096 ? 64 : 256;
-  a.piece = T == 64 ? vocab : 32768 / elem_size(dtype);
+  // gradient: 16 lanes or a wave per short row, else a workgroup per piece of 32 KB of a row (the whole loss of 262144 rows, us with
+  // 64 / 16 lanes: 18 columns f32 204 / 160, 128 213 / 186, 250 255 / 301)
+  const long long bytes = static_cast<long long>(vocab) * elem_size(dtype);
+  const int T = bytes <= 512 ? 16 : bytes <= 4096 ? 64 : 256;
+  a.piece = T < 256 ? vocab : 32768 / elem_size(dtype);
   a.splits = (vocab - 1) / a.piece + 1;
-  const long long blocks = (T == 64 ? (rows + 3) / 4 : rows) * a.splits;
+  const long long blocks = (rows + 256 / T - 1) / (256 / T) * a.splits;
   if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, blocks, pairs, pair_groups, loss_out, s);
   if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
   return launch_pref_grad<ElemF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
