@@ -1048,6 +1048,9 @@ RowShape row_shape(int V, int dtype, bool ref, bool once, bool few) {
   const long long vectors = (static_cast<long long>(V) * elem_size(dtype) + 15) / 16;
   if (vectors <= 64) return {16, vectors <= 16 ? 1 : 4};
   if (vectors <= 64 * 8) return {64, vectors <= 64 * 4 ? 4 : 8};
+  // to 16 KB a wave a row too, but for read-once rows of many columns (16384 rows bf16, us with 64 / 256 threads a row: policy loss of
+  // 4099 columns 78 / 87, 8192 122 / 125; log-probabilities of 4099 35 / 47, 5000 43 / 46, 6500 53 / 51, 8192 68 / 52)
+  if (!ref && vectors <= 64 * 16 && (!once || V <= 5120)) return {64, 16};
   // read once anyway: many rows to a CU, or, where there are no more rows than CUs, many threads to a row (32 x 32768 f32 log-
   // probabilities: 6.0 us with 1024 threads, 7.6 with 256; 32 x 12000 bf16 4.7, 5.0; shorter ones alike)
   if (once) return {few && vectors > 1024 ? 1024 : 256, 0};
@@ -1074,11 +1077,12 @@ int launch_rows(const RowArgs &a, RowShape sh, int grid, hipStream_t s) {
   }
   DX_ROWS(64, 4)
   DX_ROWS(64, 8)
+  if constexpr (!REF) DX_ROWS(64, 16)
   if constexpr (MODE != POLICY) {
     DX_ROWS(256, 0)
     DX_ROWS(1024, 0)
   } else {
-    DX_ROWS(256, 4)
+    if constexpr (REF) DX_ROWS(256, 4)
     DX_ROWS(256, 8)
     if constexpr (!REF) DX_ROWS(256, 16)
     DX_ROWS(512, REF ? 8 : 16)

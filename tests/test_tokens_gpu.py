@@ -570,6 +570,39 @@ def test_the_same_index_twice_and_every_action(dtype):
       within(got[1], dz[1], 8 * s * (dz[2] + 0.1 / vocab) + half_step(dz[1], dtype), "dlogits")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab", [16, 17, 60, 129, 255, 300, 513, 1030, 2051, 2100, 4090, 4099, 5121, 8190])
+def test_rows_of_every_length_in_lanes_and_waves(vocab, dtype):
+  """More rows than one turn of the grid takes at the lengths where the threads of a row change, masked and not, from odd
+  starts; rows beside each other share cache lines."""
+  from derl_amd import ops
+  rows = 40003 if vocab < 300 else 9001
+  z, actions = logits_of(rows, vocab, dtype, vocab)
+  old = -math.log(vocab) - 1 + 0.1 * torch.randn(rows, generator=gen(6), device=DEV)
+  adv = torch.randn(rows, generator=gen(7), device=DEV)
+  mask = mask_of(rows, "some", 8)
+  _, _, h64, lp64 = rows64(z, actions)
+  lp, entropy = ops.token_log_prob(z, actions, mask)
+  s = slack(vocab)
+  within(lp, torch.where(mask, lp64, 0.0), s + 2.0 ** -23 * (lp64.abs() + 16), "log_prob")
+  within(entropy, torch.where(mask, h64, 0.0), 2 * s * (1 + math.log(vocab + 1)) + 2.0 ** -22 * (h64 + 1), "entropy")
+  got = ops.token_policy_loss(z, actions, old, adv, None, kl_coef=0.1, entropy_coef=0.01, ref_log_prob=old, mask=mask)
+  check_policy(got, policy_oracle(z, actions, old, adv, None, 0.1, 0.01, old, None, mask), vocab, dtype)
+  wide = torch.zeros((rows, vocab + 1), dtype=dtype, device=DEV)
+  view = wide[:, 1:]
+  view.copy_(z)
+  again = ops.token_policy_loss(view, actions, old, adv, None, kl_coef=0.1, entropy_coef=0.01, ref_log_prob=old, mask=mask, dlogits_out=view)
+  for a, b in zip(again, got):
+    assert torch.equal(a, b)
+  assert not wide[:, 0].any()
+  view.copy_(z)
+  offsets = torch.tensor([0, rows // 3, rows // 2, rows - 9, rows], dtype=torch.int32, device=DEV)
+  want = ops.preference_loss(z, actions, offsets, None, 2.0 ** -10, mask=mask)
+  for a, b in zip(ops.preference_loss(view, actions, offsets, None, 2.0 ** -10, mask=mask, dlogits_out=view), want):
+    assert torch.equal(a, b)
+  check_preference(want, preference_oracle(z, actions, offsets, None, 2.0 ** -10, 0.0, mask), vocab, rows, dtype, 2.0 ** -10)
+
+
 def test_the_longest_rows():
   """Two rows of 2^30 - 3 columns, nearly 4 GB each.  A thread adds at most 2^15 columns to its sum (128 pieces of 256
   threads a row): 2^15 roundings of 2^-24 each, and the joins' 60."""
