@@ -3,12 +3,10 @@
 // with X the (r, c) matrix whose shorter side is r (a tall G is worked on transposed).  Odd polynomials of the singular
 // values only: the singular vectors stay G's, the singular values approach 1.
 //
-// The products run on the fp16 matrix cores with fp32 accumulation.  fp32 and fp16 matrices are held as TWO fp16 terms, hi + lo
-// (22 bits): a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), fp32 accuracy at a third of the fp16 rate,
-// where the fp32 matrix instructions have a sixteenth.  For bf16 X is one term, 11 bits, three more than the result keeps
-// (each step multiplies what is lost by up to `a` = 3.4); A and B keep two terms up to r = kOneTermRows, as the fewer entries
-// they have the less their roundings average out.  Against 64 bits, with the result's own rounding as 1: everything one
-// term 2.5 at r = 37, 1.54 at 520, 1.37 at 640, 1.35 at 769, 1.2 at 4096; A and B two terms 1.1; all of it two terms 1.0.
+// The products run on the fp16 matrix cores with fp32 accumulation.  Whatever the matrix's type, X, A and B are held as TWO fp16
+// terms, hi + lo (22 bits): a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), fp32 accuracy at a third of the
+// fp16 rate, where the fp32 matrix instructions have a sixteenth.  (bf16 too: with one term, 11 bits, each step multiplies what
+// is lost by up to `a` = 3.4, and a bf16 result was off by 1.1 to 2.5 times its own rounding; with two it is off by that alone.)
 // Stored values are scaled by powers of two (X by 2^12, A and B by 2^8), so that neither large entries overflow nor the second
 // term of typical ones (1 / sqrt(c)) falls under fp16's smallest step.
 //
@@ -31,18 +29,16 @@ using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 constexpr float kScaleX = 4096.f, kScaleA = 256.f;
-constexpr int kOneTermRows = 640;  // bf16: with more rows A and B are held as one fp16 term too
 constexpr int kPad = 64, kNormParts = 512;
 constexpr int kSplitGroups = 512;  // workgroups of a product that is split over K, at most
 
+constexpr int kStageK = 32;        // k of a stage of a product
+
 enum Epilogue { GRAM, POLY, UPDATE, FINAL };
 
-// A matrix of one term: rows of `ld` values.  Of two: rows of 2 ld, each 32 values' first terms followed by their second ones, so
-// that a cache line holds both terms of 32 k.
-template <int T>
-__device__ __forceinline__ long long place(long long row, int col, int ld) {
-  return T == 2 ? row * 2 * ld + (col >> 5) * 64 + (col & 31) : row * ld + col;
-}
+// A matrix: rows of 2 ld halves, each 32 values' first terms followed by their second ones, so that a cache line holds both
+// terms of 32 k.
+__device__ __forceinline__ long long place(long long row, int col, int ld) { return row * 2 * ld + (col >> 5) * 64 + (col & 31); }
 constexpr int kSecond = 32;  // from a value's first term to its second
 
 struct NsArgs {
@@ -127,24 +123,22 @@ __device__ __forceinline__ void put_final(const NsArgs &a, int z, int m, int n, 
       if (quad + k < a.cols) to[k] = static_cast<uint16_t>((k < 2 ? t.x : t.y) >> (k & 1) * 16);
 }
 
-// WR x WC waves, each FM x FN tiles of 32 x 32 x 16 instructions; K stages of 64, a ring of RING in LDS filled by LDS-DMA.
+// WR x WC waves, each FM x FN tiles of 32 x 32 x 16 instructions; K stages of 32, a ring of RING in LDS filled by LDS-DMA.
 // A row of a stage is 128 bytes -- one cache line: a CU has about 64 requests to the L2 in flight, and with rows of 64 bytes
-// (stages of 32) half of what they can carry bounded the copies (4096^3, one term: 143 us, 120 with whole lines).  Slot s of row R
+// half of what they can carry bounded the copies (4096^3, of one term: 143 us, 120 with whole lines).  Slot s of row R
 // holds the row's 16-byte chunk s ^ ((R >> 1) & 7), so that the 16 lanes of a ds_read_b128 group meet every bank once; the
 // swizzle is applied to the source address, the DMA writes LDS linearly.
 // One barrier per stage, in front of its last 16 k, whose fragments are in registers by then: behind it the stage's slot is
 // free and is filled again, and the next stage has landed everywhere, so that its first fragments are read in the shadow of
 // the last products: the matrix pipe does not wait at the barrier.  Rows past the matrix repeat its last row and are not stored.
-template <int TM, int WR, int WC, int PT, int QT, int OT, int RING, Epilogue EPI>
+template <int TM, int WR, int WC, int RING, Epilogue EPI>
 __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
   constexpr int kWaves = WR * WC, FM = TM / WR / 32, FN = TM / WC / 32;
-  // a stage: 64 k, or 32 where both operands have two terms; 128-byte lines of it per row of P and Q
-  constexpr int kStageK = PT + QT == 4 ? 32 : 64, kParts = kStageK / 16, PL = PT * kStageK / 64, QL = QT * kStageK / 64;
-  constexpr int kArray = TM * 128;               // bytes of a line of every row
-  constexpr int kStage = (PL + QL) * kArray;
+  constexpr int kArray = TM * 128;               // bytes of a stage's lines of every row of P, or of Q
+  constexpr int kStage = 2 * kArray;
   constexpr int NP = TM / 8 / kWaves;            // 1 KiB pieces (8 rows) of an array that a wave copies
-  constexpr int kPieces = (PL + QL) * NP;
+  constexpr int kPieces = 2 * NP;
   static_assert(NP * 8 * kWaves == TM && FM * 32 * WR == TM && FN * 32 * WC == TM, "tile");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -173,23 +167,21 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   for (int p = 0; p < NP; ++p) {
     const int R = (wave * NP + p) * 8 + (lane >> 3);
     const int chunk = (lane & 7) ^ ((R >> 1) & 7);
-    off[0][p] = static_cast<uint32_t>(min(R, a.rows_p - 1 - bm * TM)) * a.ldp * (2 * PT) + chunk * 16;
-    off[1][p] = static_cast<uint32_t>(min(R, a.rows_q - 1 - bn * TM)) * a.ldq * (2 * QT) + chunk * 16;
+    off[0][p] = static_cast<uint32_t>(min(R, a.rows_p - 1 - bm * TM)) * a.ldp * 4 + chunk * 16;
+    off[1][p] = static_cast<uint32_t>(min(R, a.rows_q - 1 - bn * TM)) * a.ldq * 4 + chunk * 16;
   }
   const int first = split * a.split_stages, stages = min(a.split_stages, a.K / kStageK - first);
-  const char *from[PL + QL];
-#pragma unroll
-  for (int s = 0; s < PL + QL; ++s)
-    from[s] = s < PL ? reinterpret_cast<const char *>(a.P + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp * PT) + first * (PL * 128LL) + s * 128
-                     : reinterpret_cast<const char *>(a.Q + z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq * QT) + first * (QL * 128LL) + (s - PL) * 128;
+  const char *from[2] = {
+      reinterpret_cast<const char *>(a.P + z * a.p_stride + static_cast<long long>(bm) * TM * a.ldp * 2) + first * 128LL,
+      reinterpret_cast<const char *>(a.Q + z * a.q_stride + static_cast<long long>(bn) * TM * a.ldq * 2) + first * 128LL};
   // piece k of the next stage to copy, into `slot`; an array's last one moves on
   auto copy = [&](int k, int slot) {
     const int s = k / NP, p = k % NP;
-    dma_piece(from[s], off[s < PL ? 0 : 1][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
-    if (p == NP - 1) from[s] += (s < PL ? PL : QL) * 128;
+    dma_piece(from[s], off[s][p], smem + (slot * kStage + s * kArray + (wave * NP + p) * 1024) / 4);
+    if (p == NP - 1) from[s] += 128;
   };
   // a wave of one tile keeps a sum for each product and 16 k of a stage: dependent instructions issue at half the rate
-  constexpr int kPairs = PT + QT - 1;  // products of terms: hi hi | lo hi, hi hi | lo hi, hi lo, hi hi
+  constexpr int kPairs = 3;  // products of terms: lo hi, hi lo, hi hi
   constexpr int kSums = FM * FN == 1 ? 2 * kPairs : 1;
   f32x16 acc[FM][FN], more[kSums];
 #pragma unroll
@@ -203,31 +195,31 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   }
   const int wm = wave / WC, wn = wave % WC, hi = lane >> 5, l31 = lane & 31;
   const unsigned x = (l31 >> 1) & 7;
-  // lane addresses in a line's array: of one term, 16 k of four; of two, 16 k of two and the term
+  // lane addresses in an array: 16 k of two, times two terms
   unsigned prow[4], qrow[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int pc = PT == 2 ? (k & 1) * 4 + (k >> 1) * 2 + hi : 2 * k + hi, qc = QT == 2 ? (k & 1) * 4 + (k >> 1) * 2 + hi : 2 * k + hi;
-    prow[k] = (wm * FM * 32 + l31) * 128 + (pc ^ x) * 16;
-    qrow[k] = PL * kArray + (wn * FN * 32 + l31) * 128 + (qc ^ x) * 16;
+    const int chunk = (k & 1) * 4 + (k >> 1) * 2 + hi;
+    prow[k] = (wm * FM * 32 + l31) * 128 + (chunk ^ x) * 16;
+    qrow[k] = kArray + (wn * FN * 32 + l31) * 128 + (chunk ^ x) * 16;
   }
-  f16x8 p[2][PT][FM], q[2][QT][FN];
-  // fragment k (of kReads) of 16 k of a slot
-  constexpr int kReads = PT * FM + QT * FN, kProducts = kPairs * FM * FN;
+  f16x8 p[2][2][FM], q[2][2][FN];
+  // fragment k (of kReads) of 16 k (`part`) of a slot
+  constexpr int kReads = 2 * (FM + FN), kProducts = kPairs * FM * FN;
   auto fetch = [&](int set, int slot, int part, int k) {
     const char *base = reinterpret_cast<const char *>(smem) + slot * kStage;
-    if (k < PT * FM) {
+    if (k < 2 * FM) {
       const int t = k / FM, i = k % FM;
-      p[set][t][i] = *reinterpret_cast<const f16x8 *>(base + (PT == 2 ? prow[(part & 1) * 2 + t] + part / 2 * kArray : prow[part]) + i * 4096);
+      p[set][t][i] = *reinterpret_cast<const f16x8 *>(base + prow[part * 2 + t] + i * 4096);
     } else {
-      const int t = (k - PT * FM) / FN, j = (k - PT * FM) % FN;
-      q[set][t][j] = *reinterpret_cast<const f16x8 *>(base + (QT == 2 ? qrow[(part & 1) * 2 + t] + part / 2 * kArray : qrow[part]) + j * 4096);
+      const int t = (k - 2 * FM) / FN, j = (k - 2 * FM) % FN;
+      q[set][t][j] = *reinterpret_cast<const f16x8 *>(base + qrow[part * 2 + t] + j * 4096);
     }
   };
   auto multiply = [&](int set, int k) {  // the small products first
     const int t = k / (FM * FN), i = k / FN % FM, j = k % FN;
     f32x16 &sum = kSums > 1 && t * 2 + set > 0 ? more[kSums > 1 ? t * 2 + set : 0] : acc[i][j];
-    sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[set][PT == 2 && t == 0][i], q[set][QT == 2 && t == kPairs - 2][j], sum, 0, 0, 0);
+    sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[set][t == 0][i], q[set][t == 1][j], sum, 0, 0, 0);
   };
   // 16 k of a stage: the products of one set of fragments, with the reads of the other and copies of a later stage between
   // them (one or two waves a SIMD: what is not issued in a product's shadow is paid for)
@@ -258,10 +250,6 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   for (int s = 0; s < stages; ++s) {
     const int next = slot + 1 == RING ? 0 : slot + 1;
     part(0, slot, 1, 0, false, std::false_type{});
-    if constexpr (kParts == 4) {
-      part(1, slot, 2, 0, false, std::false_type{});
-      part(0, slot, 3, 0, false, std::false_type{});
-    }
     // this wave's copies of stage s + 1 have landed and all its reads of stage s are done; behind the barrier every wave's
     if (s + RING <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * kPieces) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -330,7 +318,6 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   // Accumulator e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.  Stores: rows are made of four columns
   // per lane by a transposition within quads (8 bytes a lane, 64 a row), the transposed copy of eight rows per lane by
   // exchanging with the lane of the other half (16 bytes).
-  constexpr bool two = OT == 2;
   _Float16 *D = a.D + z * a.d_stride, *DT = a.DT + z * a.dt_stride;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -350,10 +337,8 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
         } else if constexpr (EPI == POLY) {
-          const _Float16 *at = a.P + z * a.p_stride + place<PT>(n, m, a.ldp);  // A[n][m] = A[m][n]
-          const f16x4 ah = *reinterpret_cast<const f16x4 *>(at);
-          f16x4 al = {0, 0, 0, 0};
-          if (PT == 2) al = *reinterpret_cast<const f16x4 *>(at + kSecond);
+          const _Float16 *at = a.P + z * a.p_stride + place(n, m, a.ldp);  // A[n][m] = A[m][n]
+          const f16x4 ah = *reinterpret_cast<const f16x4 *>(at), al = *reinterpret_cast<const f16x4 *>(at + kSecond);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             v[k] = a.c * (v[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(ah[k]) + static_cast<float>(al[k])) +
@@ -379,26 +364,23 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
         l[g][0] = bl.x;
         l[g][1] = bl.y;
         if (EPI == UPDATE || bm != bn) {
-          _Float16 *at = D + place<OT>(m + (lane & 3), n0 + (l31 & ~3), a.ldd);
-          const Pair2 th = quad_transpose(bh.x, bh.y, lane);
+          _Float16 *at = D + place(m + (lane & 3), n0 + (l31 & ~3), a.ldd);
+          const Pair2 th = quad_transpose(bh.x, bh.y, lane), tl = quad_transpose(bl.x, bl.y, lane);
           *reinterpret_cast<u32x2 *>(at) = u32x2{th.x, th.y};
-          if (two) {
-            const Pair2 tl = quad_transpose(bl.x, bl.y, lane);
-            *reinterpret_cast<u32x2 *>(at + kSecond) = u32x2{tl.x, tl.y};
-          }
+          *reinterpret_cast<u32x2 *>(at + kSecond) = u32x2{tl.x, tl.y};
         }
       }
       if constexpr (EPI != FINAL) {
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {  // groups g (kept by the lower half) and g + 1 (by the upper one): eight rows each
-          _Float16 *at = DT + place<OT>(n, m0 + 8 * (g + hi), a.lddt);
+          _Float16 *at = DT + place(n, m0 + 8 * (g + hi), a.lddt);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             swap_halves(h[g][k], h[g + 1][k]);
-            if (two) swap_halves(l[g][k], l[g + 1][k]);
+            swap_halves(l[g][k], l[g + 1][k]);
           }
           *reinterpret_cast<u32x4 *>(at) = u32x4{h[g][0], h[g][1], h[g + 1][0], h[g + 1][1]};
-          if (two) *reinterpret_cast<u32x4 *>(at + kSecond) = u32x4{l[g][0], l[g][1], l[g + 1][0], l[g + 1][1]};
+          *reinterpret_cast<u32x4 *>(at + kSecond) = u32x4{l[g][0], l[g][1], l[g + 1][0], l[g + 1][1]};
         }
       }
     }
@@ -455,7 +437,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long cou
 
 // X0 and its transpose from a 64 x 64 tile of G: `same` has G's orientation (ld_same), `turned` the other.  Also clears the
 // arrival counts of the split products.
-template <typename V, bool TWO>
+template <typename V>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n, const double *partials, int parts, float eps, _Float16 *same,
                                                       int ld_same, _Float16 *turned, int ld_turned, long long stride, unsigned *arrivals, int counts) {
   constexpr int E = 16 / sizeof(V);
@@ -515,13 +497,13 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n,
       l[i] = static_cast<_Float16>(v - static_cast<float>(h[i]));
     }
     *reinterpret_cast<f16x8 *>(at) = h;
-    if (TWO) *reinterpret_cast<f16x8 *>(at + kSecond) = l;
+    *reinterpret_cast<f16x8 *>(at + kSecond) = l;
   };
 #pragma unroll
   for (int k = 0; k < 2; ++k) {  // 64 rows of 8 x 8 values; the sides are multiples of 64: a row of 8 is whole or outside
     const int at = k * 256 + threadIdx.x, row = at >> 3, col = (at & 7) * 8;
-    if (r0 + row < mp && c0 + col < np) put8(same + z * stride + place<TWO ? 2 : 1>(r0 + row, c0 + col, ld_same), [&](int i) { return tile[row][col + i]; });
-    if (c0 + row < np && r0 + col < mp) put8(turned + z * stride + place<TWO ? 2 : 1>(c0 + row, r0 + col, ld_turned), [&](int i) { return tile[col + i][row]; });
+    if (r0 + row < mp && c0 + col < np) put8(same + z * stride + place(r0 + row, c0 + col, ld_same), [&](int i) { return tile[row][col + i]; });
+    if (c0 + row < np && r0 + col < mp) put8(turned + z * stride + place(c0 + row, r0 + col, ld_turned), [&](int i) { return tile[col + i][row]; });
   }
 }
 
@@ -534,9 +516,9 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n,
 constexpr int kSmallWaves = 16;
 constexpr long long kSmallLds = 160 * 1024 - 256;
 
-inline long long small_lds(int rp, int cp, int tx) {
+inline long long small_lds(int rp, int cp) {
   if (rp > 64 && rp / 32 * (cp / 32) > kSmallWaves) return kSmallLds + 1;  // more blocks of 32 x 32 than waves: see launch_small
-  return 2LL * tx * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8)) + 8LL * rp * (rp + 8);
+  return 4LL * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8)) + 8LL * rp * (rp + 8);
 }
 
 struct SmallArgs {
@@ -562,18 +544,14 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
   const int ldx = a.cp + 8, ldr = a.rp + 8;  // X: rp rows of ldx; X^T: cp rows of ldr; A, B: rp rows of ldr
   // each array: its first terms, then its second ones
   const int sx = a.rp * ldx, st = a.cp * ldr, sa = a.rp * ldr;
-  constexpr int TX = std::is_same<V, __bf16>::value ? 1 : 2;  // terms of X; A and B have two
-  using Two = std::integral_constant<int, 2>;
-  using OfX = std::integral_constant<int, TX>;
-  const int X = 0, XT = X + TX * sx, A = XT + TX * st, B = A + 2 * sa;
+  const int X = 0, XT = X + 2 * sx, A = XT + 2 * st, B = A + 2 * sa;
   auto put1 = [&](int at, int size, float v) {
     const _Float16 h = static_cast<_Float16>(v);
     lds[at] = h;
-    if (TX == 2) lds[at + size] = static_cast<_Float16>(v - static_cast<float>(h));
+    lds[at + size] = static_cast<_Float16>(v - static_cast<float>(h));
   };
   // four consecutive rows of a column: into the row of the transpose (`turned`) and, if wanted, into four rows (`at`, ld apart)
-  auto put4 = [&](auto terms, int turned, int turned_size, int at, int ld, int size, bool both, f32x4 v) {
-    constexpr bool two = decltype(terms)::value == 2;
+  auto put4 = [&](int turned, int turned_size, int at, int ld, int size, bool both, f32x4 v) {
     f16x4 h, l;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -581,12 +559,12 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
       l[k] = static_cast<_Float16>(v[k] - static_cast<float>(h[k]));
     }
     *reinterpret_cast<f16x4 *>(lds + turned) = h;
-    if (two) *reinterpret_cast<f16x4 *>(lds + turned + turned_size) = l;
+    *reinterpret_cast<f16x4 *>(lds + turned + turned_size) = l;
     if (both) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         lds[at + k * ld] = h[k];
-        if (two) lds[at + k * ld + size] = l[k];
+        lds[at + k * ld + size] = l[k];
       }
     }
   };
@@ -623,9 +601,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
   // 16 x 16 tile: row 4 (lane / 16) + e, column lane % 16
   constexpr int F = SIDE / 16, kHeld = COLUMN > 0 ? COLUMN : 1;
   struct Block { f32x4 v[F][F]; };
-  auto products = [&](auto pt, auto qt, auto &acc, int count, int P, int ldp, int sp, int Q, int ldq, int sq, int K) {
+  auto products = [&](auto &acc, int count, int P, int ldp, int sp, int Q, int ldq, int sq, int K) {
     constexpr int N = sizeof(acc) / sizeof(Block);
-    constexpr bool p2 = decltype(pt)::value == 2, q2 = decltype(qt)::value == 2;
     Block cross[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -639,7 +616,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         qh[f] = *reinterpret_cast<const f16x8 *>(lds + qo + f * 16 * ldq + k);
-        if (q2) ql[f] = *reinterpret_cast<const f16x8 *>(lds + qo + f * 16 * ldq + sq + k);
+        ql[f] = *reinterpret_cast<const f16x8 *>(lds + qo + f * 16 * ldq + sq + k);
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -647,15 +624,13 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
 #pragma unroll
         for (int f = 0; f < F; ++f) {
           const int at = po + (i * SIDE + f * 16) * ldp + k;
-          const f16x8 ph = *reinterpret_cast<const f16x8 *>(lds + at);
-          f16x8 pl;
-          if (p2) pl = *reinterpret_cast<const f16x8 *>(lds + at + sp);
+          const f16x8 ph = *reinterpret_cast<const f16x8 *>(lds + at), pl = *reinterpret_cast<const f16x8 *>(lds + at + sp);
 #pragma unroll
           for (int g = 0; g < F; ++g) {
             acc[i].v[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh[g], acc[i].v[f][g], 0, 0, 0);
             f32x4 &c = cross[i].v[f][g];  // (a sum of its own: dependent instructions issue at half the rate)
-            if (p2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh[g], c, 0, 0, 0);
-            if (q2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql[g], c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh[g], c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql[g], c, 0, 0, 0);
           }
         }
       }
@@ -680,8 +655,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
         while (left >= tr - row) left -= tr - row++;
         const int pm = row * SIDE, qn = (row + left) * SIDE;
         Block acc[1];
-        if (half) products(Two{}, Two{}, acc, 1, A + pm * ldr, ldr, sa, A + qn * ldr, ldr, sa, a.rp);
-        else products(OfX{}, OfX{}, acc, 1, X + pm * ldx, ldx, sx, X + qn * ldx, ldx, sx, a.cp);
+        if (half) products(acc, 1, A + pm * ldr, ldr, sa, A + qn * ldr, ldr, sa, a.rp);
+        else products(acc, 1, X + pm * ldx, ldx, sx, X + qn * ldx, ldx, sx, a.cp);
 #pragma unroll
         for (int f = 0; f < F; ++f)
 #pragma unroll
@@ -694,7 +669,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
 #pragma unroll
               for (int k = 0; k < 4; ++k) v[k] += a.b * (static_cast<float>(h[k]) + static_cast<float>(l[k])) + (m + k == n ? a.a * kScaleA : 0.f);
             }
-            put4(Two{}, to + n * ldr + m, sa, to + m * ldr + n, ldr, sa, pm != qn, v);
+            put4(to + n * ldr + m, sa, to + m * ldr + n, ldr, sa, pm != qn, v);
           }
       }
       __syncthreads();
@@ -708,7 +683,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
           const int m = tm * SIDE + f * 16 + 4 * quad, n = tn * SIDE + g * 16 + l15;
           const f32x4 v = b.v[f][g] * (1.f / kScaleA);
           if (!last) {
-            put4(OfX{}, XT + n * ldr + m, st, X + m * ldx + n, ldx, sx, true, v);
+            put4(XT + n * ldr + m, st, X + m * ldx + n, ldx, sx, true, v);
           } else {
             V *out = static_cast<V *>(a.out) + blockIdx.x * static_cast<long long>(count);
 #pragma unroll
@@ -719,13 +694,13 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
     };
     Block held[kHeld];
     if constexpr (COLUMN == 0) {
-      if (wave < tr * tc) products(Two{}, OfX{}, held, 1, B + wave % tr * SIDE * ldr, ldr, sa, XT + wave / tr * SIDE * ldr, ldr, st, a.rp);
+      if (wave < tr * tc) products(held, 1, B + wave % tr * SIDE * ldr, ldr, sa, XT + wave / tr * SIDE * ldr, ldr, st, a.rp);
       __syncthreads();
       if (wave < tr * tc) put_block(wave % tr, wave / tr, held[0]);
     } else {
 #pragma unroll 1
       for (int tn = wave; tn < tc; tn += kSmallWaves) {
-        products(Two{}, OfX{}, held, tr, B, ldr, sa, XT + tn * SIDE * ldr, ldr, st, a.rp);
+        products(held, tr, B, ldr, sa, XT + tn * SIDE * ldr, ldr, st, a.rp);
 #pragma unroll
         for (int i = 0; i < COLUMN; ++i)
           if (i < tr) put_block(i, tn, held[i]);
@@ -752,8 +727,8 @@ int launch_small(const SmallArgs &q, int batch, int bytes, hipStream_t s) {
 }
 
 struct Plan {
-  int r, c, rp, cp, tx, ta, parts;  // tx, ta: terms of X, of A and B
-  long long x, sq;             // halves of X and of A per matrix, padded
+  int r, c, rp, cp, parts;
+  long long x, sq;             // halves of X and of A per matrix, both terms, padded
   long long split_floats, bytes;
 };
 Plan make_plan(int dtype, int batch, int m, int n) {
@@ -762,13 +737,10 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   p.c = m < n ? n : m;
   p.rp = (p.r + kPad - 1) / kPad * kPad;
   p.cp = (p.c + kPad - 1) / kPad * kPad;
-  p.tx = dtype == DX_BF16 ? 1 : 2;
-  p.ta = dtype == DX_BF16 && p.r > kOneTermRows ? 1 : 2;
-  p.x = static_cast<long long>(p.rp) * p.cp * p.tx;
-  p.sq = static_cast<long long>(p.rp) * p.rp * p.ta;
-
+  p.x = 2LL * p.rp * p.cp;
+  p.sq = 2LL * p.rp * p.rp;
   // X, two copies of X^T, A, B, and the norm's partial sums
-  const long long blocks = (static_cast<long long>(m) * n + 8191) / 8192;  // 8192 elements a workgroup at least
+  const long long blocks = (static_cast<long long>(m) * n * (dtype == DX_F32 ? 4 : 2) + 32767) / 32768;  // 32 KB a workgroup at least
   p.parts = static_cast<int>(blocks < kNormParts ? blocks : kNormParts);
   p.split_floats = static_cast<long long>(kSplitGroups) * (p.r > 1024 ? 128 * 128 : 64 * 64);  // (128 x 128 tiles are split where there are many)
   p.bytes = batch * (2 * (3 * p.x + 2 * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4 * p.split_floats;
@@ -781,16 +753,16 @@ int check_shape(int dtype, int batch, int m, int n) {
   return DX_OK;
 }
 
-template <int TM, int WR, int WC, int PT, int QT, int OT, int RING, Epilogue EPI>
+template <int TM, int WR, int WC, int RING, Epilogue EPI>
 int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
-  constexpr int kStageK = PT + QT == 4 ? 32 : 64, bytes = RING * (PT + QT) * kStageK / 64 * TM * 128;
-  DX_LDS_OPT_IN((ns_gemm_kernel<TM, WR, WC, PT, QT, OT, RING, EPI>), bytes);
+  constexpr int bytes = RING * 2 * TM * 128;
+  DX_LDS_OPT_IN((ns_gemm_kernel<TM, WR, WC, RING, EPI>), bytes);
   a.tiles_m = cdiv(a.rows_p, TM);
   a.tiles_n = cdiv(a.rows_q, TM);
   const int tiles = EPI == GRAM || EPI == POLY ? a.tiles_m * (a.tiles_m + 1) / 2 : a.tiles_m * a.tiles_n;
   a.split_stages = cdiv(a.K / kStageK, splits);
   a.splits = cdiv(a.K / kStageK, a.split_stages);
-  hipLaunchKernelGGL((ns_gemm_kernel<TM, WR, WC, PT, QT, OT, RING, EPI>), dim3(tiles * a.splits, batch), dim3(WR * WC * 64), bytes, s, a);
+  hipLaunchKernelGGL((ns_gemm_kernel<TM, WR, WC, RING, EPI>), dim3(tiles * a.splits, batch), dim3(WR * WC * 64), bytes, s, a);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
@@ -801,10 +773,10 @@ int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
 // Measured, us a product: 2001 x 5003 f32 X X^T at 128 one part 126, three parts 94; 64, 192, 256: 127, 170, 258; its
 // update 178, 147, 177, 139 at 64, 128, 192, 256.  512 x 3136 f32 X X^T at 64: one part 23, seven 14; its update 14.6, 22, 35, 52.
 struct Choice { int tile, splits; };
-Choice choose(long long batch, int rows_p, int rows_q, bool half, bool mixed, bool may_split, int stages, int cus, long long split_floats) {
+Choice choose(long long batch, int rows_p, int rows_q, bool half, bool may_split, int stages, int cus, long long split_floats) {
   Choice best{64, 1};
   double best_time = 1e300;
-  for (int tile = 64; tile <= (mixed ? 128 : 256); tile += 64) {
+  for (int tile = 64; tile <= 256; tile += 64) {
     const long long m = cdiv(rows_p, tile), n = cdiv(rows_q, tile), tiles = (half ? m * (m + 1) / 2 : m * n) * batch;
     const double alone = tile == 64 ? 0.30 : tile == 128 ? 0.78 : tile == 192 ? 1.2 : 1.9, two = tile == 64 ? 0.52 : 1.10;
     for (int splits = 1; splits <= (may_split && tile <= 128 ? 8 : 1); ++splits) {
@@ -821,21 +793,17 @@ Choice choose(long long batch, int rows_p, int rows_q, bool half, bool mixed, bo
   }
   return best;
 }
-template <int PT, int QT, int OT, Epilogue EPI>
+template <Epilogue EPI>
 int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
-  constexpr bool half = EPI == GRAM || EPI == POLY, mixed = PT + QT + OT == 4;
+  constexpr bool half = EPI == GRAM || EPI == POLY;
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
-  const Choice c = choose(batch, a.rows_p, a.rows_q, half, mixed, half, a.K / (PT + QT == 4 ? 32 : 64), cus, a.split_floats);
-  if constexpr (!mixed) {
-    if (c.tile == 256) return launch_tile<256, 2, 4, PT, QT, OT, 2, EPI>(a, batch, 1, s);
-    if (c.tile == 192) return launch_tile<192, 2, 2, PT, QT, OT, 3, EPI>(a, batch, 1, s);
-  }
-  if (c.tile == 128) return launch_tile<128, 2, 2, PT, QT, OT, 2, EPI>(a, batch, c.splits, s);
-  return launch_tile<64, 2, 2, PT, QT, OT, mixed ? 3 : 4, EPI>(a, batch, c.splits, s);
+  const Choice c = choose(batch, a.rows_p, a.rows_q, half, half, a.K / kStageK, cus, a.split_floats);
+  if (c.tile == 256) return launch_tile<256, 2, 4, 2, EPI>(a, batch, 1, s);
+  if (c.tile == 192) return launch_tile<192, 2, 2, 3, EPI>(a, batch, 1, s);
+  if (c.tile == 128) return launch_tile<128, 2, 2, 2, EPI>(a, batch, c.splits, s);
+  return launch_tile<64, 2, 2, 4, EPI>(a, batch, c.splits, s);
 }
-// TX: terms of X, TA: of A and B
-template <int TX, int TA>
 int run_steps(const Plan &p, int batch, int steps, NsArgs a, _Float16 *X, _Float16 *XT0, _Float16 *XT1, _Float16 *A, _Float16 *B, hipStream_t s) {
   for (int k = 0; k < steps; ++k) {
     _Float16 *xt = k & 1 ? XT1 : XT0, *next = k & 1 ? XT0 : XT1;
@@ -847,12 +815,12 @@ int run_steps(const Plan &p, int batch, int steps, NsArgs a, _Float16 *X, _Float
     g.D = g.DT = A;
     g.d_stride = g.dt_stride = p.sq;
     g.ldd = g.lddt = p.rp;
-    if (int rc = launch_gemm<TX, TX, TA, GRAM>(g, batch, s)) return rc;
+    if (int rc = launch_gemm<GRAM>(g, batch, s)) return rc;
     g.P = g.Q = A;
     g.p_stride = g.q_stride = p.sq;
     g.ldp = g.ldq = g.K = p.rp;
     g.D = g.DT = B;
-    if (int rc = launch_gemm<TA, TA, TA, POLY>(g, batch, s)) return rc;
+    if (int rc = launch_gemm<POLY>(g, batch, s)) return rc;
     g.P = B;
     g.Q = xt;
     g.q_stride = p.x;
@@ -861,7 +829,7 @@ int run_steps(const Plan &p, int batch, int steps, NsArgs a, _Float16 *X, _Float
     g.DT = next;
     g.d_stride = g.dt_stride = p.x;
     g.ldd = p.cp;
-    if (int rc = k + 1 < steps ? launch_gemm<TA, TX, TX, UPDATE>(g, batch, s) : launch_gemm<TA, TX, TX, FINAL>(g, batch, s)) return rc;
+    if (int rc = k + 1 < steps ? launch_gemm<UPDATE>(g, batch, s) : launch_gemm<FINAL>(g, batch, s)) return rc;
   }
   return DX_OK;
 }
@@ -888,10 +856,10 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   const Plan p = make_plan(dtype, batch, m, n);
   if (workspace_bytes < p.bytes) return fail(DX_EWS, "dx_orthogonalize: workspace of %lld bytes, %lld needed", workspace_bytes, p.bytes);
   hipStream_t s = as_stream(stream);
-  if (small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32, p.tx) <= kSmallLds) {
+  if (small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32) <= kSmallLds) {
     const int r32 = cdiv(p.r, 32) * 32, c32 = cdiv(p.c, 32) * 32;
     const SmallArgs q{update, out, m, n, p.r, p.c, r32, c32, steps, m > n, a, b, c, eps};
-    const int bytes = static_cast<int>(small_lds(r32, c32, p.tx));
+    const int bytes = static_cast<int>(small_lds(r32, c32));
     if (dtype == DX_F32) return launch_small<float>(q, batch, bytes, s);
     if (dtype == DX_BF16) return launch_small<__bf16>(q, batch, bytes, s);
     return launch_small<_Float16>(q, batch, bytes, s);
@@ -916,13 +884,13 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   _Float16 *same = tall ? XT0 : X, *turned = tall ? X : XT0;
   const int ld_same = tall ? p.rp : p.cp, ld_turned = tall ? p.cp : p.rp;
   if (dtype == DX_F32)
-    hipLaunchKernelGGL((ns_pack_kernel<float, true>), grid, dim3(256), 0, s, static_cast<const float *>(update), m, n, partials, p.parts, eps,
+    hipLaunchKernelGGL((ns_pack_kernel<float>), grid, dim3(256), 0, s, static_cast<const float *>(update), m, n, partials, p.parts, eps,
                        same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   else if (dtype == DX_BF16)
-    hipLaunchKernelGGL((ns_pack_kernel<__bf16, false>), grid, dim3(256), 0, s, static_cast<const __bf16 *>(update), m, n, partials, p.parts, eps,
+    hipLaunchKernelGGL((ns_pack_kernel<__bf16>), grid, dim3(256), 0, s, static_cast<const __bf16 *>(update), m, n, partials, p.parts, eps,
                        same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   else
-    hipLaunchKernelGGL((ns_pack_kernel<_Float16, true>), grid, dim3(256), 0, s, static_cast<const _Float16 *>(update), m, n, partials, p.parts,
+    hipLaunchKernelGGL((ns_pack_kernel<_Float16>), grid, dim3(256), 0, s, static_cast<const _Float16 *>(update), m, n, partials, p.parts,
                        eps, same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
   DX_LAUNCH_CHECK();
   NsArgs g{};
@@ -937,6 +905,5 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   g.r = p.r;
   g.cols = p.c;
   g.tall = tall;
-  if (p.tx == 2) return run_steps<2, 2>(p, batch, steps, g, X, XT0, XT1, A, B, s);
-  return p.ta == 2 ? run_steps<1, 2>(p, batch, steps, g, X, XT0, XT1, A, B, s) : run_steps<1, 1>(p, batch, steps, g, X, XT0, XT1, A, B, s);
+  return run_steps(p, batch, steps, g, X, XT0, XT1, A, B, s);
 }
