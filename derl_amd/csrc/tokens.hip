@@ -351,8 +351,8 @@ __device__ __forceinline__ float grad_of(const RowPlan &g, float x, float y) {
   const float d = x - g.m, p = exp_of(d) * g.inv_s;
   float v = g.c0;
   if constexpr (ENT) v += g.c1 * fmaxf(d, kLowest);
-  if constexpr (REF) return p == 0.f ? 0.f : p * (g.c2 != 0.f ? v + g.c2 * (x - y) : v);  // (x - y may be infinite)
-  return p * v;
+  if constexpr (REF) v = g.c2 != 0.f ? v + g.c2 * (x - y) : v;
+  return p == 0.f ? 0.f : p * v;  // (of a banned column x - y is infinite, and c1 d where |c1| > 1)
 }
 
 struct RowTerms { float policy, entropy, kl, outside, ratio, lp; };

@@ -1,0 +1,44 @@
+"""Gradients and terms of the token losses where their arithmetic can fail: banned columns, coefficients past the row
+count.  Oracles and tolerances are those of tests/test_tokens_gpu.py."""
+import pytest
+import torch
+
+from tests.test_tokens_gpu import BF16, DEV, F16, F32, INF, check_policy, policy_inputs, policy_oracle
+
+pytestmark = pytest.mark.gpu
+
+# (rows, columns) for 16 lanes a row, a wave, 256 .. 1024 threads with the row in registers, rows read twice, rows in pieces
+KERNELS = [(3, 18), (5, 250), (4, 1000), (3, 4000), (130, 8191), (130, 20011), (130, 40003), (130, 65541), (130, 131100), (2, 20011)]
+
+
+@pytest.mark.parametrize("coefficient,batch", [(1.5, 0), (-2.0, 0), (3.0, 1), (-40.0, 16)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,vocab", KERNELS)
+def test_an_entropy_coefficient_past_the_row_count(rows, vocab, dtype, coefficient, batch):
+  """One unmasked row, or a given batch below the coefficient: banned columns (-inf, or the type's lowest value) have a
+  gradient of 0, the others theirs."""
+  from derl_amd import ops
+  z, actions, old, adv, _, _ = policy_inputs(rows, vocab, dtype, 3 * vocab)
+  z[:, 6::8] = torch.finfo(dtype).min
+  actions = torch.where(actions % 8 == 6, actions - 1, actions)
+  mask = torch.zeros(rows, dtype=torch.bool, device=DEV)
+  mask[rows // 2] = True
+  logp = torch.log_softmax(z.double(), 1).gather(1, actions[:, None])[:, 0]
+  old = (logp + 0.05).float()
+  got = ops.token_policy_loss(z, actions, old, adv, 0.2, entropy_coef=coefficient, mask=mask, global_batch=batch)
+  assert not got[1][:, 3::8].any() and not got[1][:, 6::8].any()
+  terms, dz, _, lp = policy_oracle(z, actions, old, adv, 0.2, 0.0, coefficient, None, None, mask, batch)
+  size = policy_oracle(z, actions, old, adv, 0.2, 0.0, abs(coefficient), None, None, mask, batch)[2]
+  loss = got[0].clone()
+  loss[0] = 0  # (a difference of terms that the coefficient scales: looked at below)
+  check_policy((loss, got[1], got[2]), ([0.0] + terms[1:], dz, size, lp), vocab, dtype)
+  assert abs(float(got[0][0]) - terms[0]) <= 2.0 ** -16 * (1 + abs(coefficient)) * (1 + abs(terms[2]))
+
+
+def test_an_infinite_ratio_leaves_banned_columns_alone():
+  from derl_amd import ops
+  for vocab in (40, 3000, 9000):
+    z, actions, old, _, _, _ = policy_inputs(4, vocab, F32, 1)
+    _, dz, _ = ops.token_policy_loss(z, actions, old - 200.0, torch.full((4,), -1.0, device=DEV), None)
+    assert not dz[:, 3::8].any() and not torch.isfinite(dz.gather(1, actions[:, None])).any()
+    assert INF in dz.abs()
