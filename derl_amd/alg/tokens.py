@@ -9,13 +9,28 @@ from .common import Loss
 from .. import ops, summary
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+  """What is handed on where a graph of the gradient is asked for (``create_graph``): the kernels' gradient is a constant to
+  autograd, so whoever differentiates it again, with respect to anything that the logits depend on, is told."""
+
+  @staticmethod
+  def forward(ctx, dlogits, logits):
+    return dlogits.view_as(dlogits)
+
+  @staticmethod
+  def backward(ctx, grad_output):
+    raise RuntimeError("the gradient of a token loss cannot be differentiated: it has no second derivative here")
+
+
 class _LogitsLoss(torch.autograd.Function):
   """A scalar computed from logits together with its gradient.  The gradient is handed on once: it is scaled in
-  place by the incoming gradient (left alone where that is 1)."""
+  place by the incoming gradient (left alone where that is 1).  A second derivative (a gradient's penalty, a product
+  with the Hessian) raises."""
 
   @staticmethod
   def forward(ctx, logits, evaluate):
     terms, dlogits = evaluate(logits.detach())
+    ctx.save_for_backward(logits)
     ctx.dlogits = dlogits
     return terms[0].clone()
 
@@ -24,7 +39,10 @@ class _LogitsLoss(torch.autograd.Function):
     dlogits, ctx.dlogits = ctx.dlogits, None
     if dlogits is None:
       raise RuntimeError("the gradient of this loss was already handed on: evaluate the loss again to differentiate it again")
-    ops.scale_rows(dlogits, grad_output.to(torch.float32).contiguous())
+    with torch.no_grad():
+      ops.scale_rows(dlogits, grad_output.to(torch.float32).contiguous())
+    if torch.is_grad_enabled():
+      dlogits = _NoSecondDerivative.apply(dlogits, *ctx.saved_tensors)
     return dlogits, None
 
 

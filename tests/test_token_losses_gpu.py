@@ -42,3 +42,31 @@ def test_an_infinite_ratio_leaves_banned_columns_alone():
     _, dz, _ = ops.token_policy_loss(z, actions, old - 200.0, torch.full((4,), -1.0, device=DEV), None)
     assert not dz[:, 3::8].any() and not torch.isfinite(dz.gather(1, actions[:, None])).any()
     assert INF in dz.abs()
+
+
+def losses_of(model, rows, vocab, hidden, seed=0):
+  """Both classes on ``model`` with a batch for each: [(loss, data)]."""
+  import derl_amd as derl
+  g = torch.Generator(device=DEV).manual_seed(seed)
+  obs = torch.randn(rows, hidden, generator=g, device=DEV).to(next(model.parameters()).dtype)
+  actions = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+  old = -torch.rand(rows, generator=g, device=DEV) - float(torch.tensor(vocab).log())
+  adv = torch.randn(rows, generator=g, device=DEV)
+  offsets = torch.tensor([0, rows // 4, rows // 2, rows - 1, rows], dtype=torch.int32, device=DEV)
+  mask = torch.rand(rows, generator=g, device=DEV) < 0.8
+  mask[0] = True
+  return [(derl.TokenPolicyLoss(model, cliprange=0.5, kl_coef=0.1, entropy_coef=0.01),
+           dict(observations=obs, actions=actions, log_prob=old, advantages=adv, ref_log_prob=old - 0.1, mask=mask)),
+          (derl.PreferenceLoss(model, beta=0.2), dict(observations=obs, actions=actions, offsets=offsets, mask=mask))]
+
+
+def test_second_derivatives_are_refused():
+  """Not where a graph of the gradient is only asked for: where it is differentiated, also in part."""
+  model = torch.nn.Sequential(torch.nn.Linear(8, 16), torch.nn.Tanh(), torch.nn.Linear(16, 50)).to(DEV)
+  for loss_fn, data in losses_of(model, 12, 50, 8):
+    once = torch.autograd.grad(loss_fn(data), model.parameters())
+    grads = torch.autograd.grad(loss_fn(data), model.parameters(), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, grads))
+    for part in (grads, grads[:1], grads[-1:]):
+      with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(sum(x.square().sum() for x in part), model.parameters(), retain_graph=True, allow_unused=True)
