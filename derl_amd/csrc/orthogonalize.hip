@@ -1,17 +1,22 @@
 // Newton-Schulz orthogonalisation of an update (gfx950):
-//   X0 = G / (|G|_F + eps),   A = X X^T,   B = a I + b A + c A^2,   X <- B X        (`steps` times)
+//   X0 = G / (|G|_F + eps),   A = X X^T,   X <- a X + (b A + c A^2) X        (`steps` times)
 // with X the (r, c) matrix whose shorter side is r (a tall G is worked on transposed).  Odd polynomials of the singular
 // values only: the singular vectors stay G's, the singular values approach 1.
 //
-// The products run on the fp16 matrix cores with fp32 accumulation.  Whatever the matrix's type, X, A and B are held as TWO fp16
+// The products run on the fp16 matrix cores with fp32 accumulation.  Whatever the matrix's type, X, A and M below are held as TWO fp16
 // terms, hi + lo (22 bits): a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), fp32 accuracy at a third of the
 // fp16 rate, where the fp32 matrix instructions have a sixteenth.  (bf16 too: with one term, 11 bits, each step multiplies what
 // is lost by up to `a` = 3.4, and a bf16 result was off by 1.1 to 2.5 times its own rounding; with two it is off by that alone.)
-// Stored values are scaled by powers of two (X by 2^12, A and B by 2^8), so that neither large entries overflow nor the second
-// term of typical ones (1 / sqrt(c)) falls under fp16's smallest step.
+// fp16 has few exponents, so what is stored in it is scaled, by powers of two, such that EVERY row of an operand lies in its upper
+// range: rows of X by the exponent E_i of a bound of their norms, of X^T by F_n, of A and M = b A + c A^2 (whose rows are bounded by
+// |x_i|) by E_i as well.  A row of a product is then as accurate as its own size allows, however small it is against the others
+// (256 x 512 Gaussian, 32 rows x 1e-6: those rows are off by 2e-7 after 5 steps; with one scale for the whole matrix 1.5e-3).  The
+// bounds are exact: a step maps a row x_i = sum_k U_ik s_k v_k to sum_k U_ik q(s_k^2) s_k v_k, so its norm grows by max |q| at most,
+// q(t) = a + b t + c t^2, over the singular values there can be (`grown`).  The update is X' = a X + M X with X, and b A of M, from
+// fp32 copies, so that what the polynomial leaves alone (small singular values: q = a) passes a step with one rounding.
 //
 // Every matrix product is C = P Q^T with both operands' k contiguous: X for A = X X^T, A = A^T for A^2 = A A^T, and for
-// B X the transposed copy X^T, which the epilogue of each update writes beside X.  A and B are symmetric: only tiles on
+// M X the transposed copy X^T, which the epilogue of each update writes beside X.  A and M are symmetric: only tiles on
 // and above the diagonal are formed and stored twice.  Both sides are padded
 // to a multiple of 64 with zeros in the workspace.
 #include <cmath>
@@ -23,18 +28,71 @@ namespace dx {
 namespace {
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
+using i32x4 = __attribute__((ext_vector_type(4))) int;
 using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
-constexpr float kScaleX = 4096.f, kScaleA = 256.f;
-constexpr int kPad = 64, kNormParts = 512;
+constexpr int kTop = 14;         // rows of an operand are scaled to norms below 2^kTop
+constexpr int kLowest = -160;    // exponent of a bound of 0
+constexpr int kPad = 64, kScanParts = 64;
 constexpr int kSplitGroups = 512;  // workgroups of a product that is split over K, at most
 
 constexpr int kStageK = 32;        // k of a stage of a product
 
 enum Epilogue { GRAM, POLY, UPDATE, FINAL };
+
+// the least power of two above x >= 0 (NaN, infinities: 2^128)
+__host__ __device__ inline int power_above(float x) {
+  if (!(x < 3.4e38f)) return 128;
+  if (x == 0.f) return kLowest;
+  const int e = static_cast<int>(__builtin_bit_cast(uint32_t, x) >> 23);
+  return e - 126;
+}
+// What is known of X before a step: its singular values are at most `top` < 2^cap, a row or column at most 2^shift times what it
+// was at the start; |b + c t| < 2^poly for their squares t.  2^E for a row that began below 2^e: E = min(e + shift, cap).
+// A polynomial that grows beyond 1 makes the largest value there can be explode, where the matrix's own may be far below: it is
+// taken to stay within 8, or within what `a` alone makes of it (`linear`), whichever is more.
+struct Powers { short shift, cap, poly; };
+struct Known : Powers {
+  float top, linear;
+};
+inline float larger(float x, float y) { return x > y || x != x ? x : y; }
+inline float size_of(float x) { return x < 0.f ? -x : x; }
+inline Known known_of(float top, float linear, int shift, float b, float c) {
+  const float t = top * top;
+  Known k;
+  k.top = top;
+  k.linear = linear;
+  k.shift = static_cast<short>(shift < -1000 ? -1000 : shift > 1000 ? 1000 : shift);
+  k.cap = static_cast<short>(power_above(top));
+  k.poly = static_cast<short>(power_above(larger(size_of(b), size_of(b + c * t))));
+  return k;
+}
+inline Known known_at_start(float b, float c) { return known_of(1.01f, 1.01f, 0, b, c); }  // (|X0|_F <= 1, rounded)
+inline Known grown(const Known &k, float a, float b, float c) {
+  const float t = k.top * k.top;
+  auto q = [&](float x) { return size_of(a + (b + c * x) * x); };
+  float growth = larger(q(0.f), q(t)), top = k.top * q(t);
+  const float vertex = -b / (2.f * c);
+  if (vertex > 0.f && vertex < t) growth = larger(growth, q(vertex));
+  // s q(s^2) is extreme where a + 3 b t + 5 c t^2 = 0
+  const float inner = 9.f * b * b - 20.f * a * c, root = inner > 0.f ? sqrtf(inner) : 0.f, w = -0.5f * (3.f * b + (b < 0.f ? -root : root));
+  for (int i = 0; i < 2; ++i) {
+    const float at = i ? a / w : w / (5.f * c);
+    if (at > 0.f && at < t) top = larger(top, sqrtf(at) * q(at));
+  }
+  // the values are rounded: nothing shrinks below the rounding of what it is the difference of
+  const float terms = (size_of(a) + (size_of(b) + size_of(c) * t) * t) * 3.8e-6f;
+  growth = 1.01f * larger(growth, terms);
+  top = 1.01f * larger(top, terms * k.top);
+  const float linear = 1.01f * k.linear * size_of(a), limit = linear > 8.f ? linear : 8.f;
+  top = top < limit ? top : limit;
+  return known_of(top, linear, k.shift + power_above(growth), b, c);
+}
+__device__ __forceinline__ int bound_of(int start, int shift, int cap) { return min(start + shift, cap); }
+__device__ __forceinline__ float times_power(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
 // A matrix: rows of 2 ld halves, each 32 values' first terms followed by their second ones, so that a cache line holds both
 // terms of 32 k.
@@ -50,6 +108,14 @@ struct NsArgs {
   _Float16 *D, *DT;       // [m][n] and its transpose [n][m]
   long long d_stride, dt_stride;
   int ldd, lddt;
+  // exponents of the bounds that rows m and columns n began with; what is known now and, for UPDATE, behind the step
+  const int *exp_m, *exp_n;
+  int exp_m_stride, exp_n_stride;
+  int shift, cap, poly, next_shift, next_cap;
+  // fp32 values (A: written by GRAM, read by POLY; X), in blocks of 32 x 32 as the accumulators hold them: float4 64 g + lane of
+  // block n / 32 * rows_p / 32 + m / 32 is a lane's rows 8 g + ..
+  float *master;
+  long long master_stride;
   float a, b, c;
   // split K: `splits` workgroups a tile, each over `split_stages` stages; their sums, and a count of arrivals per tile
   int splits, split_stages;
@@ -319,6 +385,8 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
   // per lane by a transposition within quads (8 bytes a lane, 64 a row), the transposed copy of eight rows per lane by
   // exchanging with the lane of the other half (16 bytes).
   _Float16 *D = a.D + z * a.d_stride, *DT = a.DT + z * a.dt_stride;
+  const int *exp_m = a.exp_m + z * static_cast<long long>(a.exp_m_stride), *exp_n = a.exp_n + z * static_cast<long long>(a.exp_n_stride);
+  f32x4 *master = reinterpret_cast<f32x4 *>(a.master + z * a.master_stride);
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -326,44 +394,62 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
       const int m0 = bm * TM + (wm * FM + i) * 32, n0 = bn * TM + (wn * FN + j) * 32;
       if (m0 >= a.rows_p || n0 >= a.rows_q) continue;  // (32-row blocks are whole)
       const int n = n0 + l31;
+      f32x4 *copy32 = master + (static_cast<long long>(n0 >> 5) * (a.rows_p >> 5) + (m0 >> 5)) * 256 + lane;
+      const int start_n = exp_n[n], en = bound_of(start_n, a.shift, a.cap);
+      f32x4 kept[4];
+      i32x4 start_m[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        start_m[g] = *reinterpret_cast<const i32x4 *>(exp_m + m0 + 8 * g + 4 * hi);
+        if constexpr (EPI != GRAM) kept[g] = copy32[64 * g];
+      }
       uint32_t h[4][2], l[4][2];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int m = m0 + 8 * g + 4 * hi;
         float v[4];
+        int scale[4], turned;  // of the results' rows and of their transpose's
+        if constexpr (EPI == UPDATE || EPI == FINAL) turned = kTop - bound_of(start_n, a.next_shift, a.next_cap);
+        else turned = kTop - en - a.cap - (EPI == POLY ? a.poly : 0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * g + k];
-        if constexpr (EPI == GRAM) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
-        } else if constexpr (EPI == POLY) {
-          const _Float16 *at = a.P + z * a.p_stride + place(n, m, a.ldp);  // A[n][m] = A[m][n]
-          const f16x4 ah = *reinterpret_cast<const f16x4 *>(at), al = *reinterpret_cast<const f16x4 *>(at + kSecond);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            v[k] = a.c * (v[k] * (1.f / kScaleA)) + a.b * (static_cast<float>(ah[k]) + static_cast<float>(al[k])) +
-                   (m + k == n ? a.a * kScaleA : 0.f);
-        } else if constexpr (EPI == UPDATE) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= 1.f / kScaleA;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= 1.f / (kScaleA * kScaleX);
+        for (int k = 0; k < 4; ++k) {
+          const int em = bound_of(start_m[g][k], a.shift, a.cap);
+          const float sum = acc[i][j][4 * g + k];
+          if constexpr (EPI == GRAM) {
+            v[k] = times_power(sum, em + en - 2 * kTop);
+            scale[k] = kTop - em - a.cap;
+          } else if constexpr (EPI == POLY) {
+            v[k] = a.c * times_power(sum, em + en + 2 * (a.cap - kTop)) + a.b * kept[g][k];
+            scale[k] = kTop - em - a.cap - a.poly;
+          } else {
+            v[k] = a.a * kept[g][k] + times_power(sum, em + en + a.cap + a.poly - 2 * kTop);
+            scale[k] = kTop - bound_of(start_m[g][k], a.next_shift, a.next_cap);
+          }
+        }
+        if constexpr (EPI == FINAL) {
           put_final(a, z, m, n, n0 + (l31 & ~3), lane, v);
           continue;
         }
-        f16x4 vh, vl;
+        if constexpr (EPI != POLY) copy32[64 * g] = f32x4{v[0], v[1], v[2], v[3]};
+        auto terms = [&](auto by, u32x2 &high, u32x2 &low) {
+          f16x4 vh, vl;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          vh[k] = static_cast<_Float16>(v[k]);
-          vl[k] = static_cast<_Float16>(v[k] - static_cast<float>(vh[k]));
-        }
-        const u32x2 bh = __builtin_bit_cast(u32x2, vh), bl = __builtin_bit_cast(u32x2, vl);
+          for (int k = 0; k < 4; ++k) {
+            const float x = times_power(v[k], by(k));
+            vh[k] = static_cast<_Float16>(x);
+            vl[k] = static_cast<_Float16>(x - static_cast<float>(vh[k]));
+          }
+          high = __builtin_bit_cast(u32x2, vh);
+          low = __builtin_bit_cast(u32x2, vl);
+        };
+        u32x2 bh, bl;
+        terms([&](int) { return turned; }, bh, bl);
         h[g][0] = bh.x;
         h[g][1] = bh.y;
         l[g][0] = bl.x;
         l[g][1] = bl.y;
         if (EPI == UPDATE || bm != bn) {
+          terms([&](int k) { return scale[k]; }, bh, bl);
           _Float16 *at = D + place(m + (lane & 3), n0 + (l31 & ~3), a.ldd);
           const Pair2 th = quad_transpose(bh.x, bh.y, lane), tl = quad_transpose(bl.x, bl.y, lane);
           *reinterpret_cast<u32x2 *>(at) = u32x2{th.x, th.y};
@@ -386,31 +472,7 @@ __global__ __launch_bounds__(WR * WC * 64) void ns_gemm_kernel(const NsArgs a) {
     }
 }
 
-// this thread's share of a sum of squares over `count` values: thread `at` of `threads`
-template <typename V>
-__device__ __forceinline__ double sum_of_squares(const V *g, long long count, long long at, long long threads) {
-  constexpr int E = 16 / sizeof(V);
-  using Vec = __attribute__((ext_vector_type(E))) V;
-  typedef Vec Loose __attribute__((aligned(sizeof(V))));  // a matrix of the batch may start at any element
-  double s = 0;
-  const long long vectors = count / E;
-#pragma unroll 4
-  for (long long i = at; i < vectors; i += threads) {
-    const Vec v = *reinterpret_cast<const Loose *>(g + i * E);
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      const double x = static_cast<double>(static_cast<float>(v[k]));
-      s += x * x;
-    }
-  }
-  if (vectors * E + at < count) {  // fewer than E values are left: one each for the first threads
-    const double x = static_cast<double>(static_cast<float>(g[vectors * E + at]));
-    s += x * x;
-  }
-  return s;
-}
-
-// kScaleX / (|G| + eps) as a fraction in [1/2, 1) and a power of two: the norm may lie outside fp32's range.  (A product in
+// 1 / (|G| + eps) as a fraction in [1/2, 1) and a power of two: the norm may lie outside fp32's range.  (A product in
 // double that goes on to fp16 is converted by 30 integer instructions: packing 512 x 3136 f32 took 14.4 us, 9.8 so.)
 struct Scale {
   float fraction;
@@ -418,159 +480,312 @@ struct Scale {
 };
 __device__ __forceinline__ Scale scale_of(double squares, float eps) {
   Scale s;
-  s.fraction = static_cast<float>(frexp(kScaleX / (sqrt(squares) + eps), &s.power));
+  s.fraction = static_cast<float>(frexp(1.0 / (sqrt(squares) + eps), &s.power));
   return s;
 }
-__device__ __forceinline__ float scaled(float x, const Scale &s) { return ldexpf(x * s.fraction, s.power); }
-
-// sums of squares, gridDim.x partial sums per matrix
-template <typename V>
-__global__ __launch_bounds__(256) void ns_norm_kernel(const V *in, long long count, double *partials) {
-  __shared__ double scratch[4];
-  double s = sum_of_squares(in + blockIdx.y * count, count, blockIdx.x * 256LL + threadIdx.x, 256LL * gridDim.x);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) partials[blockIdx.y * static_cast<long long>(gridDim.x) + blockIdx.x] = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+__device__ __forceinline__ float scaled(float x, const Scale &s) { return times_power(x * s.fraction, s.power); }
+// exponent of a bound of the norm of `count` scaled values of which none passes `most`
+__device__ __forceinline__ int start_bound(float most, int count, const Scale &s) {
+  const int ceil_log2 = count <= 1 ? 0 : 32 - __builtin_clz(count - 1);
+  return most == 0.f ? kLowest : power_above(most) + s.power + (ceil_log2 + 1) / 2;
 }
 
-// X0 and its transpose from a 64 x 64 tile of G: `same` has G's orientation (ld_same), `turned` the other.  Also clears the
-// arrival counts of the split products.
+// over the 16 lanes of a DPP row
+template <int ROR>
+__device__ __forceinline__ float more_of(float v) {
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + ROR, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float most_of_16(float v) { return more_of<1>(more_of<2>(more_of<4>(more_of<8>(v)))); }
+
+// The sum of squares of a part of a matrix (`band` rows of `strip` columns) and the largest magnitudes of its rows and columns: a wave
+// per row and 64 vectors of it.
 template <typename V>
-__global__ __launch_bounds__(256) void ns_pack_kernel(const V *in, int m, int n, const double *partials, int parts, float eps, _Float16 *same,
-                                                      int ld_same, _Float16 *turned, int ld_turned, long long stride, unsigned *arrivals, int counts) {
+__global__ __launch_bounds__(256) void ns_scan_kernel(const V *in, int m, int n, int band, int strip, double *sums, float *row_most, float *col_most) {
+  constexpr int E = 16 / sizeof(V), C = 64 * E, U = 8;
+  using Vec = __attribute__((ext_vector_type(E))) V;
+  typedef Vec Loose __attribute__((aligned(sizeof(V))));  // a matrix of the batch may start at any element
+  __shared__ float rows[65536 / kScanParts], cols[4][C];
+  __shared__ double scratch[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long z = blockIdx.z;
+  const V *g = in + z * m * n;
+  const int r0 = blockIdx.y * band, r1 = min(m, r0 + band), c0 = blockIdx.x * strip, c1 = min(n, c0 + strip);
+  double s = 0;
+  for (int chunk = c0; chunk < c1; chunk += C) {
+    const int col = chunk + lane * E;
+    float top[E] = {};
+    for (int base = r0 + wave; base < r1; base += 4 * U) {
+      Vec v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = base + 4 * u;
+        v[u] = Vec{};
+        if (row >= r1) continue;
+        const V *from = g + static_cast<long long>(row) * n + col;
+        if (col + E <= n) v[u] = *reinterpret_cast<const Loose *>(from);
+        else
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (col + k < n) v[u][k] = from[k];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = base + 4 * u;
+        if (row >= r1) continue;  // (the wave's)
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          const float x = fabsf(static_cast<float>(v[u][k]));
+          top[k] = fmaxf(top[k], x);
+          most = fmaxf(most, x);
+          s += static_cast<double>(x) * x;
+        }
+        most = most_of_16(most);
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        if (lane == 0) rows[row - r0] = chunk == c0 ? most : fmaxf(rows[row - r0], most);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) cols[wave][lane * E + k] = top[k];
+    __syncthreads();
+    for (int i = threadIdx.x; i < C && chunk + i < n; i += 256)
+      col_most[(z * gridDim.y + blockIdx.y) * n + chunk + i] = fmaxf(fmaxf(cols[0][i], cols[1][i]), fmaxf(cols[2][i], cols[3][i]));
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < r1 - r0; i += 256) row_most[(z * gridDim.x + blockIdx.x) * m + r0 + i] = rows[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (lane == 0) scratch[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) sums[(z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+}
+
+struct PackArgs {
+  const void *in;
+  int m, n, tall;
+  int bands, strips;  // of the scan
+  const double *sums;
+  const float *row_most, *col_most;
+  float eps;
+  _Float16 *same, *turned;  // X0 in G's orientation and in the other
+  int ld_same, ld_turned;
+  long long stride;
+  float *master;
+  long long master_stride;
+  int rows_x;               // padded rows of X, blocks of the copy
+  int *exp_row, *exp_col;   // of G's rows and columns
+  int exp_row_stride, exp_col_stride;
+  int cap;
+  unsigned *arrivals;
+  int counts;
+};
+
+// X0, its transpose, its fp32 copy and the exponents from a 64 x 64 tile of G.  Also clears the arrival counts of the split products.
+template <typename V>
+__global__ __launch_bounds__(256) void ns_pack_kernel(const PackArgs a) {
   constexpr int E = 16 / sizeof(V);
   using Vec = __attribute__((ext_vector_type(E))) V;
   typedef Vec Loose __attribute__((aligned(sizeof(V))));
-  __shared__ float tile[64][65];
+  __shared__ float tile[64][65], most[4][64];
+  __shared__ int exps[2][64];
   __shared__ double total[4];
   const long long z = blockIdx.z;
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-  const V *g = in + z * m * n;
+  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const V *g = static_cast<const V *>(a.in) + z * a.m * a.n;
   if (blockIdx.x == 0 && blockIdx.y == 0 && z == 0)
-    for (int i = threadIdx.x; i < counts; i += 256) arrivals[i] = 0;
+    for (int i = threadIdx.x; i < a.counts; i += 256) a.arrivals[i] = 0;
   // 64 rows of 64 / E vectors, all on their way before the first is waited for
   constexpr int kVecs = 64 * 64 / E / 256;
   Vec v[kVecs];
-  if (r0 + 64 <= m && c0 + 64 <= n) {
+  if (r0 + 64 <= a.m && c0 + 64 <= a.n) {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int at = k * 256 + threadIdx.x;
-      v[k] = *reinterpret_cast<const Loose *>(g + static_cast<long long>(r0 + at / (64 / E)) * n + c0 + at % (64 / E) * E);
+      v[k] = *reinterpret_cast<const Loose *>(g + static_cast<long long>(r0 + at / (64 / E)) * a.n + c0 + at % (64 / E) * E);
     }
   } else {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int at = k * 256 + threadIdx.x, row = at / (64 / E), col = at % (64 / E) * E;
       v[k] = Vec{};
-      if (r0 + row < m) {
-        const V *from = g + static_cast<long long>(r0 + row) * n + c0 + col;
-        if (c0 + col + E <= n) v[k] = *reinterpret_cast<const Loose *>(from);
+      if (r0 + row < a.m) {
+        const V *from = g + static_cast<long long>(r0 + row) * a.n + c0 + col;
+        if (c0 + col + E <= a.n) v[k] = *reinterpret_cast<const Loose *>(from);
         else
 #pragma unroll
           for (int i = 0; i < E; ++i)
-            if (c0 + col + i < n) v[k][i] = from[i];
+            if (c0 + col + i < a.n) v[k][i] = from[i];
       }
     }
   }
+  const int parts = a.bands * a.strips;
   double s = 0;
-  for (int i = threadIdx.x; i < parts; i += 256) s += partials[z * parts + i];
+  for (int i = threadIdx.x; i < parts; i += 256) s += a.sums[z * parts + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = s;
+  if (lane == 0) total[wave] = s;
+  {  // the largest magnitudes: waves 0 and 1 of the rows, 2 and 3 of the columns, half of the parts each
+    const bool rows = wave < 2;
+    const int at = (rows ? r0 : c0) + lane, side = rows ? a.m : a.n, count = rows ? a.strips : a.bands;
+    const float *from = (rows ? a.row_most : a.col_most) + z * count * static_cast<long long>(side) + at;
+    float x = 0.f;
+    if (at < side)
+#pragma unroll 8
+      for (int i = wave & 1; i < count; i += 2) x = fmaxf(x, from[static_cast<long long>(i) * side]);
+    most[wave][lane] = x;
+  }
+  __syncthreads();
+  const Scale scale = scale_of(total[0] + total[1] + total[2] + total[3], a.eps);
+  if (wave == 0) {
+    exps[0][lane] = start_bound(fmaxf(most[0][lane], most[1][lane]), a.n, scale);
+    if (blockIdx.x == 0) a.exp_row[z * a.exp_row_stride + r0 + lane] = exps[0][lane];
+  } else if (wave == 1) {
+    exps[1][lane] = start_bound(fmaxf(most[2][lane], most[3][lane]), a.m, scale);
+    if (blockIdx.y == 0) a.exp_col[z * a.exp_col_stride + c0 + lane] = exps[1][lane];
+  }
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
     const int at = k * 256 + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < E; ++i) tile[at / (64 / E)][at % (64 / E) * E + i] = static_cast<float>(v[k][i]);
+    for (int i = 0; i < E; ++i) tile[at / (64 / E)][at % (64 / E) * E + i] = scaled(static_cast<float>(v[k][i]), scale);
   }
   __syncthreads();
-  const Scale scale = scale_of(total[0] + total[1] + total[2] + total[3], eps);
-  const int mp = (m + kPad - 1) / kPad * kPad, np = (n + kPad - 1) / kPad * kPad;
-  auto put8 = [&](_Float16 *at, auto value) {
+  auto put8 = [&](_Float16 *at, int exponent, auto value) {
+    const int by = kTop - bound_of(exponent, 0, a.cap);
     f16x8 h, l;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float v = scaled(value(i), scale);
-      h[i] = static_cast<_Float16>(v);
-      l[i] = static_cast<_Float16>(v - static_cast<float>(h[i]));
+      const float x = times_power(value(i), by);
+      h[i] = static_cast<_Float16>(x);
+      l[i] = static_cast<_Float16>(x - static_cast<float>(h[i]));
     }
     *reinterpret_cast<f16x8 *>(at) = h;
     *reinterpret_cast<f16x8 *>(at + kSecond) = l;
   };
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {  // 64 rows of 8 x 8 values; the sides are multiples of 64: a row of 8 is whole or outside
+  for (int k = 0; k < 2; ++k) {  // 64 rows of 8 x 8 values (the padded sides are multiples of 64)
     const int at = k * 256 + threadIdx.x, row = at >> 3, col = (at & 7) * 8;
-    if (r0 + row < mp && c0 + col < np) put8(same + z * stride + place(r0 + row, c0 + col, ld_same), [&](int i) { return tile[row][col + i]; });
-    if (c0 + row < np && r0 + col < mp) put8(turned + z * stride + place(c0 + row, r0 + col, ld_turned), [&](int i) { return tile[col + i][row]; });
+    put8(a.same + z * a.stride + place(r0 + row, c0 + col, a.ld_same), exps[0][row], [&](int i) { return tile[row][col + i]; });
+    put8(a.turned + z * a.stride + place(c0 + row, r0 + col, a.ld_turned), exps[1][row], [&](int i) { return tile[col + i][row]; });
+  }
+  const int xm = a.tall ? c0 : r0, xn = a.tall ? r0 : c0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {  // blocks (k & 1, k >> 1) of 32 x 32, as the products' accumulators hold them
+    const int row = (k & 1) * 32 + wave * 8 + (lane >> 5) * 4, col = (k >> 1) * 32 + (lane & 31);
+    f32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a.tall ? tile[col][row + i] : tile[row + i][col];
+    const long long block = static_cast<long long>((xn >> 5) + (k >> 1)) * (a.rows_x >> 5) + (xm >> 5) + (k & 1);
+    reinterpret_cast<f32x4 *>(a.master + z * a.master_stride)[block * 256 + threadIdx.x] = x;
   }
 }
 
 // ---- matrices that fit a workgroup's LDS: the whole iteration in ONE launch, a workgroup per matrix -----------------
-// X, X^T, A and B stay in LDS (rows padded by 16 bytes: an odd number of 16-byte chunks, so that 16 rows' equal chunks meet
-// every bank once); 16 waves share the 16 x 16 x 32 tiles of each product.  The update holds its tiles in registers over a
-// barrier and then overwrites X and X^T.  What bounds it is the chain of 3 x steps dependent products, not their rate.
+// X, X^T, A and M stay in LDS (rows padded by 16 bytes: an odd number of 16-byte chunks, so that 16 rows' equal chunks meet
+// every bank once); 16 waves share the 16 x 16 x 32 tiles of each product, every wave the same ones in every step, so that the
+// fp32 copies of X and A are in its registers (G too: it is read once).  What bounds it is the chain of 3 x steps dependent
+// products, not their rate.
 // LDS is addressed by plain offsets into one array: through pointers that are chosen at run time the compiler cannot see that
 // they are LDS, and flat accesses and spills made a step of 64 x 64 f32 3.9 us long (1.5 now).
 constexpr int kSmallWaves = 16;
-constexpr long long kSmallLds = 160 * 1024 - 256;
+constexpr long long kSmallLds = 160 * 1024;
 
+// bytes: the matrices, the exponents of X's rows and columns, the parts of the norm; more than there are if the waves cannot hold X
 inline long long small_lds(int rp, int cp) {
-  if (rp > 64 && rp / 32 * (cp / 32) > kSmallWaves) return kSmallLds + 1;  // more blocks of 32 x 32 than waves: see launch_small
-  return 4LL * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8)) + 8LL * rp * (rp + 8);
+  if (rp > 64 ? rp / 32 * (cp / 32) > kSmallWaves : cp / 16 > kSmallWaves * (rp > 32 ? 1 : 2)) return kSmallLds + 1;
+  return 4LL * (static_cast<long long>(rp) * (cp + 8) + static_cast<long long>(cp) * (rp + 8)) + 8LL * rp * (rp + 8) + 4LL * (rp + cp) + 8 * kSmallWaves;
 }
 
+// (the powers of every step are formed on the host: on the device a step's cost 1 us of its 4)
+constexpr int kSmallSteps = 32;
 struct SmallArgs {
   const void *in;
   void *out;
   int m, n, r, c, rp, cp, steps, tall;
   float a, b, k, eps;
+  Powers powers[kSmallSteps + 1];
 };
 
 // SIDE: the products are formed in blocks of 16 x 16 (one instruction tile: the shortest chain, and enough blocks of A for the
-// waves up to 64 rows) or 32 x 32 (two fragments of each side for four tiles: half the LDS reads).  us for 5 steps: 17 x 300 f32
-// 20 at 16, 32 at 32; 64 x 400 bf16 35, 38; 128 x 128 bf16 40, 34.
-// COLUMN = 0: X has no more blocks than there are waves; a block is held over a barrier before it overwrites X.
-// COLUMN > 0: a wave takes columns of blocks, which depend on nothing but themselves: held, COLUMN of them at most, without a
-// barrier, their X^T fragments read once (64 x 400 bf16: blocks dealt out, held and written by straight code 51 us, half of
+// waves up to 64 rows) or 32 x 32 (two fragments of each side for four tiles: half the LDS reads).
+// COLUMNS = 0: X has no more blocks than there are waves; a block is held over a barrier before it overwrites X.
+// COLUMNS > 0: a wave takes COLUMNS columns of BLOCKS blocks at most, which depend on nothing but themselves: held without a
+// barrier, their X^T fragments read once (64 x 400 of one term: blocks dealt out, held and written by straight code 51 us, half of
 // them its instruction fetches; by columns 35).
-template <typename V, int SIDE, int COLUMN>
+template <typename V, int SIDE, int COLUMNS, int BLOCKS>
 __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallArgs a) {
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
-  __shared__ double parts[kSmallWaves];
-  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, quad = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63;
+  int l15 = lane & 15, quad = lane >> 4;
+  // (opaque: addresses that do not change would be kept over the steps, more than there are registers)
+  auto forget = [&] { asm volatile("" : "+v"(l15), "+v"(quad)); };
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ldx = a.cp + 8, ldr = a.rp + 8;  // X: rp rows of ldx; X^T: cp rows of ldr; A, B: rp rows of ldr
+  const int ldx = a.cp + 8, ldr = a.rp + 8;  // X: rp rows of ldx; X^T: cp rows of ldr; A, M: rp rows of ldr
   // each array: its first terms, then its second ones
   const int sx = a.rp * ldx, st = a.cp * ldr, sa = a.rp * ldr;
-  const int X = 0, XT = X + 2 * sx, A = XT + 2 * st, B = A + 2 * sa;
-  auto put1 = [&](int at, int size, float v) {
-    const _Float16 h = static_cast<_Float16>(v);
-    lds[at] = h;
-    lds[at + size] = static_cast<_Float16>(v - static_cast<float>(h));
-  };
-  // four consecutive rows of a column: into the row of the transpose (`turned`) and, if wanted, into four rows (`at`, ld apart)
-  auto put4 = [&](int turned, int turned_size, int at, int ld, int size, bool both, f32x4 v) {
-    f16x4 h, l;
+  const int X = 0, XT = X + 2 * sx, A = XT + 2 * st, M = A + 2 * sa;
+  double *parts = reinterpret_cast<double *>(lds + M + 2 * sa);
+  int *exp_row = reinterpret_cast<int *>(parts + kSmallWaves), *exp_col = exp_row + a.rp;  // first the largest magnitudes' bits
+  constexpr int F = SIDE / 16, kCols = COLUMNS > 0 ? COLUMNS : 1;
+  struct Block { f32x4 v[F][F]; };
+  const int tr = a.rp / SIDE, tc = a.cp / SIDE, upper = tr * (tr + 1) / 2;
+  // this wave's blocks of X: (i, tn) or, where COLUMNS = 0, one; accumulator e of a lane and 16 x 16 tile: row 4 (lane / 16) + e,
+  // column lane % 16
+  auto block_row = [&](int i) { return COLUMNS > 0 ? i * SIDE : wave % tr * SIDE; };
+  auto block_col = [&](int it) { return COLUMNS > 0 ? (wave + it * kSmallWaves) * SIDE : wave / tr * SIDE; };
+  auto has = [&](int i, int it) { return COLUMNS > 0 ? i < tr && wave + it * kSmallWaves < tc : wave < tr * tc; };
+  Block x[kCols][BLOCKS];
+  const V *in = static_cast<const V *>(a.in) + blockIdx.x * (static_cast<long long>(a.m) * a.n);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[k] = static_cast<_Float16>(v[k]);
-      l[k] = static_cast<_Float16>(v[k] - static_cast<float>(h[k]));
-    }
-    *reinterpret_cast<f16x4 *>(lds + turned) = h;
-    *reinterpret_cast<f16x4 *>(lds + turned + turned_size) = l;
-    if (both) {
+  for (int it = 0; it < kCols; ++it)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        lds[at + k * ld] = h[k];
-        lds[at + k * ld + size] = l[k];
+    for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int g = 0; g < F; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = block_row(i) + f * 16 + 4 * quad + e, col = block_col(it) + g * 16 + l15;
+            const int r0 = min(row, a.r - 1), c0 = min(col, a.c - 1);
+            const float v = static_cast<float>(in[a.tall ? c0 * a.n + r0 : r0 * a.n + c0]);
+            x[it][i].v[f][g][e] = has(i, it) && row < a.r && col < a.c ? v : 0.f;
+          }
+  for (int i = tid; i < a.rp + a.cp; i += kSmallWaves * 64) exp_row[i] = 0;
+  __syncthreads();
+  double s = 0;
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float most = 0.f;
+#pragma unroll
+        for (int it = 0; it < kCols; ++it)
+#pragma unroll
+          for (int g = 0; g < F; ++g) {
+            const float v = x[it][i].v[f][g][e];
+            s += static_cast<double>(v) * v;
+            most = fmaxf(most, fabsf(v));
+          }
+        most = most_of_16(most);
+        if (l15 == 0 && has(i, 0)) atomicMax(exp_row + block_row(i) + f * 16 + 4 * quad + e, __builtin_bit_cast(int, most));
       }
+#pragma unroll
+  for (int it = 0; it < kCols; ++it)
+#pragma unroll
+    for (int g = 0; g < F; ++g) {
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[it][i].v[f][g][e]));
+      if (has(0, it)) atomicMax(exp_col + block_col(it) + g * 16 + l15, __builtin_bit_cast(int, most));
     }
-  };
-  const int count = a.m * a.n;
-  const V *in = static_cast<const V *>(a.in) + blockIdx.x * static_cast<long long>(count);
-  double s = sum_of_squares(in, count, tid, kSmallWaves * 64);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if (lane == 0) parts[wave] = s;
@@ -579,28 +794,54 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
 #pragma unroll
   for (int i = 0; i < kSmallWaves; ++i) s += parts[i];
   const Scale scale = scale_of(s, a.eps);
-  for (int row = wave; row < a.rp; row += kSmallWaves)  // a wave per row of X, 256 columns' loads at a time
-    for (int col0 = lane; col0 < a.cp; col0 += 256) {
-      V g[4];
+  for (int i = tid; i < a.rp + a.cp; i += kSmallWaves * 64)
+    exp_row[i] = start_bound(__builtin_bit_cast(float, exp_row[i]), i < a.rp ? a.c : a.r, scale);
+  __syncthreads();
+  // four consecutive rows of a column, scaled by 2^turn into the row of the transpose and, if wanted, each by its own power into four rows
+  auto put4 = [&](int turned, int turned_size, int turn, int at, int ld, int size, i32x4 by, bool both, f32x4 v) {
+    f16x4 h, l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float y = times_power(v[k], turn);
+      h[k] = static_cast<_Float16>(y);
+      l[k] = static_cast<_Float16>(y - static_cast<float>(h[k]));
+    }
+    *reinterpret_cast<f16x4 *>(lds + turned) = h;
+    *reinterpret_cast<f16x4 *>(lds + turned + turned_size) = l;
+    if (both) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int col = min(col0 + 64 * k, a.c - 1), from = min(row, a.r - 1);
-        g[k] = in[a.tall ? col * a.n + from : from * a.n + col];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int col = col0 + 64 * k;
-        if (col >= a.cp) continue;
-        const float v = row < a.r && col < a.c ? scaled(static_cast<float>(g[k]), scale) : 0.f;
-        put1(X + row * ldx + col, sx, v);
-        put1(XT + col * ldr + row, st, v);
+        const float y = times_power(v[k], by[k]);
+        const _Float16 high = static_cast<_Float16>(y);
+        lds[at + k * ld] = high;
+        lds[at + k * ld + size] = static_cast<_Float16>(y - static_cast<float>(high));
       }
     }
+  };
+  auto put_x = [&](int m, int n, const Powers &k, f32x4 v) {
+    const i32x4 start = *reinterpret_cast<const i32x4 *>(exp_row + m);
+    i32x4 by;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) by[e] = kTop - bound_of(start[e], k.shift, k.cap);
+    put4(XT + n * ldr + m, st, kTop - bound_of(exp_col[n], k.shift, k.cap), X + m * ldx + n, ldx, sx, by, true, v);
+  };
+#pragma unroll
+  for (int it = 0; it < kCols; ++it)
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      if (!has(i, it)) continue;
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int g = 0; g < F; ++g) {
+          f32x4 &v = x[it][i].v[f][g];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = scaled(v[e], scale);
+          put_x(block_row(i) + f * 16 + 4 * quad, block_col(it) + g * 16 + l15, a.powers[0], v);
+        }
+    }
   __syncthreads();
-  // acc[i] = rows SIDE i .. of P times SIDE rows of Q transposed, the first `count` of N blocks.  Accumulator e of a lane and
-  // 16 x 16 tile: row 4 (lane / 16) + e, column lane % 16
-  constexpr int F = SIDE / 16, kHeld = COLUMN > 0 ? COLUMN : 1;
-  struct Block { f32x4 v[F][F]; };
+  // acc[i] = rows SIDE i .. of P times SIDE rows of Q transposed, the first `count` of N blocks
   auto products = [&](auto &acc, int count, int P, int ldp, int sp, int Q, int ldq, int sq, int K) {
     constexpr int N = sizeof(acc) / sizeof(Block);
     Block cross[N];
@@ -642,94 +883,123 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(const SmallA
 #pragma unroll
         for (int g = 0; g < F; ++g) acc[i].v[f][g] += cross[i].v[f][g];
   };
-  const int tr = a.rp / SIDE, tc = a.cp / SIDE, upper = tr * (tr + 1) / 2;
+  // this wave's block of A and M: there are 10 at most (rp <= 64 in blocks of 16, <= 128 of 32), on and above the diagonal
+  int pm = 0, qn = 0;
+  if (wave < upper) {
+    int left = wave, row = 0;
+    while (left >= tr - row) left -= tr - row++;
+    pm = row * SIDE;
+    qn = (row + left) * SIDE;
+  }
+  Block gram[1], acc[1];
 #pragma unroll 1
   for (int step = 0; step < a.steps; ++step) {
-    // A = X X^T, then B = a I + b A + c A A: their upper triangles, stored twice
-#pragma unroll 1
+    const bool last = step + 1 == a.steps;
+    const Powers known = a.powers[step], next = a.powers[step + 1];
+    // A = X X^T, then M = b A + c A A: their upper triangles, stored twice
+#pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int to = half ? B : A;
-#pragma unroll 1
-      for (int tile = wave; tile < upper; tile += kSmallWaves) {
-        int left = tile, row = 0;
-        while (left >= tr - row) left -= tr - row++;
-        const int pm = row * SIDE, qn = (row + left) * SIDE;
-        Block acc[1];
+      forget();
+      if (wave < upper) {
         if (half) products(acc, 1, A + pm * ldr, ldr, sa, A + qn * ldr, ldr, sa, a.rp);
-        else products(acc, 1, X + pm * ldx, ldx, sx, X + qn * ldx, ldx, sx, a.cp);
+        else products(gram, 1, X + pm * ldx, ldx, sx, X + qn * ldx, ldx, sx, a.cp);
+        const int to = half ? M : A, less = known.cap + (half ? known.poly : 0);
 #pragma unroll
         for (int f = 0; f < F; ++f)
 #pragma unroll
           for (int g = 0; g < F; ++g) {
             const int m = pm + f * 16 + 4 * quad, n = qn + g * 16 + l15;
-            f32x4 v = acc[0].v[f][g] * (half ? a.k / kScaleA : kScaleA / (kScaleX * kScaleX));
-            if (half) {
-              const f16x4 h = *reinterpret_cast<const f16x4 *>(lds + A + n * ldr + m);
-              const f16x4 l = *reinterpret_cast<const f16x4 *>(lds + A + n * ldr + m + sa);
+            const i32x4 start = *reinterpret_cast<const i32x4 *>(exp_row + m);
+            const int en = bound_of(exp_row[n], known.shift, known.cap);
+            i32x4 by;
+            f32x4 v;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) v[k] += a.b * (static_cast<float>(h[k]) + static_cast<float>(l[k])) + (m + k == n ? a.a * kScaleA : 0.f);
+            for (int e = 0; e < 4; ++e) {
+              const int em = bound_of(start[e], known.shift, known.cap);
+              if (half) v[e] = a.k * times_power(acc[0].v[f][g][e], em + en + 2 * (known.cap - kTop)) + a.b * gram[0].v[f][g][e];
+              else v[e] = times_power(gram[0].v[f][g][e], em + en - 2 * kTop);
+              by[e] = kTop - em - less;
             }
-            put4(to + n * ldr + m, sa, to + m * ldr + n, ldr, sa, pm != qn, v);
+            if (!half) gram[0].v[f][g] = v;
+            put4(to + n * ldr + m, sa, kTop - en - less, to + m * ldr + n, ldr, sa, by, pm != qn, v);
           }
       }
       __syncthreads();
     }
-    const bool last = step + 1 == a.steps;
-    auto put_block = [&](int tm, int tn, const Block &b) {
+    forget();
+    Block held[BLOCKS];
 #pragma unroll
-      for (int f = 0; f < F; ++f)
+    for (int it = 0; it < kCols; ++it) {
+      if (COLUMNS > 0 && !has(0, it)) continue;
+      if (has(0, it)) products(held, tr, M + (COLUMNS > 0 ? 0 : block_row(0)) * ldr, ldr, sa, XT + block_col(it) * ldr, ldr, st, a.rp);
+      if (COLUMNS == 0) __syncthreads();
 #pragma unroll
-        for (int g = 0; g < F; ++g) {
-          const int m = tm * SIDE + f * 16 + 4 * quad, n = tn * SIDE + g * 16 + l15;
-          const f32x4 v = b.v[f][g] * (1.f / kScaleA);
-          if (!last) {
-            put4(XT + n * ldr + m, st, X + m * ldx + n, ldx, sx, true, v);
-          } else {
-            V *out = static_cast<V *>(a.out) + blockIdx.x * static_cast<long long>(count);
+      for (int i = 0; i < BLOCKS; ++i) {
+        if (!has(i, it)) continue;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (m + k < a.r && n < a.c) out[a.tall ? n * a.n + m + k : (m + k) * a.n + n] = static_cast<V>(v[k] * (1.f / kScaleX));
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+          for (int g = 0; g < F; ++g) {
+            const int m = block_row(i) + f * 16 + 4 * quad, n = block_col(it) + g * 16 + l15;
+            const i32x4 start = *reinterpret_cast<const i32x4 *>(exp_row + m);
+            const int en = bound_of(exp_col[n], known.shift, known.cap) + known.cap + known.poly - 2 * kTop;
+            f32x4 &v = x[it][i].v[f][g];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = a.a * v[e] + times_power(held[i].v[f][g][e], bound_of(start[e], known.shift, known.cap) + en);
+            if (!last) {
+              put_x(m, n, next, v);
+            } else {
+              V *out = static_cast<V *>(a.out) + blockIdx.x * (static_cast<long long>(a.m) * a.n);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (m + e < a.r && n < a.c) out[a.tall ? n * a.n + m + e : (m + e) * a.n + n] = static_cast<V>(v[e]);
+            }
           }
-        }
-    };
-    Block held[kHeld];
-    if constexpr (COLUMN == 0) {
-      if (wave < tr * tc) products(held, 1, B + wave % tr * SIDE * ldr, ldr, sa, XT + wave / tr * SIDE * ldr, ldr, st, a.rp);
-      __syncthreads();
-      if (wave < tr * tc) put_block(wave % tr, wave / tr, held[0]);
-    } else {
-#pragma unroll 1
-      for (int tn = wave; tn < tc; tn += kSmallWaves) {
-        products(held, tr, B, ldr, sa, XT + tn * SIDE * ldr, ldr, st, a.rp);
-#pragma unroll
-        for (int i = 0; i < COLUMN; ++i)
-          if (i < tr) put_block(i, tn, held[i]);
       }
     }
     __syncthreads();
   }
 }
 
-template <typename V, int SIDE, int COLUMN>
+template <typename V, int SIDE, int COLUMNS, int BLOCKS>
 int launch_small_as(const SmallArgs &q, int batch, int bytes, hipStream_t s) {
-  DX_LDS_OPT_IN((ns_small_kernel<V, SIDE, COLUMN>), kSmallLds);
-  hipLaunchKernelGGL((ns_small_kernel<V, SIDE, COLUMN>), dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
+  DX_LDS_OPT_IN((ns_small_kernel<V, SIDE, COLUMNS, BLOCKS>), kSmallLds);
+  hipLaunchKernelGGL((ns_small_kernel<V, SIDE, COLUMNS, BLOCKS>), dim3(batch), dim3(kSmallWaves * 64), bytes, s, q);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
 template <typename V>
 int launch_small(const SmallArgs &q, int batch, int bytes, hipStream_t s) {
   const int blocks = q.rp / 32 * (q.cp / 32);
-  if (blocks * 4 <= kSmallWaves) return launch_small_as<V, 16, 0>(q, batch, bytes, s);
-  if (q.rp <= 32) return launch_small_as<V, 16, 2>(q, batch, bytes, s);
-  if (q.rp <= 64) return launch_small_as<V, 16, 4>(q, batch, bytes, s);
-  return launch_small_as<V, 32, 0>(q, batch, bytes, s);
+  if (blocks * 4 <= kSmallWaves) return launch_small_as<V, 16, 0, 1>(q, batch, bytes, s);
+  if (q.rp <= 32) return launch_small_as<V, 16, 2, 2>(q, batch, bytes, s);
+  if (q.rp <= 64) return launch_small_as<V, 16, 1, 4>(q, batch, bytes, s);
+  return launch_small_as<V, 32, 0, 1>(q, batch, bytes, s);
 }
 
+struct Scan {
+  int bands, strips, band, strip;  // workgroups along the rows and the columns, rows and columns of each
+  long long floats() const { return static_cast<long long>(rows) * strips + static_cast<long long>(columns) * bands; }
+  int rows, columns;
+};
+Scan make_scan(int dtype, int m, int n) {
+  const int chunk = dtype == DX_F32 ? 256 : 512;  // a wave's 16-byte vectors of a row; 8 rows a workgroup at least
+  Scan s;
+  s.rows = m;
+  s.columns = n;
+  const int chunks = cdiv(n, chunk), eights = cdiv(m, 8);
+  s.strip = cdiv(chunks, chunks < kScanParts ? chunks : kScanParts) * chunk;
+  s.strips = cdiv(n, s.strip);
+  s.band = cdiv(eights, eights < kScanParts ? eights : kScanParts) * 8;
+  s.bands = cdiv(m, s.band);
+  return s;
+}
 struct Plan {
-  int r, c, rp, cp, parts;
-  long long x, sq;             // halves of X and of A per matrix, both terms, padded
-  long long split_floats, bytes;
+  int r, c, rp, cp;
+  Scan scan;
+  long long x, sq;             // values of X and of A per matrix, padded
+  long long split_floats, sums, most, bytes;
 };
 Plan make_plan(int dtype, int batch, int m, int n) {
   Plan p;
@@ -737,13 +1007,17 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   p.c = m < n ? n : m;
   p.rp = (p.r + kPad - 1) / kPad * kPad;
   p.cp = (p.c + kPad - 1) / kPad * kPad;
-  p.x = 2LL * p.rp * p.cp;
-  p.sq = 2LL * p.rp * p.rp;
-  // X, two copies of X^T, A, B, and the norm's partial sums
-  const long long blocks = (static_cast<long long>(m) * n * (dtype == DX_F32 ? 4 : 2) + 32767) / 32768;  // 32 KB a workgroup at least
-  p.parts = static_cast<int>(blocks < kNormParts ? blocks : kNormParts);
+  p.x = static_cast<long long>(p.rp) * p.cp;
+  p.sq = static_cast<long long>(p.rp) * p.rp;
+  p.scan = make_scan(dtype, m, n);
+  const Scan other = make_scan(dtype, n, m);  // (a matrix and its transpose take the same workspace)
+  auto most = [](long long x, long long y) { return x > y ? x : y; };
+  p.sums = most(p.scan.bands * p.scan.strips, other.bands * other.strips);
+  p.most = most(p.scan.floats(), other.floats());
   p.split_floats = static_cast<long long>(kSplitGroups) * (p.r > 1024 ? 128 * 128 : 64 * 64);  // (128 x 128 tiles are split where there are many)
-  p.bytes = batch * (2 * (3 * p.x + 2 * p.sq) + 8LL * p.parts) + 4LL * kSplitGroups + 4 * p.split_floats;
+  // two terms of X, two copies of X^T, A and M; fp32 copies of X and A; the parts of split products; the norm's sums, the exponents,
+  // the largest magnitudes
+  p.bytes = batch * (4 * (3 * p.x + 2 * p.sq) + 4 * (p.x + p.sq) + 8 * p.sums + 4LL * (p.rp + p.cp) + 4 * p.most) + 4LL * kSplitGroups + 4 * p.split_floats;
   return p;
 }
 int check_shape(int dtype, int batch, int m, int n) {
@@ -804,33 +1078,63 @@ int launch_gemm(const NsArgs &a, int batch, hipStream_t s) {
   if (c.tile == 128) return launch_tile<128, 2, 2, 2, EPI>(a, batch, c.splits, s);
   return launch_tile<64, 2, 2, 4, EPI>(a, batch, c.splits, s);
 }
-int run_steps(const Plan &p, int batch, int steps, NsArgs a, _Float16 *X, _Float16 *XT0, _Float16 *XT1, _Float16 *A, _Float16 *B, hipStream_t s) {
+struct Buffers {
+  _Float16 *X, *XT[2], *A, *M;
+  float *master_x, *master_a;
+  int *exp_r, *exp_c;
+};
+int run_steps(const Plan &p, int batch, int steps, NsArgs a, const Buffers &w, hipStream_t s) {
+  Known known = known_at_start(a.b, a.c);
   for (int k = 0; k < steps; ++k) {
-    _Float16 *xt = k & 1 ? XT1 : XT0, *next = k & 1 ? XT0 : XT1;
+    const Known next = grown(known, a.a, a.b, a.c);
     NsArgs g = a;
-    g.P = g.Q = X;
-    g.p_stride = g.q_stride = p.x;
+    g.shift = known.shift;
+    g.cap = known.cap;
+    g.poly = known.poly;
+    g.next_shift = next.shift;
+    g.next_cap = next.cap;
+    g.P = g.Q = w.X;
+    g.p_stride = g.q_stride = 2 * p.x;
     g.ldp = g.ldq = g.K = p.cp;
     g.rows_p = g.rows_q = p.rp;
-    g.D = g.DT = A;
-    g.d_stride = g.dt_stride = p.sq;
+    g.D = g.DT = w.A;
+    g.d_stride = g.dt_stride = 2 * p.sq;
     g.ldd = g.lddt = p.rp;
+    g.exp_m = g.exp_n = w.exp_r;
+    g.exp_m_stride = g.exp_n_stride = p.rp;
+    g.master = w.master_a;
+    g.master_stride = p.sq;
     if (int rc = launch_gemm<GRAM>(g, batch, s)) return rc;
-    g.P = g.Q = A;
-    g.p_stride = g.q_stride = p.sq;
+    g.P = g.Q = w.A;
+    g.p_stride = g.q_stride = 2 * p.sq;
     g.ldp = g.ldq = g.K = p.rp;
-    g.D = g.DT = B;
+    g.D = g.DT = w.M;
     if (int rc = launch_gemm<POLY>(g, batch, s)) return rc;
-    g.P = B;
-    g.Q = xt;
-    g.q_stride = p.x;
+    g.P = w.M;
+    g.Q = w.XT[k & 1];
+    g.q_stride = 2 * p.x;
     g.rows_q = p.cp;
-    g.D = X;
-    g.DT = next;
-    g.d_stride = g.dt_stride = p.x;
+    g.D = w.X;
+    g.DT = w.XT[1 - (k & 1)];
+    g.d_stride = g.dt_stride = 2 * p.x;
     g.ldd = p.cp;
+    g.exp_n = w.exp_c;
+    g.exp_n_stride = p.cp;
+    g.master = w.master_x;
+    g.master_stride = p.x;
     if (int rc = k + 1 < steps ? launch_gemm<UPDATE>(g, batch, s) : launch_gemm<FINAL>(g, batch, s)) return rc;
+    known = next;
   }
+  return DX_OK;
+}
+
+template <typename V>
+int launch_start(const V *update, const Plan &p, int batch, PackArgs k, double *sums, float *row_most, float *col_most, hipStream_t s) {
+  hipLaunchKernelGGL(ns_scan_kernel<V>, dim3(p.scan.strips, p.scan.bands, batch), dim3(256), 0, s, update, k.m, k.n, p.scan.band, p.scan.strip, sums, row_most,
+                     col_most);
+  DX_LAUNCH_CHECK();
+  hipLaunchKernelGGL(ns_pack_kernel<V>, dim3(cdiv(k.n, kPad), cdiv(k.m, kPad), batch), dim3(256), 0, s, k);
+  DX_LAUNCH_CHECK();
   return DX_OK;
 }
 
@@ -856,43 +1160,69 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   const Plan p = make_plan(dtype, batch, m, n);
   if (workspace_bytes < p.bytes) return fail(DX_EWS, "dx_orthogonalize: workspace of %lld bytes, %lld needed", workspace_bytes, p.bytes);
   hipStream_t s = as_stream(stream);
-  if (small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32) <= kSmallLds) {
+  if (steps <= kSmallSteps && small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32) <= kSmallLds) {
     const int r32 = cdiv(p.r, 32) * 32, c32 = cdiv(p.c, 32) * 32;
-    const SmallArgs q{update, out, m, n, p.r, p.c, r32, c32, steps, m > n, a, b, c, eps};
+    SmallArgs q{update, out, m, n, p.r, p.c, r32, c32, steps, m > n, a, b, c, eps, {}};
+    Known known = known_at_start(b, c);
+    for (int i = 0; i <= steps; ++i, known = grown(known, a, b, c)) q.powers[i] = known;
     const int bytes = static_cast<int>(small_lds(r32, c32));
     if (dtype == DX_F32) return launch_small<float>(q, batch, bytes, s);
     if (dtype == DX_BF16) return launch_small<__bf16>(q, batch, bytes, s);
     return launch_small<_Float16>(q, batch, bytes, s);
   }
-  _Float16 *at = static_cast<_Float16 *>(workspace);
-  auto take = [&](long long halves) {
-    _Float16 *t = at;
-    at += halves * batch;
-    return t;
+  char *at = static_cast<char *>(workspace);
+  auto take = [&](auto *&to, long long count) {
+    to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(at);
+    at += count * static_cast<long long>(sizeof(*to));
   };
-  _Float16 *X = take(p.x), *XT0 = take(p.x), *XT1 = take(p.x), *A = take(p.sq), *B = take(p.sq);
-  double *partials = reinterpret_cast<double *>(at);
-  unsigned *arrivals = reinterpret_cast<unsigned *>(partials + static_cast<long long>(batch) * p.parts);
-  float *split = reinterpret_cast<float *>(arrivals + kSplitGroups);
-  const long long count = static_cast<long long>(m) * n;
-  if (dtype == DX_F32) hipLaunchKernelGGL(ns_norm_kernel<float>, dim3(p.parts, batch), dim3(256), 0, s, static_cast<const float *>(update), count, partials);
-  else if (dtype == DX_BF16) hipLaunchKernelGGL(ns_norm_kernel<__bf16>, dim3(p.parts, batch), dim3(256), 0, s, static_cast<const __bf16 *>(update), count, partials);
-  else hipLaunchKernelGGL(ns_norm_kernel<_Float16>, dim3(p.parts, batch), dim3(256), 0, s, static_cast<const _Float16 *>(update), count, partials);
-  DX_LAUNCH_CHECK();
+  Buffers w;
+  float *split, *row_most, *col_most;
+  double *sums;
+  unsigned *arrivals;
+  take(w.X, 2 * p.x * batch);
+  take(w.XT[0], 2 * p.x * batch);
+  take(w.XT[1], 2 * p.x * batch);
+  take(w.A, 2 * p.sq * batch);
+  take(w.M, 2 * p.sq * batch);
+  take(w.master_x, p.x * batch);
+  take(w.master_a, p.sq * batch);
+  take(split, p.split_floats);
+  take(sums, p.sums * batch);
+  take(w.exp_r, static_cast<long long>(p.rp) * batch);
+  take(w.exp_c, static_cast<long long>(p.cp) * batch);
+  take(arrivals, kSplitGroups);
+  take(row_most, static_cast<long long>(m) * p.scan.strips * batch);
+  take(col_most, static_cast<long long>(n) * p.scan.bands * batch);
   const bool tall = m > n;
-  const dim3 grid(cdiv(tall ? p.rp : p.cp, 64), cdiv(tall ? p.cp : p.rp, 64), batch);
-  _Float16 *same = tall ? XT0 : X, *turned = tall ? X : XT0;
-  const int ld_same = tall ? p.rp : p.cp, ld_turned = tall ? p.cp : p.rp;
-  if (dtype == DX_F32)
-    hipLaunchKernelGGL((ns_pack_kernel<float>), grid, dim3(256), 0, s, static_cast<const float *>(update), m, n, partials, p.parts, eps,
-                       same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
-  else if (dtype == DX_BF16)
-    hipLaunchKernelGGL((ns_pack_kernel<__bf16>), grid, dim3(256), 0, s, static_cast<const __bf16 *>(update), m, n, partials, p.parts, eps,
-                       same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
-  else
-    hipLaunchKernelGGL((ns_pack_kernel<_Float16>), grid, dim3(256), 0, s, static_cast<const _Float16 *>(update), m, n, partials, p.parts,
-                       eps, same, ld_same, turned, ld_turned, p.x, arrivals, kSplitGroups);
-  DX_LAUNCH_CHECK();
+  PackArgs k{};
+  k.in = update;
+  k.m = m;
+  k.n = n;
+  k.tall = tall;
+  k.bands = p.scan.bands;
+  k.strips = p.scan.strips;
+  k.sums = sums;
+  k.row_most = row_most;
+  k.col_most = col_most;
+  k.eps = eps;
+  k.same = tall ? w.XT[0] : w.X;
+  k.turned = tall ? w.X : w.XT[0];
+  k.ld_same = tall ? p.rp : p.cp;
+  k.ld_turned = tall ? p.cp : p.rp;
+  k.stride = 2 * p.x;
+  k.master = w.master_x;
+  k.master_stride = p.x;
+  k.rows_x = p.rp;
+  k.exp_row = tall ? w.exp_c : w.exp_r;
+  k.exp_col = tall ? w.exp_r : w.exp_c;
+  k.exp_row_stride = tall ? p.cp : p.rp;
+  k.exp_col_stride = tall ? p.rp : p.cp;
+  k.cap = known_at_start(b, c).cap;
+  k.arrivals = arrivals;
+  k.counts = kSplitGroups;
+  if (int rc = dtype == DX_F32 ? launch_start(static_cast<const float *>(update), p, batch, k, sums, row_most, col_most, s)
+               : dtype == DX_BF16 ? launch_start(static_cast<const __bf16 *>(update), p, batch, k, sums, row_most, col_most, s)
+                                  : launch_start(static_cast<const _Float16 *>(update), p, batch, k, sums, row_most, col_most, s)) return rc;
   NsArgs g{};
   g.arrivals = arrivals;
   g.partials = split;
@@ -905,5 +1235,5 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   g.r = p.r;
   g.cols = p.c;
   g.tall = tall;
-  return run_steps(p, batch, steps, g, X, XT0, XT1, A, B, s);
+  return run_steps(p, batch, steps, g, w, s);
 }

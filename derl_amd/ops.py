@@ -452,10 +452,11 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
   """Newton-Schulz orthogonalisation of (..., m, n) matrices: X = G / (|G|_F + eps), then ``steps`` times
   X <- a X + (b A + c A A) X with A = X X^T (of the shorter side).  The singular vectors stay, the singular
-  values approach 1.  float32, float16 or bfloat16, computed alike (22-bit operands, fp32 sums)
-  and rounded to the type once; contiguous; the result has update's type and shape.  ``out`` may be ``update``.  With eps > 0 a zero matrix gives
-  zeros; a matrix with a NaN or an infinity gives NaN.  Coefficients that let a singular value pass 8 on the way
-  leave fp16's range."""
+  values approach 1.  float32, float16 or bfloat16, computed alike (22-bit operands, fp32 sums and
+  copies) and rounded to the type once; every row and column keeps the digits its own size allows, however small it is
+  against the others.  Contiguous; the result has update's type and shape.  ``out`` may be ``update``.  With eps > 0 a
+  zero matrix gives zeros; a matrix with a NaN or an infinity gives NaN.  Coefficients that let a singular value pass
+  8, and what `a` alone makes of 1, leave fp16's range."""
   if not isinstance(update, torch.Tensor) or not update.is_cuda:
     raise ValueError("update must be a tensor on the GPU (derl_amd has no CPU path)")
   if update.dtype not in _ELEMENT_TYPES:

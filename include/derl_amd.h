@@ -247,8 +247,8 @@ int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pit
  *   X = G / (|G|_F + eps);  `steps` times: A = X X^T (of the shorter side), X <- a X + (b A + c A^2) X
  * and `out` = X in the same type (out may be update).  Products on the fp16 matrix cores: two fp16 terms per
  * operand and three products (22 bits), fp32 sums, whatever the type; rounded to it once, at the end.
- * Intermediate entries are held scaled: |X| < 16 and |b A + c A^2 + a| < 256 must hold, which any
- * coefficients whose iteration keeps singular values near 1 do.
+ * Rows and columns are scaled by powers of two of their own, so that each keeps the digits its size allows.
+ * A singular value may reach 8, or what `a` alone makes of 1, on the way.
  * dx_orthogonalize_workspace: bytes of `workspace` (256-byte aligned), negative DX_E* on bad shapes.
  * --------------------------------------------------------------------------------- */
 long long dx_orthogonalize_workspace(int dtype, int batch, int m, int n);

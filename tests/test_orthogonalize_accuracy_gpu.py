@@ -7,7 +7,7 @@ at most, as the nearest value to x is no further from x than round(want) is."""
 import pytest
 import torch
 
-from tests.test_tokens_gpu import BF16, DEV, F16, F32, gen, half_step, newton_schulz64
+from tests.test_tokens_gpu import A, B, BF16, C, DEV, F16, F32, gen, half_step, newton_schulz64
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,72 @@ def test_only_the_result_is_rounded(m, n, dtype):
     assert bool((off <= half_step(want, dtype) + 2 * d).all()), float((off - half_step(want, dtype)).max() / d)
     for edge in (off[-1], off[:, -1], off[-4:, -4:]):  # rows and columns that end inside a tile or a vector
       assert float(edge.norm()) <= float(half_step(want, dtype).max()) * edge.numel() ** 0.5 + 2 * d
+
+
+SCALED = [(17, 70), (32, 300), (60, 200), (200, 60), (93, 96), (64, 576), (256, 512), (512, 256), (300, 1203), (1203, 300), (701, 1410)]
+
+
+@pytest.mark.parametrize("scale", [1e-4, 1e-6, 1e-9])
+@pytest.mark.parametrize("m,n", SCALED)
+def test_rows_and_columns_of_any_size(m, n, scale):
+  """Every eighth row, every seventh column, or both, are far smaller than the rest (rare tokens, units that are nearly dead; the
+  iteration amplifies just those): each row and column is as accurate as its own size allows.  Relative errors of a row are those
+  of ``unit``: it starts, as all rows do, with growth of `a` a step for all of its parts."""
+  from derl_amd import ops
+  for which in ("rows", "columns", "both"):
+    g = torch.randn(m, n, generator=gen(m + n), device=DEV)
+    if which != "columns":
+      g[3::8] *= scale
+    if which != "rows":
+      g[:, 2::7] *= scale
+    got = ops.orthogonalize(g).double()
+    want, _ = newton_schulz64(g, 5)
+    off = got - want
+    bound = 2 * unit(max(m, n))
+    for dim in (0, 1):
+      worst = float((off.norm(dim=dim) / want.norm(dim=dim)).max())
+      assert worst <= bound, (which, dim, worst, bound)
+    if which == "both":
+      corner = float(off[3::8, 2::7].norm() / want[3::8, 2::7].norm())
+      assert corner <= bound, (corner, bound)
+
+
+@pytest.mark.parametrize("m,n", [(20, 90), (60, 60), (96, 90), (130, 600), (600, 130)])
+def test_a_norm_far_below_eps(m, n):
+  """X0 is close to 0: every step multiplies it by `a` (five steps of a product and a sum, X0's two roundings and the norm's:
+  14 half steps of an entry) and adds (b A + c A^2) X, whose entry (i, j) is off by ``unit`` / 5 of |M_i| |x_j| at most (the norms of
+  a row and a column), |M_i| <= (|b| + |c| s^2) s |x_i| with s the largest singular value; step k has |x|, |x_i|, s of a^k those of
+  X0 at most and its error is multiplied by `a` in the 4 - k steps behind it.  Twice that, as the errors of X move M as well."""
+  from derl_amd import ops
+  for norm in (1e-12, 1e-20, 1e-30):
+    g = torch.randn(m, n, generator=gen(m), device=DEV) * norm
+    got = ops.orthogonalize(g).double()
+    want, _ = newton_schulz64(g, 5)
+    x = g.double() / (g.double().norm() + 1e-7)
+    s = float(torch.linalg.matrix_norm(x, 2))
+    outer = x.norm(dim=1)[:, None] * x.norm(dim=0)[None]
+    moved = 2 * unit(max(m, n)) / 5 * (-B + C * s * s * A ** 8) * s * outer * sum(A ** (4 + 2 * k) for k in range(5))
+    assert bool(((got - want).abs() <= 14 * 2.0 ** -24 * want.abs() + moved).all()), norm
+
+
+@pytest.mark.parametrize("m,n", [(24, 90), (60, 64), (90, 96), (200, 800), (800, 200)])
+@pytest.mark.parametrize("coefficients,steps", [((3.0, 0.0, 0.0), 6), ((1.5, -0.5, 0.0), 12), ((2.0, -1.5, 0.5), 7), ((0.25, 0.0, 0.0), 5),
+                                                ((15 / 8, -10 / 8, 3 / 8), 9), ((-1.0, 0.5, 0.0), 4), ((1.0, 2.0, 0.0), 4)])
+def test_other_coefficients(m, n, coefficients, steps):
+  """Singular values that pass 8, shrink, change sign or converge.  A step's rounding is ``unit`` / 5 of the magnitudes of its
+  terms, |a| s + |b| s^3 + |c| s^5 for the largest singular value s, and what it moves is multiplied by the slope |a| + 3 |b| s^2
+  + 5 |c| s^4 at most in the steps behind it."""
+  from derl_amd import ops
+  g = torch.randn(m, n, generator=gen(5), device=DEV)
+  got = ops.orthogonalize(g, steps=steps, coefficients=coefficients).double()
+  a, b, c = coefficients
+  x = g.double() / g.double().norm()
+  s = torch.linalg.svdvals(x)
+  bound = 0.0
+  for _ in range(steps):
+    slope = abs(a) + 3 * abs(b) * s.max() ** 2 + 5 * abs(c) * s.max() ** 4
+    terms = (abs(a) * s + abs(b) * s ** 3 + abs(c) * s ** 5).norm()
+    bound = float(slope) * bound + unit(max(m, n)) / 5 * float(terms)
+    s = (a * s + b * s ** 3 + c * s ** 5).abs()
+  want, _ = newton_schulz64(g, steps, coefficients, eps=1e-7)
+  assert float((got - want).norm()) <= bound, (float((got - want).norm()), bound)
