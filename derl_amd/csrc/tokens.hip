@@ -146,7 +146,8 @@ __device__ __forceinline__ void store_chunk(char *row, char *at, int t, int firs
     if (first + k < V) reinterpret_cast<typename D::Store *>(row)[first + k] = D::put(x[k]);
 }
 
-// running statistics of a row (see the head of the file); `gap` = sum e (z - q), (mr, sr) those of the reference row q
+// running statistics of a row (see the head of the file); (mr, sr) those of the reference row q, and `gap` = sum e ((z - m) - (q - mr)):
+// two models' logits have no common zero, and of differences z - q the distance of the rows would leave only the last bits
 struct RowStats { float m, s, ed, gap, mr, sr; };
 
 __device__ __forceinline__ float wave_max_all(float v) {
@@ -155,7 +156,7 @@ __device__ __forceinline__ float wave_max_all(float v) {
   return v;
 }
 
-// e (z - q), where e = 0 (a banned column) counts as 0 whatever z - q is
+// e (z - q) of logits relative to their maxima, where e = 0 (a banned column) counts as 0 whatever z - q is
 __device__ __forceinline__ float gap_term(float e, float z, float q) { return e == 0.f ? 0.f : e * (z - q); }
 
 // raises the running maximum to at least x: the sums move to the new reference point.  Sums that vanish against the new
@@ -164,12 +165,13 @@ __device__ __forceinline__ void raise_max(RowStats &r, float x) {
   const float mn = fmaxf(r.m, x);
   const float d = r.m - mn, f = exp_of(d);
   r.ed = f == 0.f ? 0.f : f * (r.ed + r.s * d);
-  r.gap = f == 0.f ? 0.f : f * r.gap;
+  r.gap = f == 0.f ? 0.f : f * (r.gap + r.s * d);
   r.s *= f;
   r.m = mn;
 }
 __device__ __forceinline__ void raise_ref(RowStats &r, float x) {
   const float mn = fmaxf(r.mr, x);
+  r.gap += r.s == 0.f ? 0.f : r.s * (mn - r.mr);
   r.sr *= exp_of(r.mr - mn);
   r.mr = mn;
 }
@@ -192,8 +194,9 @@ __device__ __forceinline__ void add_vec(RowStats &r, const float (&x)[D::E], con
     r.s += e;
     r.ed += e * fmaxf(d, kLowest);  // e = 0 and d = -inf: 0
     if constexpr (REF) {
-      r.sr += exp_of(q[k] - r.mr);
-      r.gap += gap_term(e, x[k], q[k]);
+      const float dq = q[k] - r.mr;
+      r.sr += exp_of(dq);
+      r.gap += gap_term(e, d, dq);
     }
   }
 }
@@ -205,8 +208,9 @@ __device__ __forceinline__ void add_term(RowStats &r, float x, float q) {
   r.s += e;
   r.ed += e * fmaxf(d, kLowest);
   if constexpr (REF) {
-    r.sr += exp_of(q - r.mr);
-    r.gap += gap_term(e, x, q);
+    const float dq = q - r.mr;
+    r.sr += exp_of(dq);
+    r.gap += gap_term(e, d, dq);
   }
 }
 template <class D, bool REF>
@@ -295,13 +299,13 @@ __device__ __forceinline__ void write_columns(const char *z, const char *q, char
 template <bool REF>
 __device__ __forceinline__ void join_wave(RowStats &r) {
   raise_max(r, wave_max_all(r.m));
-  r.s = wave_sum_all(r.s);
-  r.ed = wave_sum_all(r.ed);
   if constexpr (REF) {
-    raise_ref(r, wave_max_all(r.mr));
+    raise_ref(r, wave_max_all(r.mr));  // (before r.s is another's too)
     r.sr = wave_sum_all(r.sr);
     r.gap = wave_sum_all(r.gap);
   }
+  r.s = wave_sum_all(r.s);
+  r.ed = wave_sum_all(r.ed);
 }
 constexpr RowStats kNothing = {kLowest, 0.f, 0.f, 0.f, kLowest, 0.f};
 
@@ -343,16 +347,16 @@ struct RowArgs {
 
 enum Mode { LOGP, STATS, POLICY };
 
-// what a row's gradient is made of: dz_j = p_j (c0 + c1 (z_j - m) + c2 (z_j - q_j)) + at 1{j = action}
-struct RowPlan { float m, inv_s, c0, c1, c2, at; };
+// what a row's gradient is made of: dz_j = p_j (c0 + c1 (z_j - m) + c2 ((z_j - m) - (q_j - mr))) + at 1{j = action}
+struct RowPlan { float m, inv_s, c0, c1, c2, at, mr; };
 
 template <class D, bool REF, bool ENT>
 __device__ __forceinline__ float grad_of(const RowPlan &g, float x, float y) {
   const float d = x - g.m, p = exp_of(d) * g.inv_s;
   float v = g.c0;
   if constexpr (ENT) v += g.c1 * fmaxf(d, kLowest);
-  if constexpr (REF) v = g.c2 != 0.f ? v + g.c2 * (x - y) : v;
-  return p == 0.f ? 0.f : p * v;  // (of a banned column x - y is infinite, and c1 d where |c1| > 1)
+  if constexpr (REF) v = g.c2 != 0.f ? v + g.c2 * (d - (y - g.mr)) : v;
+  return p == 0.f ? 0.f : p * v;  // (of a banned column d or y - mr is infinite, and c1 d where |c1| > 1)
 }
 
 struct RowTerms { float policy, entropy, kl, outside, ratio, lp; };
@@ -380,14 +384,14 @@ __device__ __forceinline__ RowPlan policy_row(const RowArgs &a, const RowStats &
     if (a.kl_coef != 0.f) g -= a.kl_coef * em;  // (0: the divergence, which may be infinite, is reported only)
   }
   if constexpr (REF) {
-    shift = (r.m - r.mr) + logf(r.s / r.sr);  // difference of the two log-normalisers
+    shift = logf(r.s / r.sr);  // difference of the two log-normalisers, beyond that of the maxima
     kl = r.gap / r.s - shift;
   }
   *terms = {policy, H, kl, outside ? 1.f : 0.f, ratio, lp};
   // dz_j = w [ g (1{j = a} - p_j) + c_H p_j (log p_j + H) + c_K p_j (log p_j - log q_j - KL) ]
   const float c1 = w * a.ent_coef, c2 = REF ? w * a.kl_coef : 0.f;
   const float c0 = w * (a.ent_coef * (H - log_s) - g);
-  return RowPlan{r.m, 1.f / r.s, c2 != 0.f ? c0 - c2 * (shift + kl) : c0, c1, c2, w * g};
+  return RowPlan{r.m, 1.f / r.s, c2 != 0.f ? c0 - c2 * (shift + kl) : c0, c1, c2, w * g, r.mr};
 }
 
 // this thread's share of the unmasked rows, thread `at` of `threads`: 16 bytes of the mask at a time, a bit for each that is not 0
@@ -732,7 +736,7 @@ __global__ __launch_bounds__(256) void token_short_kernel(const RowArgs a) {
     if (now.action < 0 || now.action >= a.V) za = __builtin_nanf("");
     RowTerms out = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if constexpr (MODE == POLICY) {
-      RowPlan g = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      RowPlan g = {};
       if (now.keep) g = policy_row<REF>(a, r, za, now.old, now.adv, now.ref, w, &out);
       char *dz = a.dz + row * a.dz_pitch;
 #pragma unroll
@@ -801,14 +805,14 @@ __device__ __forceinline__ RowStats join_pieces(const RowArgs &a, long long row)
     RowStats q = p;
     raise_max(q, r.m);
     raise_max(r, p.m);
-    r.s += q.s;
-    r.ed += q.ed;
     if constexpr (REF) {
       raise_ref(q, r.mr);
       raise_ref(r, p.mr);
       r.sr += q.sr;
       r.gap += q.gap;
     }
+    r.s += q.s;
+    r.ed += q.ed;
   }
   join_wave<REF>(r);
   return r;
@@ -843,7 +847,7 @@ __global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a)
   const long long row = blockIdx.y;
   const bool keep = !a.mask || a.mask[row];
   RowTerms out = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  RowPlan g = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  RowPlan g = {};
   long long action = -1;
   if (keep) {
     const float w = row_weight<4>(a);

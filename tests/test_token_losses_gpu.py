@@ -70,3 +70,19 @@ def test_second_derivatives_are_refused():
     for part in (grads, grads[:1], grads[-1:]):
       with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(sum(x.square().sum() for x in part), model.parameters(), retain_graph=True, allow_unused=True)
+
+
+@pytest.mark.parametrize("apart", [30.0, -3000.0, 30000.0])
+@pytest.mark.parametrize("rows,vocab", KERNELS)
+def test_exact_divergence_of_logits_at_a_distance(rows, vocab, apart):
+  """Logits are defined up to a constant, and two models' have no common one: the divergence and its gradient do not depend on it
+  (but for the rounding of the logits themselves, which the oracle reads as they are)."""
+  from derl_amd import ops
+  z, actions, old, adv, _, ref_z = policy_inputs(rows, vocab, F32, vocab)
+  for x, y in ((z, ref_z + apart), (z + apart, ref_z), (z + apart, ref_z - apart)):
+    _, _, _, lp = policy_oracle(x, actions, old, adv, 0.2, 0.0, 0.0, None, None, None)
+    drift = torch.where(adv > 0, -0.07, 0.07).double()
+    old = (lp - drift).float()
+    got = ops.token_policy_loss(x, actions, old, adv, 0.2, kl_coef=0.5, entropy_coef=0.01, ref_logits=y)
+    want = policy_oracle(x, actions, old, adv, 0.2, 0.5, 0.01, None, y, None)
+    check_policy(got, want, vocab, F32)
