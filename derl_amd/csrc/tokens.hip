@@ -356,7 +356,11 @@ __device__ __forceinline__ float grad_of(const RowPlan &g, float x, float y) {
   float v = g.c0;
   if constexpr (ENT) v += g.c1 * fmaxf(d, kLowest);
   if constexpr (REF) v = g.c2 != 0.f ? v + g.c2 * (d - (y - g.mr)) : v;
-  return p == 0.f ? 0.f : p * v;  // (of a banned column d or y - mr is infinite, and c1 d where |c1| > 1)
+  // of a banned column d or y - mr is infinite, and c1 d where |c1| > 1: 0 times anything is 0 here (v_mul_legacy_f32; a select
+  // instead cost 2 % of the policy loss of 8192 x 131072 bf16)
+  float product;
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(product) : "v"(p), "v"(v));
+  return product;
 }
 
 struct RowTerms { float policy, entropy, kl, outside, ratio, lp; };
