@@ -15,7 +15,7 @@ if os.environ.get("DERL_AMD_LIBRARY", "") == "diag":
   LIB_PATH = os.path.join(_PKG, "libderl_amd_diag.so")
 elif os.environ.get("DERL_AMD_LIBRARY", "").endswith(".so"):  # another build of the library (tools/: A/B on one box)
   LIB_PATH = os.path.join(_PKG, os.path.basename(os.environ["DERL_AMD_LIBRARY"]))
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 c_int, c_float, c_void_p, c_char_p = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p
 c_size_t, c_int64, c_uint64, c_double = ctypes.c_size_t, ctypes.c_int64, ctypes.c_uint64, ctypes.c_double
@@ -56,6 +56,9 @@ SIGNATURES = {
                              c_float, c_float, c_longlong, P, c_longlong, P, P, c_longlong, P, P],
     "dx_preference_loss": [P, c_int, c_longlong, c_int, c_longlong, P, P, c_int, P, P, c_float, c_float,
                            c_longlong, P, c_longlong, P, P, P, c_longlong, P, P],
+    "dx_token_policy_grad_scaled": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, P, P, c_longlong, P, c_float,
+                                    c_float, c_float, c_longlong, P, c_longlong, P, c_longlong, P, P],
+    "dx_preference_grad_scaled": [P, c_int, c_longlong, c_int, c_longlong, P, P, P, c_longlong, P, P],
     "dx_scale_rows": [P, c_int, c_longlong, c_int, c_longlong, P, P],
     "dx_orthogonalize_workspace": [c_int, c_int, c_int, c_int],
     "dx_orthogonalize": [P, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, c_float, P, P,

@@ -23,14 +23,15 @@ class _NoSecondDerivative(torch.autograd.Function):
 
 
 class _LogitsLoss(torch.autograd.Function):
-  """A scalar computed from logits together with its gradient.  The gradient is handed on once: it is scaled in
-  place by the incoming gradient (left alone where that is 1).  A second derivative (a gradient's penalty, a product
-  with the Hessian) raises."""
+  """A scalar computed from logits together with its gradient.  The gradient is handed on once, times the incoming
+  gradient: as it is where that is 1; 16-bit gradients are formed again otherwise, from the logits, so that they are
+  rounded once and a loss scale saves what rounding at scale 1 would lose; float32 ones are scaled in place.  A second
+  derivative (a gradient's penalty, a product with the Hessian) raises."""
 
   @staticmethod
   def forward(ctx, logits, evaluate):
-    terms, dlogits = evaluate(logits.detach())
-    ctx.save_for_backward(logits)
+    terms, dlogits, ctx.again, inputs = evaluate(logits.detach())
+    ctx.save_for_backward(logits, *inputs)
     ctx.dlogits = dlogits
     return terms[0].clone()
 
@@ -39,10 +40,15 @@ class _LogitsLoss(torch.autograd.Function):
     dlogits, ctx.dlogits = ctx.dlogits, None
     if dlogits is None:
       raise RuntimeError("the gradient of this loss was already handed on: evaluate the loss again to differentiate it again")
+    logits, *inputs = ctx.saved_tensors
     with torch.no_grad():
-      ops.scale_rows(dlogits, grad_output.to(torch.float32).contiguous())
+      factor = grad_output.to(torch.float32).contiguous()
+      if dlogits.dtype == torch.float32:
+        ops.scale_rows(dlogits, factor)
+      else:
+        ctx.again(dlogits, factor, logits.detach(), *inputs)
     if torch.is_grad_enabled():
-      dlogits = _NoSecondDerivative.apply(dlogits, *ctx.saved_tensors)
+      dlogits = _NoSecondDerivative.apply(dlogits, logits)
     return dlogits, None
 
 
@@ -72,6 +78,7 @@ class TokenLoss(Loss):
     return None if mask is None else self.to_device(mask, torch.bool).reshape(-1)
 
   def _evaluate(self, logits, data):
+    """(terms, dlogits, function (dlogits, factor, logits, *inputs) that forms the gradient again times a factor, inputs)."""
     raise NotImplementedError
 
   def _summaries(self, terms):
@@ -82,9 +89,9 @@ class TokenLoss(Loss):
     logits = self._logits(data)
 
     def evaluate(raw):
-      terms, dlogits, _ = self._evaluate(raw, data)
-      self.last_terms = terms
-      return terms, dlogits
+      found = self._evaluate(raw, data)
+      self.last_terms = found[0]
+      return found
 
     loss = _LogitsLoss.apply(logits, evaluate)
     if summary.should_record():
@@ -108,10 +115,17 @@ class TokenPolicyLoss(TokenLoss):
     ref_logits = data.get("ref_logits")
     if ref_logits is not None:
       ref_logits = self.to_device(ref_logits, logits.dtype).reshape(logits.shape)
-    return ops.token_policy_loss(
-        logits, self._flat(data, "actions", torch.int64), self._flat(data, "log_prob", f32),
-        self._flat(data, "advantages", f32), self.cliprange, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef,
-        ref_log_prob=self._flat(data, "ref_log_prob", f32, required=False), ref_logits=ref_logits, mask=self._mask(data))
+    given = dict(actions=self._flat(data, "actions", torch.int64), old_log_prob=self._flat(data, "log_prob", f32),
+                 advantages=self._flat(data, "advantages", f32), ref_log_prob=self._flat(data, "ref_log_prob", f32, required=False),
+                 ref_logits=ref_logits, mask=self._mask(data))
+    fixed = dict(cliprange=self.cliprange, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
+    terms, dlogits, _ = ops.token_policy_loss(logits, **given, **fixed)
+    names = [name for name, value in given.items() if value is not None]
+
+    def again(dlogits, factor, logits, *inputs):
+      ops.token_policy_grad_scaled(dlogits, factor, logits, **dict(zip(names, inputs)), **fixed)
+
+    return terms, dlogits, again, [given[name] for name in names]
 
 
 class PreferenceLoss(TokenLoss):
@@ -124,7 +138,8 @@ class PreferenceLoss(TokenLoss):
     self.beta, self.label_smoothing = beta, label_smoothing
 
   def _evaluate(self, logits, data):
-    return ops.preference_loss(
-        logits, self._flat(data, "actions", torch.int64), self._flat(data, "offsets", torch.int32),
-        self._flat(data, "ref_log_prob", torch.float32, required=False), self.beta,
-        label_smoothing=self.label_smoothing, mask=self._mask(data))
+    actions = self._flat(data, "actions", torch.int64)
+    terms, dlogits, _, row_stats = ops._preference_loss(  # pylint: disable=protected-access
+        logits, actions, self._flat(data, "offsets", torch.int32), self._flat(data, "ref_log_prob", torch.float32, required=False),
+        self.beta, self.label_smoothing, self._mask(data), 0)
+    return terms, dlogits, ops._preference_grad_scaled, [actions, row_stats]  # pylint: disable=protected-access

@@ -338,6 +338,7 @@ struct RowArgs {
   const double *count;  // unmasked rows, when `mask` is given; null: to be counted
   double batch;         // > 0: what the gradient is divided by, else the unmasked rows
   float cliprange, kl_coef, ent_coef;
+  const float *factor;  // null, or what the gradient is multiplied by before it is rounded; 1: it is there already, nothing is done
   double *partials;
   // rows cut into `splits` pieces of `piece` columns (a multiple of 2048)
   int splits, piece;
@@ -346,6 +347,8 @@ struct RowArgs {
 };
 
 enum Mode { LOGP, STATS, POLICY };
+
+__device__ __forceinline__ bool is_there(const float *factor) { return factor && *factor == 1.f; }
 
 // what a row's gradient is made of: dz_j = p_j (c0 + c1 (z_j - m) + c2 ((z_j - m) - (q_j - mr))) + at 1{j = action}
 struct RowPlan { float m, inv_s, c0, c1, c2, at, mr; };
@@ -434,7 +437,7 @@ __device__ __forceinline__ float row_weight(const RowArgs &a) {
   double n = static_cast<double>(a.rows);
   if (a.batch > 0) n = a.batch;
   else if (a.mask) n = a.count ? *a.count : count_rows<W>(a.mask, a.rows);
-  return static_cast<float>(1.0 / n);
+  return static_cast<float>(a.factor ? *a.factor / n : 1.0 / n);
 }
 
 template <class D>
@@ -455,6 +458,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const Row
   constexpr int E = D::E, N = NV ? NV : 1;
   __shared__ RowStats parts[2][kWaves];
   __shared__ double sums[kRows][8];
+  if (MODE == POLICY && is_there(a.factor)) return;
   const int t = threadIdx.x % T, slot = threadIdx.x / T, lane = threadIdx.x & 63;
   const float w = MODE == POLICY ? row_weight<T < 256 ? 4 : kWaves>(a) : 0.f;
   if (MODE == POLICY && t < 8) sums[slot][t] = 0.0;
@@ -623,7 +627,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void token_rows_kernel(const Row
       }
     }
     if (t < 64) {  // the first wave of the row: 64 rows' results at once
-      if (MODE != STATS && exists) a.lp[mine] = out.lp;
+      if (MODE != STATS && exists && a.lp) a.lp[mine] = out.lp;
       if (MODE == LOGP && exists && a.entropy) a.entropy[mine] = out.entropy;
       if (MODE == POLICY) {
         const float all[6] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp};
@@ -674,6 +678,7 @@ template <class D, int NV, Mode MODE, bool REF, bool ENT>
 __global__ __launch_bounds__(256) void token_short_kernel(const RowArgs a) {
   constexpr int E = D::E;
   __shared__ double sums[16][8];
+  if (MODE == POLICY && is_there(a.factor)) return;
   const int t = threadIdx.x & 15, slot = threadIdx.x >> 4;
   const float w = MODE == POLICY ? row_weight<4>(a) : 0.f;
   const long long step = gridDim.x * 16LL;
@@ -763,7 +768,7 @@ __global__ __launch_bounds__(256) void token_short_kernel(const RowArgs a) {
       out.entropy = now.keep ? log_s - r.ed / r.s : 0.f;
     }
     if (t == 0) {
-      if (MODE != STATS) a.lp[row] = out.lp;
+      if (MODE != STATS && a.lp) a.lp[row] = out.lp;
       if (MODE == LOGP && a.entropy) a.entropy[row] = out.entropy;
       if (MODE == STATS) a.stats[row] = now.keep ? make_float4(r.m, 1.f / r.s, out.lp, 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -787,7 +792,7 @@ template <class D, Mode MODE, bool REF>
 __global__ __launch_bounds__(256) void token_pieces_kernel(const RowArgs a) {
   __shared__ RowStats parts[2][4];
   const long long row = blockIdx.y;
-  if (a.mask && !a.mask[row]) return;
+  if ((a.mask && !a.mask[row]) || is_there(a.factor)) return;
   const int begin = blockIdx.x * a.piece, end = min(a.V, begin + a.piece);
   const char *z = a.z + row * a.z_pitch, *q = REF ? a.q + row * a.q_pitch : nullptr;
   RowStats r = kNothing;
@@ -848,6 +853,7 @@ __global__ __launch_bounds__(64) void token_join_kernel(const RowArgs a) {
 // a row writes its results
 template <class D, bool REF>
 __global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a) {
+  if (is_there(a.factor)) return;
   const long long row = blockIdx.y;
   const bool keep = !a.mask || a.mask[row];
   RowTerms out = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -860,7 +866,7 @@ __global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a)
     action = a.actions[row];
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    a.lp[row] = out.lp;
+    if (a.lp) a.lp[row] = out.lp;
     const double all[8] = {out.policy, out.entropy, out.kl, out.outside, out.ratio, out.lp, 0.0, 0.0};
     for (int k = 0; k < 8; ++k) a.partials[row * 8 + k] = all[k];
   }
@@ -871,7 +877,8 @@ __global__ __launch_bounds__(256) void token_pieces_grad_kernel(const RowArgs a)
                              [&](float x, float y, int col) { return grad_of<D, REF, true>(g, x, y) + (col == action ? g.at : 0.f); });
 }
 
-__global__ __launch_bounds__(1024) void mask_count_kernel(const uint8_t *mask, long long n, double *count) {
+__global__ __launch_bounds__(1024) void mask_count_kernel(const uint8_t *mask, long long n, double *count, const float *factor) {
+  if (is_there(factor)) return;
   const int c = count_rows<16>(mask, n);
   if (threadIdx.x == 0) *count = static_cast<double>(c);
 }
@@ -995,12 +1002,13 @@ __global__ __launch_bounds__(T) void preference_pairs_kernel(const PairArgs a) {
 }
 
 // dz_j = c (1{j = a} - p_j) of every row, c the coefficient of its sequence (0: no sequence's, or masked).  T threads take a
-// piece of a row; also the loss's terms, by the first workgroup.
+// piece of a row; also the loss's terms (loss_out), by the first workgroup.
 template <class D, int T>
 __global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, long long blocks, int pairs, int pair_groups, float *loss_out) {
   constexpr int kRows = 256 / T;
+  if (is_there(a.factor)) return;
   const int t = threadIdx.x % T, slot = threadIdx.x / T;
-  if (blockIdx.x == 0) {
+  if (loss_out && blockIdx.x == 0) {
     double s[8];
     sum_partials<256>(a.partials, pair_groups, s);
     if (threadIdx.x == 0) {
@@ -1017,7 +1025,7 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const RowArgs a, l
     const float4 st = a.stats[row];
     char *dz = a.dz + row * a.dz_pitch;
     const char *z = a.z + row * a.z_pitch;
-    const float c = st.w, k = -c * st.y;
+    const float c = a.factor ? st.w * *a.factor : st.w, k = -c * st.y;
     const long long action = c != 0.f ? a.actions[row] : -1;
     write_columns<D, T, false>(z, nullptr, dz, a.V, begin, end, t, c != 0.f,
                                [&](float x, float, int col) { return k * exp_of(x - st.x) + (col == action ? c : 0.f); });
@@ -1174,6 +1182,20 @@ int check_logits(const char *who, const void *logits, int dtype, long long rows,
   return DX_OK;
 }
 
+// the gradient of the preference loss from its rows' statistics
+int preference_grad(RowArgs a, int dtype, int pairs, int pair_groups, float *loss_out, hipStream_t s) {
+  // gradient: 16 lanes or a wave per short row, else a workgroup per piece of 32 KB of a row (the whole loss of 262144 rows, us with
+  // 64 / 16 lanes: 18 columns f32 204 / 160, 128 213 / 186, 250 255 / 301)
+  const long long bytes = static_cast<long long>(a.V) * elem_size(dtype);
+  const int T = bytes <= 512 ? 16 : bytes <= 4096 ? 64 : 256;
+  a.piece = T < 256 ? a.V : 32768 / elem_size(dtype);
+  a.splits = (a.V - 1) / a.piece + 1;
+  const long long blocks = (a.rows + 256 / T - 1) / (256 / T) * a.splits;
+  if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, blocks, pairs, pair_groups, loss_out, s);
+  if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
+  return launch_pref_grad<ElemF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
+}
+
 // workspace, in doubles: 8 for the count, 8 a workgroup for its sums, the pieces' statistics and their rows' chosen logits
 constexpr int kPartialsAt = 8, kPiecesAt = 8 + 8 * kMaxWorkers, kChosenAt = kPiecesAt + kMaxPieces * 3;
 static_assert(sizeof(RowStats) == 24 && kChosenAt + kMaxPieces / 4 == DX_TOKEN_WORKSPACE, "workspace");
@@ -1182,10 +1204,12 @@ RowArgs row_args(const void *logits, int dtype, long long rows, int vocab, long 
                  double *workspace) {
   RowArgs a{};
   a.splits = 1;
-  a.count = workspace;
-  a.partials = workspace + kPartialsAt;
-  a.piece_stats = reinterpret_cast<RowStats *>(workspace + kPiecesAt);
-  a.chosen = reinterpret_cast<float *>(workspace + kChosenAt);
+  if (workspace) {
+    a.count = workspace;
+    a.partials = workspace + kPartialsAt;
+    a.piece_stats = reinterpret_cast<RowStats *>(workspace + kPiecesAt);
+    a.chosen = reinterpret_cast<float *>(workspace + kChosenAt);
+  }
   const int size = elem_size(dtype);
   a.z = static_cast<const char *>(logits);
   a.z_pitch = pitch * size;
@@ -1227,22 +1251,25 @@ extern "C" int dx_sequence_log_prob(const float *token_log_prob, const int32_t *
   return DX_OK;
 }
 
-extern "C" int dx_token_policy_loss(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
-                                    const float *old_log_prob, const float *advantages, const float *ref_log_prob,
-                                    const void *ref_logits, long long ref_pitch, const uint8_t *mask, float cliprange, float kl_coef,
-                                    float entropy_coef, long long global_batch, void *dlogits, long long dlogits_pitch,
-                                    float *log_prob, double *workspace, long long workspace_count, float *loss_out, void *stream) {
-  DX_TRACE("dx_token_policy_loss");
-  if (int rc = check_logits("dx_token_policy_loss", logits, dtype, rows, vocab, pitch, actions)) return rc;
-  DX_REQUIRE(loss_out != nullptr && workspace != nullptr, "dx_token_policy_loss: null pointer");
-  DX_REQUIRE(rows == 0 || (old_log_prob && advantages && dlogits && log_prob), "dx_token_policy_loss: null pointer");
-  DX_REQUIRE(!(ref_log_prob && ref_logits), "dx_token_policy_loss: give ref_log_prob or ref_logits, not both");
-  DX_REQUIRE(rows <= 1 || dlogits_pitch >= vocab, "dx_token_policy_loss: rows of dlogits overlap");
-  DX_REQUIRE(!ref_logits || rows <= 1 || ref_pitch >= vocab, "dx_token_policy_loss: rows of ref_logits overlap");
+namespace {
+
+// the policy loss (loss_out), or its gradient alone times *factor
+int policy_loss(const char *who, const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
+                const float *old_log_prob, const float *advantages, const float *ref_log_prob, const void *ref_logits, long long ref_pitch,
+                const uint8_t *mask, float cliprange, float kl_coef, float entropy_coef, long long global_batch, void *dlogits,
+                long long dlogits_pitch, float *log_prob, double *workspace, long long workspace_count, const float *factor, float *loss_out,
+                void *stream) {
+  if (int rc = check_logits(who, logits, dtype, rows, vocab, pitch, actions)) return rc;
+  DX_REQUIRE((loss_out || factor) && workspace != nullptr, "%s: null pointer", who);
+  DX_REQUIRE(rows == 0 || (old_log_prob && advantages && dlogits && (log_prob || factor)), "%s: null pointer", who);
+  DX_REQUIRE(!(ref_log_prob && ref_logits), "%s: give ref_log_prob or ref_logits, not both", who);
+  DX_REQUIRE(rows <= 1 || dlogits_pitch >= vocab, "%s: rows of dlogits overlap", who);
+  DX_REQUIRE(!ref_logits || rows <= 1 || ref_pitch >= vocab, "%s: rows of ref_logits overlap", who);
   DX_REQUIRE(dx::aligned(dlogits, dtype == DX_F32 ? 4 : 2) && dx::aligned(ref_logits, dtype == DX_F32 ? 4 : 2),
-             "dx_token_policy_loss: dlogits / ref_logits are not aligned to their type");
+             "%s: dlogits / ref_logits are not aligned to their type", who);
+  DX_REQUIRE(!factor || rows == 0 || dlogits != logits, "%s: the logits are read again, dlogits must not be they", who);
   if (workspace_count < DX_TOKEN_WORKSPACE)
-    return dx::fail(DX_EWS, "dx_token_policy_loss: workspace of %lld doubles, %d needed", workspace_count, DX_TOKEN_WORKSPACE);
+    return dx::fail(DX_EWS, "%s: workspace of %lld doubles, %d needed", who, workspace_count, DX_TOKEN_WORKSPACE);
   hipStream_t s = dx::as_stream(stream);
   RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, mask, workspace);
   const int size = elem_size(dtype);
@@ -1258,19 +1285,47 @@ extern "C" int dx_token_policy_loss(const void *logits, int dtype, long long row
   a.cliprange = cliprange;
   a.kl_coef = kl_coef;
   a.ent_coef = entropy_coef;
+  a.factor = factor;
   if (rows <= kCountedHere) a.count = nullptr;
   else if (mask) {
-    hipLaunchKernelGGL(mask_count_kernel, dim3(1), dim3(1024), 0, s, mask, rows, workspace);
+    hipLaunchKernelGGL(mask_count_kernel, dim3(1), dim3(1024), 0, s, mask, rows, workspace, factor);
     DX_LAUNCH_CHECK();
   }
   int groups = 0;
   if (rows > 0)
     if (int rc = dtype == DX_F32 ? run_policy<ElemF32>(a, dtype, &groups, s)
                  : dtype == DX_BF16 ? run_policy<ElemBF16>(a, dtype, &groups, s) : run_policy<ElemF16>(a, dtype, &groups, s)) return rc;
+  if (!loss_out) return DX_OK;
   hipLaunchKernelGGL(policy_terms_kernel, dim3(1), dim3(1024), 0, s, a.partials, groups, mask, a.count, rows, kl_coef, entropy_coef,
                      loss_out);
   DX_LAUNCH_CHECK();
   return DX_OK;
+}
+
+}  // namespace
+
+extern "C" int dx_token_policy_loss(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
+                                    const float *old_log_prob, const float *advantages, const float *ref_log_prob,
+                                    const void *ref_logits, long long ref_pitch, const uint8_t *mask, float cliprange, float kl_coef,
+                                    float entropy_coef, long long global_batch, void *dlogits, long long dlogits_pitch,
+                                    float *log_prob, double *workspace, long long workspace_count, float *loss_out, void *stream) {
+  DX_TRACE("dx_token_policy_loss");
+  DX_REQUIRE(loss_out != nullptr, "dx_token_policy_loss: null pointer");
+  return policy_loss("dx_token_policy_loss", logits, dtype, rows, vocab, pitch, actions, old_log_prob, advantages, ref_log_prob, ref_logits,
+                     ref_pitch, mask, cliprange, kl_coef, entropy_coef, global_batch, dlogits, dlogits_pitch, log_prob, workspace,
+                     workspace_count, nullptr, loss_out, stream);
+}
+
+extern "C" int dx_token_policy_grad_scaled(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
+                                           const float *old_log_prob, const float *advantages, const float *ref_log_prob,
+                                           const void *ref_logits, long long ref_pitch, const uint8_t *mask, float cliprange, float kl_coef,
+                                           float entropy_coef, long long global_batch, void *dlogits, long long dlogits_pitch,
+                                           double *workspace, long long workspace_count, const float *factor, void *stream) {
+  DX_TRACE("dx_token_policy_grad_scaled");
+  DX_REQUIRE(factor != nullptr, "dx_token_policy_grad_scaled: null pointer");
+  return policy_loss("dx_token_policy_grad_scaled", logits, dtype, rows, vocab, pitch, actions, old_log_prob, advantages, ref_log_prob,
+                     ref_logits, ref_pitch, mask, cliprange, kl_coef, entropy_coef, global_batch, dlogits, dlogits_pitch, nullptr, workspace,
+                     workspace_count, factor, nullptr, stream);
 }
 
 extern "C" int dx_preference_loss(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
@@ -1301,16 +1356,24 @@ extern "C" int dx_preference_loss(const void *logits, int dtype, long long rows,
   if (long_sequences(rows, 2LL * pairs)) hipLaunchKernelGGL(preference_pairs_kernel<1024>, dim3(pair_groups), dim3(1024), 0, s, p);
   else hipLaunchKernelGGL(preference_pairs_kernel<256>, dim3(pair_groups), dim3(256), 0, s, p);
   DX_LAUNCH_CHECK();
-  // gradient: 16 lanes or a wave per short row, else a workgroup per piece of 32 KB of a row (the whole loss of 262144 rows, us with
-  // 64 / 16 lanes: 18 columns f32 204 / 160, 128 213 / 186, 250 255 / 301)
-  const long long bytes = static_cast<long long>(vocab) * elem_size(dtype);
-  const int T = bytes <= 512 ? 16 : bytes <= 4096 ? 64 : 256;
-  a.piece = T < 256 ? vocab : 32768 / elem_size(dtype);
-  a.splits = (vocab - 1) / a.piece + 1;
-  const long long blocks = (rows + 256 / T - 1) / (256 / T) * a.splits;
-  if (dtype == DX_F32) return launch_pref_grad<ElemF32>(a, T, blocks, pairs, pair_groups, loss_out, s);
-  if (dtype == DX_BF16) return launch_pref_grad<ElemBF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
-  return launch_pref_grad<ElemF16>(a, T, blocks, pairs, pair_groups, loss_out, s);
+  return preference_grad(a, dtype, pairs, pair_groups, loss_out, s);
+}
+
+extern "C" int dx_preference_grad_scaled(const void *logits, int dtype, long long rows, int vocab, long long pitch, const int64_t *actions,
+                                         const float *row_stats, void *dlogits, long long dlogits_pitch, const float *factor, void *stream) {
+  DX_TRACE("dx_preference_grad_scaled");
+  if (int rc = check_logits("dx_preference_grad_scaled", logits, dtype, rows, vocab, pitch, actions)) return rc;
+  if (rows == 0) return DX_OK;
+  DX_REQUIRE(row_stats && dlogits && factor, "dx_preference_grad_scaled: null pointer");
+  DX_REQUIRE(rows <= 1 || dlogits_pitch >= vocab, "dx_preference_grad_scaled: rows of dlogits overlap");
+  DX_REQUIRE(dx::aligned(dlogits, dtype == DX_F32 ? 4 : 2) && dx::aligned(row_stats, 16), "dx_preference_grad_scaled: misaligned dlogits / row_stats");
+  DX_REQUIRE(dlogits != logits, "dx_preference_grad_scaled: the logits are read again, dlogits must not be they");
+  RowArgs a = row_args(logits, dtype, rows, vocab, pitch, actions, nullptr, nullptr);
+  a.stats = reinterpret_cast<float4 *>(const_cast<float *>(row_stats));  // (read only)
+  a.dz = static_cast<char *>(dlogits);
+  a.dz_pitch = dlogits_pitch * elem_size(dtype);
+  a.factor = factor;
+  return preference_grad(a, dtype, 0, 0, nullptr, dx::as_stream(stream));
 }
 
 extern "C" int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pitch, const float *factor, void *stream) {

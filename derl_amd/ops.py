@@ -297,12 +297,12 @@ def _span(t):
   return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _gradient_buffer(dlogits_out, logits, *others):
-  """The tensor the gradient goes to: new, the caller's, or ``logits`` itself (in place)."""
+def _gradient_buffer(dlogits_out, logits, *others, in_place=True):
+  """The tensor the gradient goes to: new, the caller's, or (``in_place``) ``logits`` itself."""
   if dlogits_out is None:
     return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
   _rows_of(dlogits_out, "dlogits_out", like=logits)
-  same = dlogits_out.data_ptr() == logits.data_ptr() and (logits.shape[0] <= 1 or dlogits_out.stride(0) == logits.stride(0))
+  same = in_place and dlogits_out.data_ptr() == logits.data_ptr() and (logits.shape[0] <= 1 or dlogits_out.stride(0) == logits.stride(0))
   begin, end = _span(dlogits_out)
   for other in others + (() if same else (logits,)):
     if other is not None:
@@ -368,6 +368,21 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
   Returns (loss float32 (8,), dlogits (N, V), log_prob float32 (N,)); loss = {loss, policy loss, entropy, KL,
   share of ratios outside the range, mean ratio, mean log-probability, unmasked rows}.  ``dlogits_out`` may
   be ``logits``.  Masked rows have gradient and log_prob 0; without an unmasked row the loss is 0."""
+  rows, vocab, _ = _rows_of(logits, "logits")
+  dev = logits.device
+  given = _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask,
+                            global_batch)
+  dlogits = _gradient_buffer(dlogits_out, logits, ref_logits)
+  log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
+  loss_out = torch.empty(8, dtype=torch.float32, device=dev)
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
+  _call_on(dev, "dx_token_policy_loss", *given, dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, log_prob.data_ptr(),
+           workspace.data_ptr(), workspace.numel(), loss_out.data_ptr(), _lib.stream_ptr(dev))
+  return loss_out, dlogits, log_prob
+
+
+def _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask, global_batch):
+  """The checked inputs of the native policy loss, in its order."""
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
   if ref_log_prob is not None and ref_logits is not None:
@@ -379,20 +394,33 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
   ref_pitch = vocab
   if ref_logits is not None:
     _, _, ref_pitch = _rows_of(ref_logits, "ref_logits", like=logits)
-  act = _vector(actions, "actions", rows, dev, _INDEX)
-  old = _vector(old_log_prob, "old_log_prob", rows, dev, _FLOAT)
-  adv = _vector(advantages, "advantages", rows, dev, _FLOAT)
-  ref = _vector(ref_log_prob, "ref_log_prob", rows, dev, _FLOAT)
-  keep = _vector(mask, "mask", rows, dev, _FLAG)
-  dlogits = _gradient_buffer(dlogits_out, logits, ref_logits)
-  log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
-  loss_out = torch.empty(8, dtype=torch.float32, device=dev)
+  return (logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, _vector(actions, "actions", rows, dev, _INDEX),
+          _vector(old_log_prob, "old_log_prob", rows, dev, _FLOAT), _vector(advantages, "advantages", rows, dev, _FLOAT),
+          _vector(ref_log_prob, "ref_log_prob", rows, dev, _FLOAT), None if ref_logits is None else ref_logits.data_ptr(), ref_pitch,
+          _vector(mask, "mask", rows, dev, _FLAG), -1.0 if cliprange is None else float(cliprange), float(kl_coef), float(entropy_coef),
+          int(global_batch))
+
+
+def _factor(factor, device):
+  _dev(factor, "factor", torch.float32)
+  if factor.numel() != 1 or factor.device != device:
+    raise ValueError(f"factor must be one float32 on {device}, got {tuple(factor.shape)} on {factor.device}")
+  return factor.data_ptr()
+
+
+def token_policy_grad_scaled(dlogits, factor, logits, actions, old_log_prob, advantages, cliprange, kl_coef=0., entropy_coef=0.,
+                             ref_log_prob=None, ref_logits=None, mask=None, global_batch=0):
+  """``dlogits``, the gradient that ``token_policy_loss`` gave for these arguments, becomes ``factor`` (float32 device scalar)
+  times the gradient, multiplied before it is rounded: formed again from the logits, left alone where the factor is 1."""
+  rows, vocab, _ = _rows_of(logits, "logits")
+  dev = logits.device
+  given = _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask,
+                            global_batch)
+  _gradient_buffer(dlogits, logits, ref_logits, in_place=False)
   workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
-  _call_on(dev, "dx_token_policy_loss", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, old, adv, ref,
-           None if ref_logits is None else ref_logits.data_ptr(), ref_pitch, keep, -1.0 if cliprange is None else float(cliprange), float(kl_coef),
-           float(entropy_coef), int(global_batch), dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab,
-           log_prob.data_ptr(), workspace.data_ptr(), workspace.numel(), loss_out.data_ptr(), _lib.stream_ptr(dev))
-  return loss_out, dlogits, log_prob
+  _call_on(dev, "dx_token_policy_grad_scaled", *given, dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, workspace.data_ptr(),
+           workspace.numel(), _factor(factor, dev), _lib.stream_ptr(dev))
+  return dlogits
 
 
 def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothing=0., mask=None, global_pairs=0,
@@ -409,6 +437,11 @@ def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothin
   Returns (loss float32 (8,), dlogits (N, V), sequence log-probabilities float32 (2 P,)); loss = {loss, share of
   pairs with h > 0, h, beta (chosen - ref), beta (rejected - ref), chosen, rejected, P}.  Rows that are masked
   or belong to no sequence have gradient 0.  ``dlogits_out`` may be ``logits``."""
+  return _preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothing, mask, global_pairs, dlogits_out)[:3]
+
+
+def _preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothing, mask, global_pairs, dlogits_out=None):
+  """``preference_loss`` and the rows' statistics behind its gradient."""
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
   sequences = _check_offsets(offsets, dev)
@@ -424,22 +457,33 @@ def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothin
   dlogits = _gradient_buffer(dlogits_out, logits)
   sequence = torch.empty(sequences, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
-  # the library's scratch and behind it four floats a row
-  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE + 2 * rows, dtype=torch.float64, device=dev)
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
+  row_stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
   _call_on(dev, "dx_preference_loss", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act,
            offsets.data_ptr(), sequences // 2, ref, keep, float(beta), float(label_smoothing), int(global_pairs),
-           dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, sequence.data_ptr(),
-           workspace.data_ptr() + 8 * _lib.DX_TOKEN_WORKSPACE, workspace.data_ptr(), _lib.DX_TOKEN_WORKSPACE, loss_out.data_ptr(), _lib.stream_ptr(dev))
-  return loss_out, dlogits, sequence
+           dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, sequence.data_ptr(), row_stats.data_ptr(),
+           workspace.data_ptr(), workspace.numel(), loss_out.data_ptr(), _lib.stream_ptr(dev))
+  return loss_out, dlogits, sequence, row_stats
+
+
+def _preference_grad_scaled(dlogits, factor, logits, actions, row_stats):
+  """As ``token_policy_grad_scaled``, from the statistics that ``_preference_loss`` gave."""
+  rows, vocab, pitch = _rows_of(logits, "logits")
+  dev = logits.device
+  _gradient_buffer(dlogits, logits, in_place=False)
+  _dev(row_stats, "row_stats", torch.float32)
+  if row_stats.shape != (rows, 4) or row_stats.device != dev:
+    raise ValueError(f"row_stats must be ({rows}, 4) on {dev}, got {tuple(row_stats.shape)} on {row_stats.device}")
+  _call_on(dev, "dx_preference_grad_scaled", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch,
+           _vector(actions, "actions", rows, dev, _INDEX), row_stats.data_ptr(), dlogits.data_ptr(),
+           dlogits.stride(0) if rows > 1 else vocab, _factor(factor, dev), _lib.stream_ptr(dev))
+  return dlogits
 
 
 def scale_rows(x, factor):
   """x *= factor in place, ``factor`` a float32 device scalar; nothing but the factor is read when it is 1."""
   rows, columns, pitch = _rows_of(x, "x")
-  _dev(factor, "factor", torch.float32)
-  if factor.numel() != 1 or factor.device != x.device:
-    raise ValueError(f"factor must be one float32 on {x.device}, got {tuple(factor.shape)} on {factor.device}")
-  _call_on(x.device, "dx_scale_rows", x.data_ptr(), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, factor.data_ptr(),
+  _call_on(x.device, "dx_scale_rows", x.data_ptr(), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, _factor(factor, x.device),
            _lib.stream_ptr(x.device))
   return x
 

@@ -40,7 +40,7 @@ extern "C" {
 #define DX_EWS (-4)      /* workspace too small                                     */
 #define DX_ETIMEOUT (-5) /* a persistent kernel's grid barrier gave up (dx_mlp_ppo_epoch) */
 
-#define DX_ABI_VERSION 7
+#define DX_ABI_VERSION 8
 
 int dx_abi_version(void);
 /* The DX_* environment switches ("Diagnostic switches") are parsed when a call first needs them and cached.
@@ -213,6 +213,10 @@ int dx_reward_summary_f32(const float *rewards, const uint8_t *resets, int T, in
  *        sequence have gradient 0.  row_stats: scratch of 4 floats per row, 16-byte aligned.
  *        loss_out[8] = {loss, share with h > 0, h, beta (chosen - ref), beta (rejected - ref), chosen,
  *        rejected, pairs}.  global_pairs > 0 divides the gradient instead of pairs.
+ *   token_policy_grad_scaled, preference_grad_scaled : the gradient of the loss again, times *factor (device scalar)
+ *        BEFORE it is rounded to dtype: what a loss scale is for, as a gradient of f16 that was rounded at scale 1 has
+ *        lost what lies below 6e-8.  The arguments of the loss call, dlogits the gradient it wrote (not the logits,
+ *        which are read again), row_stats as preference_loss left it.  *factor 1: nothing is done.
  *   scale_rows : x *= *factor (device scalar) in place; reads nothing but the factor when it is 1.
  * `workspace`: scratch of DX_TOKEN_WORKSPACE doubles.  Sums of a row in fp32, over rows in fp64, every
  * result independent of timing (no atomics).
@@ -239,6 +243,17 @@ int dx_preference_loss(const void *logits, int dtype, long long rows, int vocab,
                        float label_smoothing, long long global_pairs, void *dlogits,
                        long long dlogits_pitch, float *sequence_log_prob, float *row_stats,
                        double *workspace, long long workspace_count, float *loss_out, void *stream);
+int dx_token_policy_grad_scaled(const void *logits, int dtype, long long rows, int vocab,
+                                long long pitch, const int64_t *actions, const float *old_log_prob,
+                                const float *advantages, const float *ref_log_prob,
+                                const void *ref_logits, long long ref_pitch, const uint8_t *mask,
+                                float cliprange, float kl_coef, float entropy_coef,
+                                long long global_batch, void *dlogits, long long dlogits_pitch,
+                                double *workspace, long long workspace_count, const float *factor,
+                                void *stream);
+int dx_preference_grad_scaled(const void *logits, int dtype, long long rows, int vocab, long long pitch,
+                              const int64_t *actions, const float *row_stats, void *dlogits,
+                              long long dlogits_pitch, const float *factor, void *stream);
 int dx_scale_rows(void *x, int dtype, long long rows, int columns, long long pitch,
                   const float *factor, void *stream);
 

@@ -3,7 +3,8 @@ count.  Oracles and tolerances are those of tests/test_tokens_gpu.py."""
 import pytest
 import torch
 
-from tests.test_tokens_gpu import BF16, DEV, F16, F32, INF, check_policy, policy_inputs, policy_oracle
+from tests.test_tokens_gpu import (BF16, DEV, F16, F32, INF, check_policy, gen, half_step, policy_inputs, policy_oracle,
+                                   preference_oracle, slack, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,73 @@ def test_exact_divergence_of_logits_at_a_distance(rows, vocab, apart):
     got = ops.token_policy_loss(x, actions, old, adv, 0.2, kl_coef=0.5, entropy_coef=0.01, ref_logits=y)
     want = policy_oracle(x, actions, old, adv, 0.2, 0.5, 0.01, None, y, None)
     check_policy(got, want, vocab, F32)
+
+
+class Table(torch.nn.Module):
+  """Logits that are parameters themselves: their gradient is what the loss hands on."""
+
+  def __init__(self, logits):
+    super().__init__()
+    self.logits = torch.nn.Parameter(logits)
+
+  def forward(self, observations):
+    return self.logits
+
+
+@pytest.mark.parametrize("factor", [1.0, 3.0, 4096.0])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,vocab", KERNELS + [(17000, 40)])
+def test_a_scaled_loss_is_rounded_once(rows, vocab, dtype, factor):
+  """loss * factor: the gradient is the factor's multiple in 64 bits, rounded once, also where at scale 1 it would have been
+  below f16's smallest step; the same for the preference loss; a graph of both gives the same bits."""
+  import derl_amd as derl
+  z, actions, old, adv, _, ref_z = policy_inputs(rows, vocab, dtype, 5 * vocab)
+  mask = torch.rand(rows, generator=gen(vocab), device=DEV) < 0.7
+  mask[0] = True
+  model = Table(z.clone())
+  policy = derl.TokenPolicyLoss(model, cliprange=0.2, kl_coef=0.1, entropy_coef=0.01)
+  data = dict(observations=None, actions=actions, log_prob=old, advantages=adv, ref_logits=ref_z, mask=mask)
+  offsets = torch.tensor([0, rows // 3, rows - 1], dtype=torch.int32, device=DEV)
+  preference = derl.PreferenceLoss(model, beta=0.3, label_smoothing=0.1)
+  pair = dict(observations=None, actions=actions, offsets=offsets, mask=mask)
+  s = slack(vocab)
+  _, dz, size, _ = policy_oracle(z, actions, old, adv, 0.2, 0.1, 0.01, None, ref_z, mask)
+  (policy(data) * factor).backward()
+  within(model.logits.grad, factor * dz, 8 * s * factor * size + half_step(factor * dz, dtype), "policy")
+  want, model.logits.grad = model.logits.grad, None
+  _, dz, size, _ = preference_oracle(z, actions, offsets, None, 0.3, 0.1, mask)
+  size = (8 * s + 4 * 0.3 * rows * (s + 2.0 ** -23 * 40)) * size
+  (preference(pair) * factor).backward()
+  within(model.logits.grad, factor * dz, factor * size + half_step(factor * dz, dtype), "preference")
+  want2, model.logits.grad = model.logits.grad, None
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    (a,) = torch.autograd.grad(policy(data) * factor, model.logits)
+    (b,) = torch.autograd.grad(preference(pair) * factor, model.logits)
+  for _ in range(3):
+    graph.replay()
+    policy(data)
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want2)
+
+
+def test_what_the_scaled_gradient_depends_on_is_kept():
+  """An input that is changed in place between the loss and its gradient is found out, as autograd does for its own."""
+  import derl_amd as derl
+  z, actions, old, adv, _, _ = policy_inputs(6, 300, F16, 1)
+  model = Table(z)
+  loss = derl.TokenPolicyLoss(model)(dict(observations=None, actions=actions, log_prob=old, advantages=adv))
+  adv.mul_(2.0)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    (loss * 8.0).backward()
+
+
+def test_refusals_of_the_scaled_gradients():
+  from derl_amd import ops
+  z, actions, old, adv, _, _ = policy_inputs(6, 40, F16, 1)
+  one = torch.ones(1, device=DEV)
+  _, dz, _ = ops.token_policy_loss(z, actions, old, adv, 0.2)
+  for bad in (dict(dlogits=z), dict(dlogits=dz[:5]), dict(dlogits=dz.float()), dict(factor=one.double()), dict(factor=one.cpu()),
+              dict(factor=torch.ones(2, device=DEV)), dict(cliprange=-1.0), dict(actions=actions[:3])):
+    with pytest.raises(ValueError):
+      ops.token_policy_grad_scaled(**{**dict(dlogits=dz, factor=one, logits=z, actions=actions, old_log_prob=old, advantages=adv, cliprange=0.2), **bad})
