@@ -139,7 +139,7 @@ class PreferenceLoss(TokenLoss):
 
   def _evaluate(self, logits, data):
     actions = self._flat(data, "actions", torch.int64)
-    terms, dlogits, _, row_stats = ops._preference_loss(  # pylint: disable=protected-access
+    terms, dlogits, _, workspace = ops._preference_loss(  # pylint: disable=protected-access
         logits, actions, self._flat(data, "offsets", torch.int32), self._flat(data, "ref_log_prob", torch.float32, required=False),
         self.beta, self.label_smoothing, self._mask(data), 0)
-    return terms, dlogits, ops._preference_grad_scaled, [actions, row_stats]  # pylint: disable=protected-access
+    return terms, dlogits, ops._preference_grad_scaled, [actions, workspace]  # pylint: disable=protected-access

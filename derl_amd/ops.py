@@ -368,10 +368,9 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
   Returns (loss float32 (8,), dlogits (N, V), log_prob float32 (N,)); loss = {loss, policy loss, entropy, KL,
   share of ratios outside the range, mean ratio, mean log-probability, unmasked rows}.  ``dlogits_out`` may
   be ``logits``.  Masked rows have gradient and log_prob 0; without an unmasked row the loss is 0."""
-  rows, vocab, _ = _rows_of(logits, "logits")
-  dev = logits.device
   given = _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask,
                             global_batch)
+  dev, rows, vocab = logits.device, given[2], given[3]
   dlogits = _gradient_buffer(dlogits_out, logits, ref_logits)
   log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
@@ -412,10 +411,9 @@ def token_policy_grad_scaled(dlogits, factor, logits, actions, old_log_prob, adv
                              ref_log_prob=None, ref_logits=None, mask=None, global_batch=0):
   """``dlogits``, the gradient that ``token_policy_loss`` gave for these arguments, becomes ``factor`` (float32 device scalar)
   times the gradient, multiplied before it is rounded: formed again from the logits, left alone where the factor is 1."""
-  rows, vocab, _ = _rows_of(logits, "logits")
-  dev = logits.device
   given = _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask,
                             global_batch)
+  dev, rows, vocab = logits.device, given[2], given[3]
   _gradient_buffer(dlogits, logits, ref_logits, in_place=False)
   workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
   _call_on(dev, "dx_token_policy_grad_scaled", *given, dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, workspace.data_ptr(),
@@ -441,7 +439,7 @@ def preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothin
 
 
 def _preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothing, mask, global_pairs, dlogits_out=None):
-  """``preference_loss`` and the rows' statistics behind its gradient."""
+  """``preference_loss`` and its workspace, with the rows' statistics that its gradient is made of."""
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
   sequences = _check_offsets(offsets, dev)
@@ -457,25 +455,24 @@ def _preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothi
   dlogits = _gradient_buffer(dlogits_out, logits)
   sequence = torch.empty(sequences, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
-  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
-  row_stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
+  # the library's scratch and behind it four floats a row
+  workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE + 2 * rows, dtype=torch.float64, device=dev)
   _call_on(dev, "dx_preference_loss", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act,
            offsets.data_ptr(), sequences // 2, ref, keep, float(beta), float(label_smoothing), int(global_pairs),
-           dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, sequence.data_ptr(), row_stats.data_ptr(),
-           workspace.data_ptr(), workspace.numel(), loss_out.data_ptr(), _lib.stream_ptr(dev))
-  return loss_out, dlogits, sequence, row_stats
+           dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, sequence.data_ptr(),
+           workspace.data_ptr() + 8 * _lib.DX_TOKEN_WORKSPACE, workspace.data_ptr(), _lib.DX_TOKEN_WORKSPACE, loss_out.data_ptr(),
+           _lib.stream_ptr(dev))
+  return loss_out, dlogits, sequence, workspace
 
 
-def _preference_grad_scaled(dlogits, factor, logits, actions, row_stats):
-  """As ``token_policy_grad_scaled``, from the statistics that ``_preference_loss`` gave."""
+def _preference_grad_scaled(dlogits, factor, logits, actions, workspace):
+  """As ``token_policy_grad_scaled``, from the workspace that ``_preference_loss`` gave."""
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
   _gradient_buffer(dlogits, logits, in_place=False)
-  _dev(row_stats, "row_stats", torch.float32)
-  if row_stats.shape != (rows, 4) or row_stats.device != dev:
-    raise ValueError(f"row_stats must be ({rows}, 4) on {dev}, got {tuple(row_stats.shape)} on {row_stats.device}")
+  _vector(workspace, "workspace", _lib.DX_TOKEN_WORKSPACE + 2 * rows, dev, (torch.float64,))
   _call_on(dev, "dx_preference_grad_scaled", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch,
-           _vector(actions, "actions", rows, dev, _INDEX), row_stats.data_ptr(), dlogits.data_ptr(),
+           _vector(actions, "actions", rows, dev, _INDEX), workspace.data_ptr() + 8 * _lib.DX_TOKEN_WORKSPACE, dlogits.data_ptr(),
            dlogits.stride(0) if rows > 1 else vocab, _factor(factor, dev), _lib.stream_ptr(dev))
   return dlogits
 
