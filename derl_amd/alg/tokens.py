@@ -103,16 +103,28 @@ class TokenLoss(Loss):
 class TokenPolicyLoss(TokenLoss):
   """Clipped policy loss with a KL term and an entropy bonus (``ops.token_policy_loss``).  ``data``: observations,
   actions, log_prob (of the policy that acted), advantages; optional ref_log_prob or ref_logits (of the reference
-  policy), mask."""
+  policy), mask.  Reference logits of a wider type than the policy's are not rounded to it: the loss is then taken of
+  the policy's logits in the type that holds both (the gradient is rounded to theirs on its way back)."""
   tags = ("loss", "policy_loss", "entropy", "kl", "clip_fraction", "ratio", "log_prob", "tokens")
 
   def __init__(self, model, cliprange=0.2, kl_coef=0., entropy_coef=0., name=None):
     super().__init__(model, name=name)
     self.cliprange, self.kl_coef, self.entropy_coef = cliprange, kl_coef, entropy_coef
 
+  def _ref_logits(self, data):
+    ref_logits = data.get("ref_logits")
+    if ref_logits is None:
+      return None
+    ref_logits = torch.as_tensor(ref_logits)
+    return ref_logits if ref_logits.dtype in (torch.bfloat16, torch.float16) else ref_logits.float()
+
+  def _logits(self, data):
+    logits, ref_logits = super()._logits(data), self._ref_logits(data)
+    return logits if ref_logits is None else logits.to(torch.promote_types(logits.dtype, ref_logits.dtype))
+
   def _evaluate(self, logits, data):
     f32 = torch.float32
-    ref_logits = data.get("ref_logits")
+    ref_logits = self._ref_logits(data)
     if ref_logits is not None:
       ref_logits = self.to_device(ref_logits, logits.dtype).reshape(logits.shape)
     given = dict(actions=self._flat(data, "actions", torch.int64), old_log_prob=self._flat(data, "log_prob", f32),

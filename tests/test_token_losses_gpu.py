@@ -157,3 +157,22 @@ def test_refusals_of_the_scaled_gradients():
               dict(factor=torch.ones(2, device=DEV)), dict(cliprange=-1.0), dict(actions=actions[:3])):
     with pytest.raises(ValueError):
       ops.token_policy_grad_scaled(**{**dict(dlogits=dz, factor=one, logits=z, actions=actions, old_log_prob=old, advantages=adv, cliprange=0.2), **bad})
+
+
+@pytest.mark.parametrize("dtype,ref_dtype", [(BF16, F32), (F16, F32), (BF16, F16), (F16, BF16), (F32, BF16), (F16, torch.float64)])
+def test_reference_logits_of_another_type_are_not_rounded(dtype, ref_dtype):
+  """The divergence is that of the logits as they are given (float64 ones rounded to float32, once)."""
+  import derl_amd as derl
+  rows, vocab = 5, 700
+  z, actions, old, adv, _, _ = policy_inputs(rows, vocab, dtype, 1)
+  ref_z = (z.float() + 0.3 * torch.randn(z.shape, generator=gen(5), device=DEV)).to(ref_dtype)
+  model = Table(z)
+  for given in (ref_z, ref_z.cpu().numpy() if ref_dtype is not BF16 else ref_z.cpu()):
+    loss_fn = derl.TokenPolicyLoss(model, cliprange=0.2, kl_coef=0.7)
+    model.logits.grad = None
+    loss_fn(dict(observations=None, actions=actions, log_prob=old, advantages=adv, ref_logits=given)).backward()
+    terms, dz, size, _ = policy_oracle(z, actions, old, adv, 0.2, 0.7, 0.0, None, ref_z, None)
+    s = slack(vocab)
+    assert model.logits.grad.dtype == dtype
+    within(model.logits.grad, dz, 8 * s * size + half_step(dz, dtype), "dlogits")
+    assert abs(float(loss_fn.last_terms[3]) - terms[3]) <= 16 * s * (1 + abs(terms[3]))
