@@ -297,6 +297,16 @@ def _span(t):
   return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _writable(t, name):
+  """A tensor of the caller's that a kernel overwrites: as torch's own operations in place, autograd learns of it (a backward
+  pass that has kept the old values raises), and a leaf that requires grad is refused."""
+  if t.requires_grad and t.is_leaf and torch.is_grad_enabled():
+    raise ValueError(f"{name} is a leaf that requires grad: it cannot be written in place")
+  if not t.is_inference():
+    torch.autograd.graph.increment_version(t)
+  return t
+
+
 def _gradient_buffer(dlogits_out, logits, *others, in_place=True):
   """The tensor the gradient goes to: new, the caller's, or (``in_place``) ``logits`` itself."""
   if dlogits_out is None:
@@ -309,7 +319,7 @@ def _gradient_buffer(dlogits_out, logits, *others, in_place=True):
       b, e = _span(other)
       if b < end and begin < e:
         raise ValueError("dlogits_out overlaps an input (it may only be logits itself)")
-  return dlogits_out
+  return _writable(dlogits_out, "dlogits_out")
 
 
 def token_log_prob(logits, actions, mask=None):
@@ -480,8 +490,9 @@ def _preference_grad_scaled(dlogits, factor, logits, actions, workspace):
 def scale_rows(x, factor):
   """x *= factor in place, ``factor`` a float32 device scalar; nothing but the factor is read when it is 1."""
   rows, columns, pitch = _rows_of(x, "x")
-  _call_on(x.device, "dx_scale_rows", x.data_ptr(), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, _factor(factor, x.device),
-           _lib.stream_ptr(x.device))
+  by = _factor(factor, x.device)
+  _writable(x, "x")
+  _call_on(x.device, "dx_scale_rows", x.data_ptr(), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, by, _lib.stream_ptr(x.device))
   return x
 
 
@@ -518,6 +529,7 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
     (b0, e0), (b1, e1) = _span(update), _span(out)
     if b0 != b1 and b0 < e1 and b1 < e0:
       raise ValueError("out overlaps update (it may only be update itself)")
+    _writable(out, "out")
   m, n = update.shape[-2:]
   if update.numel() == 0:
     return out

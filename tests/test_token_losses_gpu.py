@@ -176,3 +176,29 @@ def test_reference_logits_of_another_type_are_not_rounded(dtype, ref_dtype):
     assert model.logits.grad.dtype == dtype
     within(model.logits.grad, dz, 8 * s * size + half_step(dz, dtype), "dlogits")
     assert abs(float(loss_fn.last_terms[3]) - terms[3]) <= 16 * s * (1 + abs(terms[3]))
+
+
+def test_what_is_written_in_place_is_known_to_autograd():
+  """dlogits_out, scale_rows and orthogonalize's out: a backward pass that needs the old values raises, a leaf that requires
+  grad is refused, under no_grad it is not."""
+  from derl_amd import ops
+  z, actions, old, adv, _, _ = policy_inputs(4, 50, F32, 1)
+  offsets = torch.tensor([0, 2, 4], dtype=torch.int32, device=DEV)
+  one = torch.full((1,), 2.0, device=DEV)
+  writes = (lambda x: ops.token_policy_loss(x.detach(), actions, old, adv, 0.2, dlogits_out=x),
+            lambda x: ops.preference_loss(x.detach(), actions, offsets, None, 0.1, dlogits_out=x),
+            lambda x: ops.scale_rows(x, one), lambda x: ops.orthogonalize(x.detach(), out=x))
+  for write in writes:
+    w = torch.nan_to_num(z, neginf=-5.0).requires_grad_()
+    y = w.sigmoid()  # saves its result
+    write(y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+      y.sum().backward()
+    with pytest.raises(ValueError, match="leaf"):
+      write(w)
+    before = w.detach().clone()
+    with torch.no_grad():
+      write(w)
+    assert not torch.equal(before, w)
+    with torch.inference_mode():
+      write(torch.nan_to_num(z, neginf=-5.0))
