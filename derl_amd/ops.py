@@ -381,7 +381,7 @@ def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_c
   given = _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask,
                             global_batch)
   dev, rows, vocab = logits.device, given[2], given[3]
-  dlogits = _gradient_buffer(dlogits_out, logits, ref_logits)
+  dlogits = _gradient_buffer(dlogits_out, logits, actions, old_log_prob, advantages, ref_log_prob, ref_logits, mask)
   log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
   workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
@@ -424,7 +424,7 @@ def token_policy_grad_scaled(dlogits, factor, logits, actions, old_log_prob, adv
   given = _policy_arguments(logits, actions, old_log_prob, advantages, cliprange, kl_coef, entropy_coef, ref_log_prob, ref_logits, mask,
                             global_batch)
   dev, rows, vocab = logits.device, given[2], given[3]
-  _gradient_buffer(dlogits, logits, ref_logits, in_place=False)
+  _gradient_buffer(dlogits, logits, actions, old_log_prob, advantages, ref_log_prob, ref_logits, mask, in_place=False)
   workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
   _call_on(dev, "dx_token_policy_grad_scaled", *given, dlogits.data_ptr(), dlogits.stride(0) if rows > 1 else vocab, workspace.data_ptr(),
            workspace.numel(), _factor(factor, dev), _lib.stream_ptr(dev))
@@ -462,7 +462,7 @@ def _preference_loss(logits, actions, offsets, ref_log_prob, beta, label_smoothi
   act = _vector(actions, "actions", rows, dev, _INDEX)
   ref = _vector(ref_log_prob, "ref_log_prob", sequences, dev, _FLOAT)
   keep = _vector(mask, "mask", rows, dev, _FLAG)
-  dlogits = _gradient_buffer(dlogits_out, logits)
+  dlogits = _gradient_buffer(dlogits_out, logits, actions, offsets, ref_log_prob, mask)
   sequence = torch.empty(sequences, dtype=torch.float32, device=dev)
   loss_out = torch.empty(8, dtype=torch.float32, device=dev)
   # the library's scratch and behind it four floats a row
@@ -479,7 +479,7 @@ def _preference_grad_scaled(dlogits, factor, logits, actions, workspace):
   """As ``token_policy_grad_scaled``, from the workspace that ``_preference_loss`` gave."""
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
-  _gradient_buffer(dlogits, logits, in_place=False)
+  _gradient_buffer(dlogits, logits, actions, workspace, in_place=False)
   _vector(workspace, "workspace", _lib.DX_TOKEN_WORKSPACE + 2 * rows, dev, (torch.float64,))
   _call_on(dev, "dx_preference_grad_scaled", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch,
            _vector(actions, "actions", rows, dev, _INDEX), workspace.data_ptr() + 8 * _lib.DX_TOKEN_WORKSPACE, dlogits.data_ptr(),
@@ -491,6 +491,9 @@ def scale_rows(x, factor):
   """x *= factor in place, ``factor`` a float32 device scalar; nothing but the factor is read when it is 1."""
   rows, columns, pitch = _rows_of(x, "x")
   by = _factor(factor, x.device)
+  begin, end = _span(x)
+  if begin <= by < end:
+    raise ValueError("factor lies in x")
   _writable(x, "x")
   _call_on(x.device, "dx_scale_rows", x.data_ptr(), _ELEMENT_TYPES[x.dtype], rows, columns, pitch, by, _lib.stream_ptr(x.device))
   return x

@@ -202,3 +202,29 @@ def test_what_is_written_in_place_is_known_to_autograd():
     assert not torch.equal(before, w)
     with torch.inference_mode():
       write(torch.nan_to_num(z, neginf=-5.0))
+
+
+def test_a_gradient_that_lies_over_an_input_is_refused():
+  """Other workgroups read masks, actions and scalars while the gradient is being written."""
+  from derl_amd import ops
+  z, actions, old, adv, ref_lp, _ = policy_inputs(6, 40, F32, 1)
+  mask = torch.ones(6, dtype=torch.bool, device=DEV)
+  offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
+  policy = dict(logits=z, actions=actions, old_log_prob=old, advantages=adv, cliprange=0.2, ref_log_prob=ref_lp, mask=mask)
+  preference = dict(logits=z, actions=actions, offsets=offsets, ref_log_prob=ref_lp[:2], beta=0.1, mask=mask)
+  for call, given in ((ops.token_policy_loss, policy), (ops.preference_loss, preference)):
+    for name, value in given.items():
+      if not isinstance(value, torch.Tensor) or name == "logits":
+        continue
+      store = torch.zeros(6 * 40 + 64, device=DEV)
+      inside = store[100:].view(value.dtype)[:value.numel()].view(value.shape)  # (16-byte aligned)
+      inside.copy_(value)
+      with pytest.raises(ValueError, match="overlaps"):
+        call(**{**given, name: inside}, dlogits_out=store[:240].view(6, 40))
+      behind = store[240:].view(value.dtype)[:value.numel()].view(value.shape)
+      behind.copy_(value)
+      got = call(**{**given, name: behind}, dlogits_out=store[:240].view(6, 40))
+      assert all(torch.equal(a, b) for a, b in zip(got, call(**given)))
+  x = torch.ones(4, 6, device=DEV)
+  with pytest.raises(ValueError, match="lies in x"):
+    ops.scale_rows(x, x[1, 2:3])
