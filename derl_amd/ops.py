@@ -246,6 +246,28 @@ def normal_loss(head_out, logstd, actions, old_log_prob, advantages, old_values,
 _ELEMENT_TYPES = {torch.float32: _lib.DX_F32, torch.bfloat16: _lib.DX_BF16, torch.float16: _lib.DX_F16}
 
 
+class _NoGradient(torch.autograd.Function):
+  """Results of a call that has no gradient, on inputs that require one: they belong to the graph, and whoever
+  differentiates them is told (detached, their terms would be missing from a gradient without a word)."""
+
+  @staticmethod
+  def forward(ctx, source, name, *results):
+    ctx.name = name
+    return tuple(t.view_as(t) for t in results)
+
+  @staticmethod
+  def backward(ctx, *grads):
+    raise RuntimeError(f"{ctx.name} has no gradient: call it under torch.no_grad() or on detached inputs; "
+                       "TokenPolicyLoss and PreferenceLoss are the losses to differentiate")
+
+
+def _constants(source, name, *results):
+  """``results``, tied to ``source`` where autograd would expect a gradient to it."""
+  if source.requires_grad and torch.is_grad_enabled():
+    results = _NoGradient.apply(source, name, *results)
+  return results
+
+
 def _call_on(device, name, *args):
   """One native call with ``device`` current (kernels launch on the current device)."""
   if device.index == torch.cuda.current_device():
@@ -329,7 +351,11 @@ def token_log_prob(logits, actions, mask=None):
   int64, mask (N,) bool or uint8: rows that are False are not read and give 0.  Returns (log_prob,
   entropy), float32 (N,).  A logit of -inf is an action that cannot be chosen; a row without any
   distribution (all -inf, NaN, +inf) or an action outside [0, V) gives NaN.  N = 1 .. is the form for
-  single tokens of sequences being generated."""
+  single tokens of sequences being generated.  They have no gradient: differentiating them raises."""
+  return _constants(logits, "token_log_prob", *_token_log_prob(logits, actions, mask))
+
+
+def _token_log_prob(logits, actions, mask):
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
   log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
@@ -352,15 +378,15 @@ def _check_offsets(offsets, device):
 def sequence_log_prob(logits, actions, offsets, mask=None):
   """Summed log-probabilities of packed sequences: sequence s holds the rows offsets[s] .. offsets[s + 1]
   of ``logits`` (offsets int32 (S + 1,), non-decreasing; empty sequences give 0).  float32 (S,): what
-  ``preference_loss`` takes as ``ref_log_prob`` when the logits are the reference's."""
+  ``preference_loss`` takes as ``ref_log_prob`` when the logits are the reference's.  Differentiating them raises."""
   rows, _, _ = _rows_of(logits, "logits")
   dev = logits.device
   sequences = _check_offsets(offsets, dev)
-  log_prob, _ = token_log_prob(logits, actions, mask)
+  log_prob, _ = _token_log_prob(logits, actions, mask)
   out = torch.empty(sequences, dtype=torch.float32, device=dev)
   _call_on(dev, "dx_sequence_log_prob", log_prob.data_ptr(), offsets.data_ptr(), rows, sequences, out.data_ptr(),
            _lib.stream_ptr(dev))
-  return out
+  return _constants(logits, "sequence_log_prob", out)[0]
 
 
 def token_policy_loss(logits, actions, old_log_prob, advantages, cliprange, kl_coef=0., entropy_coef=0.,
@@ -511,7 +537,7 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
   copies) and rounded to the type once; every row and column keeps the digits its own size allows, however small it is
   against the others.  Contiguous; the result has update's type and shape.  ``out`` may be ``update``.  With eps > 0 a
   zero matrix gives zeros; a matrix with a NaN or an infinity gives NaN.  Coefficients that let a singular value pass
-  8, and what `a` alone makes of 1, leave fp16's range."""
+  8, and what `a` alone makes of 1, leave fp16's range.  Differentiating the result raises."""
   if not isinstance(update, torch.Tensor) or not update.is_cuda:
     raise ValueError("update must be a tensor on the GPU (derl_amd has no CPU path)")
   if update.dtype not in _ELEMENT_TYPES:
@@ -523,9 +549,12 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
   a, b, c = (float(v) for v in coefficients)
   if not all(math.isfinite(v) for v in (a, b, c, eps)) or eps < 0:
     raise ValueError(f"coefficients and eps must be finite, eps >= 0: {coefficients}, {eps}")
-  if out is None:
+  given = out is not None
+  if not given:
     out = torch.empty_like(update)
   else:
+    if update.requires_grad and torch.is_grad_enabled():
+      raise ValueError("out is given and update requires grad: orthogonalize has no gradient")
     _dev(out, "out", update.dtype)
     if out.shape != update.shape or out.device != update.device:
       raise ValueError(f"out must match update: {tuple(out.shape)} on {out.device}")
@@ -543,7 +572,7 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
   workspace = torch.empty(need, dtype=torch.uint8, device=update.device)
   _call_on(update.device, "dx_orthogonalize", update.data_ptr(), kind, batch, m, n, int(steps), a, b, c, float(eps),
            out.data_ptr(), workspace.data_ptr(), need, _lib.stream_ptr(update.device))
-  return out
+  return out if given else _constants(update, "orthogonalize", out)[0]
 
 
 def muon_momentum(grads, momentum, update, partials, max_norm, mu, nesterov=True, norm_out=None):

@@ -228,3 +228,27 @@ def test_a_gradient_that_lies_over_an_input_is_refused():
   x = torch.ones(4, 6, device=DEV)
   with pytest.raises(ValueError, match="lies in x"):
     ops.scale_rows(x, x[1, 2:3])
+
+
+def test_results_without_a_gradient_say_so():
+  """token_log_prob, sequence_log_prob and orthogonalize on inputs that require grad: the same values; a gradient through them
+  raises, alone or beside other terms; nothing changes under no_grad or for detached inputs."""
+  from derl_amd import ops
+  z, actions, _, _, _, _ = policy_inputs(6, 300, F32, 1)
+  z = torch.nan_to_num(z, neginf=-9.0)
+  offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
+  calls = (lambda x: ops.token_log_prob(x, actions)[0], lambda x: ops.token_log_prob(x, actions)[1],
+           lambda x: ops.sequence_log_prob(x, actions, offsets), lambda x: ops.orthogonalize(x))
+  for call in calls:
+    want = call(z)
+    assert not want.requires_grad
+    w = z.clone().requires_grad_()
+    got = call(w * 1.0)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="no gradient"):
+      (got.sum() + w.sum()).backward()
+    with torch.no_grad():
+      assert not call(w).requires_grad
+    assert not call(w.detach()).requires_grad
+  with pytest.raises(ValueError, match="no gradient"):
+    ops.orthogonalize(w * 1.0, out=torch.empty_like(z))
