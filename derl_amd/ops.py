@@ -355,16 +355,16 @@ def token_log_prob(logits, actions, mask=None):
   return _constants(logits, "token_log_prob", *_token_log_prob(logits, actions, mask))
 
 
-def _token_log_prob(logits, actions, mask):
+def _token_log_prob(logits, actions, mask, entropies=True):
   rows, vocab, pitch = _rows_of(logits, "logits")
   dev = logits.device
   log_prob = torch.empty(rows, dtype=torch.float32, device=dev)
-  entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+  entropy = torch.empty(rows, dtype=torch.float32, device=dev) if entropies else None
   workspace = torch.empty(_lib.DX_TOKEN_WORKSPACE, dtype=torch.float64, device=dev)
   act = _vector(actions, "actions", rows, dev, _INDEX)
   keep = _vector(mask, "mask", rows, dev, _FLAG)
   _call_on(dev, "dx_token_log_prob", logits.data_ptr(), _ELEMENT_TYPES[logits.dtype], rows, vocab, pitch, act, keep,
-           log_prob.data_ptr(), entropy.data_ptr(), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(dev))
+           log_prob.data_ptr(), entropy.data_ptr() if entropies else None, workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(dev))
   return log_prob, entropy
 
 
@@ -382,7 +382,7 @@ def sequence_log_prob(logits, actions, offsets, mask=None):
   rows, _, _ = _rows_of(logits, "logits")
   dev = logits.device
   sequences = _check_offsets(offsets, dev)
-  log_prob, _ = _token_log_prob(logits, actions, mask)
+  log_prob, _ = _token_log_prob(logits, actions, mask, entropies=False)
   out = torch.empty(sequences, dtype=torch.float32, device=dev)
   _call_on(dev, "dx_sequence_log_prob", log_prob.data_ptr(), offsets.data_ptr(), rows, sequences, out.data_ptr(),
            _lib.stream_ptr(dev))
