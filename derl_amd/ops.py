@@ -243,6 +243,7 @@ def normal_loss(head_out, logstd, actions, old_log_prob, advantages, old_values,
 
 # ---- policies over a vocabulary -----------------------------------------------------------------
 
+_INT_MAX = (1 << 31) - 1  # ctypes would wrap what is larger around
 _ELEMENT_TYPES = {torch.float32: _lib.DX_F32, torch.bfloat16: _lib.DX_BF16, torch.float16: _lib.DX_F16}
 
 
@@ -286,6 +287,8 @@ def _rows_of(t, name, like=None):
   if t.ndim != 2 or t.shape[1] < 1:
     raise ValueError(f"{name} must be (rows, vocab) with vocab >= 1, got {tuple(t.shape)}")
   rows, columns = t.shape
+  if columns > 1 << 30:
+    raise ValueError(f"{name} must have 2^30 columns at most, got {columns}")
   pitch = t.stride(0) if rows > 1 else columns
   if (columns > 1 and t.stride(1) != 1) or pitch < columns:
     raise ValueError(f"the rows of {name} must be contiguous and must not overlap: strides {t.stride()}")
@@ -372,6 +375,8 @@ def _check_offsets(offsets, device):
   _dev(offsets, "offsets", torch.int32)
   if offsets.ndim != 1 or offsets.numel() < 1 or offsets.device != device:
     raise ValueError(f"offsets must be a vector of sequence borders on {device}, got {tuple(offsets.shape)} on {offsets.device}")
+  if offsets.numel() > _INT_MAX:
+    raise ValueError(f"offsets must have fewer than 2^31 entries, got {offsets.numel()}")
   return offsets.numel() - 1
 
 
@@ -544,8 +549,8 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
     raise ValueError(f"update must be float32, bfloat16 or float16, got {update.dtype}")
   if update.ndim < 2 or not update.is_contiguous():
     raise ValueError(f"update must be contiguous (..., m, n), got {tuple(update.shape)}, strides {update.stride()}")
-  if int(steps) < 1:
-    raise ValueError(f"steps must be >= 1, got {steps}")
+  if not 1 <= int(steps) <= _INT_MAX:
+    raise ValueError(f"steps must be >= 1 (and below 2^31), got {steps}")
   a, b, c = (float(v) for v in coefficients)
   if not all(math.isfinite(v) for v in (a, b, c, eps)) or eps < 0:
     raise ValueError(f"coefficients and eps must be finite, eps >= 0: {coefficients}, {eps}")
@@ -565,7 +570,7 @@ def orthogonalize(update, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=N
   m, n = update.shape[-2:]
   if update.numel() == 0:
     return out
-  batch = update.numel() // (m * n)
+  batch, m, n = (min(size, _INT_MAX) for size in (update.numel() // (m * n), m, n))  # (the library says what it takes)
   kind = _ELEMENT_TYPES[update.dtype]
   need = _lib.load().dx_orthogonalize_workspace(kind, batch, m, n)
   _lib.check(min(need, 0), "dx_orthogonalize_workspace")

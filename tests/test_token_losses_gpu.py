@@ -252,3 +252,25 @@ def test_results_without_a_gradient_say_so():
     assert not call(w.detach()).requires_grad
   with pytest.raises(ValueError, match="no gradient"):
     ops.orthogonalize(w * 1.0, out=torch.empty_like(z))
+
+
+def test_sizes_that_no_int_holds_are_refused():
+  """2^32 + 3 columns, sides or matrices are not 3."""
+  from derl_amd import ops
+  if torch.cuda.mem_get_info()[0] < 40e9:
+    pytest.skip("needs 35 GB of device memory")
+  size = (1 << 32) + 3
+  wide = torch.empty(1, size, dtype=BF16, device=DEV)
+  actions = torch.zeros(1, dtype=torch.int64, device=DEV)
+  one = torch.ones(1, device=DEV)
+  for call in (lambda: ops.token_log_prob(wide, actions), lambda: ops.token_policy_loss(wide, actions, one, one, 0.2),
+               lambda: ops.scale_rows(wide, one), lambda: ops.sequence_log_prob(wide, actions, torch.zeros(2, dtype=torch.int32, device=DEV))):
+    with pytest.raises(ValueError, match="columns"):
+      call()
+  for shape in ((1, size), (size, 1)):
+    with pytest.raises(RuntimeError, match="sides"):
+      ops.orthogonalize(wide.view(shape))
+  with pytest.raises(RuntimeError, match="batch"):
+    ops.orthogonalize(wide.view(size, 1, 1))
+  with pytest.raises(ValueError, match="steps"):
+    ops.orthogonalize(torch.ones(2, 2, device=DEV), steps=(1 << 32) + 1)
