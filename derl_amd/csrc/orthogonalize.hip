@@ -996,6 +996,8 @@ Scan make_scan(int dtype, int m, int n) {
   return s;
 }
 struct Plan {
+  bool one_launch;             // the matrices fit a workgroup's LDS
+  int batch;                   // matrices at a time of the products' launches
   int r, c, rp, cp;
   Scan scan;
   long long x, sq;             // values of X and of A per matrix, padded
@@ -1005,6 +1007,8 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   Plan p;
   p.r = m < n ? m : n;
   p.c = m < n ? n : m;
+  p.one_launch = small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32) <= kSmallLds;
+  p.batch = p.one_launch ? 1 : batch;
   p.rp = (p.r + kPad - 1) / kPad * kPad;
   p.cp = (p.c + kPad - 1) / kPad * kPad;
   p.x = static_cast<long long>(p.rp) * p.cp;
@@ -1014,10 +1018,14 @@ Plan make_plan(int dtype, int batch, int m, int n) {
   auto most = [](long long x, long long y) { return x > y ? x : y; };
   p.sums = most(p.scan.bands * p.scan.strips, other.bands * other.strips);
   p.most = most(p.scan.floats(), other.floats());
-  p.split_floats = static_cast<long long>(kSplitGroups) * (p.r > 1024 ? 128 * 128 : 64 * 64);  // (128 x 128 tiles are split where there are many)
+  // (128 x 128 tiles are split where there are many)
+  p.split_floats = p.one_launch ? 0 : static_cast<long long>(kSplitGroups) * (p.r > 1024 ? 128 * 128 : 64 * 64);
   // two terms of X, two copies of X^T, A and M; fp32 copies of X and A; the parts of split products; the norm's sums, the exponents,
   // the largest magnitudes
-  p.bytes = batch * (4 * (3 * p.x + 2 * p.sq) + 4 * (p.x + p.sq) + 8 * p.sums + 4LL * (p.rp + p.cp) + 4 * p.most) + 4LL * kSplitGroups + 4 * p.split_floats;
+  p.bytes = p.batch * (4 * (3 * p.x + 2 * p.sq) + 4 * (p.x + p.sq) + 8 * p.sums + 4LL * (p.rp + p.cp) + 4 * p.most) + 4LL * kSplitGroups + 4 * p.split_floats;
+  // one launch takes nothing of it (kSmallSteps): what the launches of one matrix take, whose steps may be more, and a token amount
+  // a matrix, so that sizes grow with the batch
+  if (p.one_launch) p.bytes += 256LL * batch;
   return p;
 }
 int check_shape(int dtype, int batch, int m, int n) {
@@ -1083,7 +1091,8 @@ struct Buffers {
   float *master_x, *master_a;
   int *exp_r, *exp_c;
 };
-int run_steps(const Plan &p, int batch, int steps, NsArgs a, const Buffers &w, hipStream_t s) {
+int run_steps(const Plan &p, int steps, NsArgs a, const Buffers &w, hipStream_t s) {
+  const int batch = p.batch;
   Known known = known_at_start(a.b, a.c);
   for (int k = 0; k < steps; ++k) {
     const Known next = grown(known, a.a, a.b, a.c);
@@ -1129,47 +1138,18 @@ int run_steps(const Plan &p, int batch, int steps, NsArgs a, const Buffers &w, h
 }
 
 template <typename V>
-int launch_start(const V *update, const Plan &p, int batch, PackArgs k, double *sums, float *row_most, float *col_most, hipStream_t s) {
-  hipLaunchKernelGGL(ns_scan_kernel<V>, dim3(p.scan.strips, p.scan.bands, batch), dim3(256), 0, s, update, k.m, k.n, p.scan.band, p.scan.strip, sums, row_most,
+int launch_start(const V *update, const Plan &p, PackArgs k, double *sums, float *row_most, float *col_most, hipStream_t s) {
+  hipLaunchKernelGGL(ns_scan_kernel<V>, dim3(p.scan.strips, p.scan.bands, p.batch), dim3(256), 0, s, update, k.m, k.n, p.scan.band, p.scan.strip, sums, row_most,
                      col_most);
   DX_LAUNCH_CHECK();
-  hipLaunchKernelGGL(ns_pack_kernel<V>, dim3(cdiv(k.n, kPad), cdiv(k.m, kPad), batch), dim3(256), 0, s, k);
+  hipLaunchKernelGGL(ns_pack_kernel<V>, dim3(cdiv(k.n, kPad), cdiv(k.m, kPad), p.batch), dim3(256), 0, s, k);
   DX_LAUNCH_CHECK();
   return DX_OK;
 }
 
-}  // namespace
-}  // namespace dx
-
-extern "C" long long dx_orthogonalize_workspace(int dtype, int batch, int m, int n) {
-  DX_TRACE("dx_orthogonalize_workspace");
-  if (int rc = dx::check_shape(dtype, batch, m, n)) return rc;
-  return dx::make_plan(dtype, batch, m, n).bytes;
-}
-
-extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m, int n, int steps, float a, float b, float c, float eps,
-                                void *out, void *workspace, long long workspace_bytes, void *stream) {
-  DX_TRACE("dx_orthogonalize");
-  using namespace dx;
-  if (int rc = check_shape(dtype, batch, m, n)) return rc;
-  DX_REQUIRE(steps >= 1, "dx_orthogonalize: steps %d < 1", steps);
-  if (batch == 0) return DX_OK;
-  const int size = dtype == DX_F32 ? 4 : 2;
-  DX_REQUIRE(update && out && workspace, "dx_orthogonalize: null pointer");
-  DX_REQUIRE(aligned(update, size) && aligned(out, size) && aligned(workspace, 256), "dx_orthogonalize: misaligned pointer");
-  const Plan p = make_plan(dtype, batch, m, n);
-  if (workspace_bytes < p.bytes) return fail(DX_EWS, "dx_orthogonalize: workspace of %lld bytes, %lld needed", workspace_bytes, p.bytes);
-  hipStream_t s = as_stream(stream);
-  if (steps <= kSmallSteps && small_lds(cdiv(p.r, 32) * 32, cdiv(p.c, 32) * 32) <= kSmallLds) {
-    const int r32 = cdiv(p.r, 32) * 32, c32 = cdiv(p.c, 32) * 32;
-    SmallArgs q{update, out, m, n, p.r, p.c, r32, c32, steps, m > n, a, b, c, eps, {}};
-    Known known = known_at_start(b, c);
-    for (int i = 0; i <= steps; ++i, known = grown(known, a, b, c)) q.powers[i] = known;
-    const int bytes = static_cast<int>(small_lds(r32, c32));
-    if (dtype == DX_F32) return launch_small<float>(q, batch, bytes, s);
-    if (dtype == DX_BF16) return launch_small<__bf16>(q, batch, bytes, s);
-    return launch_small<_Float16>(q, batch, bytes, s);
-  }
+// every step's products as launches, p.batch matrices
+int run_launches(const Plan &p, const void *update, int dtype, int m, int n, int steps, float a, float b, float c, float eps, void *out,
+                 void *workspace, hipStream_t s) {
   char *at = static_cast<char *>(workspace);
   auto take = [&](auto *&to, long long count) {
     to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(at);
@@ -1179,20 +1159,20 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   float *split, *row_most, *col_most;
   double *sums;
   unsigned *arrivals;
-  take(w.X, 2 * p.x * batch);
-  take(w.XT[0], 2 * p.x * batch);
-  take(w.XT[1], 2 * p.x * batch);
-  take(w.A, 2 * p.sq * batch);
-  take(w.M, 2 * p.sq * batch);
-  take(w.master_x, p.x * batch);
-  take(w.master_a, p.sq * batch);
+  take(w.X, 2 * p.x * p.batch);
+  take(w.XT[0], 2 * p.x * p.batch);
+  take(w.XT[1], 2 * p.x * p.batch);
+  take(w.A, 2 * p.sq * p.batch);
+  take(w.M, 2 * p.sq * p.batch);
+  take(w.master_x, p.x * p.batch);
+  take(w.master_a, p.sq * p.batch);
   take(split, p.split_floats);
-  take(sums, p.sums * batch);
-  take(w.exp_r, static_cast<long long>(p.rp) * batch);
-  take(w.exp_c, static_cast<long long>(p.cp) * batch);
+  take(sums, p.sums * p.batch);
+  take(w.exp_r, static_cast<long long>(p.rp) * p.batch);
+  take(w.exp_c, static_cast<long long>(p.cp) * p.batch);
   take(arrivals, kSplitGroups);
-  take(row_most, static_cast<long long>(m) * p.scan.strips * batch);
-  take(col_most, static_cast<long long>(n) * p.scan.bands * batch);
+  take(row_most, static_cast<long long>(m) * p.scan.strips * p.batch);
+  take(col_most, static_cast<long long>(n) * p.scan.bands * p.batch);
   const bool tall = m > n;
   PackArgs k{};
   k.in = update;
@@ -1220,9 +1200,9 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   k.cap = known_at_start(b, c).cap;
   k.arrivals = arrivals;
   k.counts = kSplitGroups;
-  if (int rc = dtype == DX_F32 ? launch_start(static_cast<const float *>(update), p, batch, k, sums, row_most, col_most, s)
-               : dtype == DX_BF16 ? launch_start(static_cast<const __bf16 *>(update), p, batch, k, sums, row_most, col_most, s)
-                                  : launch_start(static_cast<const _Float16 *>(update), p, batch, k, sums, row_most, col_most, s)) return rc;
+  if (int rc = dtype == DX_F32 ? launch_start(static_cast<const float *>(update), p, k, sums, row_most, col_most, s)
+               : dtype == DX_BF16 ? launch_start(static_cast<const __bf16 *>(update), p, k, sums, row_most, col_most, s)
+                                  : launch_start(static_cast<const _Float16 *>(update), p, k, sums, row_most, col_most, s)) return rc;
   NsArgs g{};
   g.arrivals = arrivals;
   g.partials = split;
@@ -1235,5 +1215,45 @@ extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m,
   g.r = p.r;
   g.cols = p.c;
   g.tall = tall;
-  return run_steps(p, batch, steps, g, w, s);
+  return run_steps(p, steps, g, w, s);
+}
+
+}  // namespace
+}  // namespace dx
+
+extern "C" long long dx_orthogonalize_workspace(int dtype, int batch, int m, int n) {
+  DX_TRACE("dx_orthogonalize_workspace");
+  if (int rc = dx::check_shape(dtype, batch, m, n)) return rc;
+  return dx::make_plan(dtype, batch, m, n).bytes;
+}
+
+extern "C" int dx_orthogonalize(const void *update, int dtype, int batch, int m, int n, int steps, float a, float b, float c, float eps,
+                                void *out, void *workspace, long long workspace_bytes, void *stream) {
+  DX_TRACE("dx_orthogonalize");
+  using namespace dx;
+  if (int rc = check_shape(dtype, batch, m, n)) return rc;
+  DX_REQUIRE(steps >= 1, "dx_orthogonalize: steps %d < 1", steps);
+  if (batch == 0) return DX_OK;
+  const int size = dtype == DX_F32 ? 4 : 2;
+  DX_REQUIRE(update && out && workspace, "dx_orthogonalize: null pointer");
+  DX_REQUIRE(aligned(update, size) && aligned(out, size) && aligned(workspace, 256), "dx_orthogonalize: misaligned pointer");
+  const Plan p = make_plan(dtype, batch, m, n);
+  if (workspace_bytes < p.bytes) return fail(DX_EWS, "dx_orthogonalize: workspace of %lld bytes, %lld needed", workspace_bytes, p.bytes);
+  hipStream_t s = as_stream(stream);
+  if (p.one_launch && steps <= kSmallSteps) {
+    const int r32 = cdiv(p.r, 32) * 32, c32 = cdiv(p.c, 32) * 32;
+    SmallArgs q{update, out, m, n, p.r, p.c, r32, c32, steps, m > n, a, b, c, eps, {}};
+    Known known = known_at_start(b, c);
+    for (int i = 0; i <= steps; ++i, known = grown(known, a, b, c)) q.powers[i] = known;
+    const int bytes = static_cast<int>(small_lds(r32, c32));
+    if (dtype == DX_F32) return launch_small<float>(q, batch, bytes, s);
+    if (dtype == DX_BF16) return launch_small<__bf16>(q, batch, bytes, s);
+    return launch_small<_Float16>(q, batch, bytes, s);
+  }
+  const long long bytes = static_cast<long long>(m) * n * size;
+  for (int z = 0; z < batch; z += p.batch) {
+    const char *from = static_cast<const char *>(update) + z * bytes;
+    if (int rc = run_launches(p, from, dtype, m, n, steps, a, b, c, eps, static_cast<char *>(out) + z * bytes, workspace, s)) return rc;
+  }
+  return DX_OK;
 }

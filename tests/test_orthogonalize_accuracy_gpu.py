@@ -102,3 +102,32 @@ def test_other_coefficients(m, n, coefficients, steps):
     s = (a * s + b * s ** 3 + c * s ** 5).abs()
   want, _ = newton_schulz64(g, steps, coefficients, eps=1e-7)
   assert float((got - want).norm()) <= bound, (float((got - want).norm()), bound)
+
+
+@pytest.mark.parametrize("shape", [(3, 20, 60), (2, 60, 60), (3, 96, 90), (2, 130, 200)])
+def test_any_number_of_steps(shape):
+  """Coefficients whose iteration converges (slope 0 at 1): the last steps leave their own rounding alone; more steps than the
+  one-launch kernel holds the scales of."""
+  from derl_amd import ops
+  g = torch.randn(shape, generator=gen(3), device=DEV)
+  coefficients = (15 / 8, -10 / 8, 3 / 8)
+  got = ops.orthogonalize(g, steps=45, coefficients=coefficients)
+  for k in range(shape[0]):
+    want, norms = newton_schulz64(g[k], 45, coefficients)
+    assert float((got[k].double() - want).norm()) <= unit(max(shape)) * norms[-1]
+  again = g.clone()
+  assert torch.equal(ops.orthogonalize(again, steps=45, coefficients=coefficients, out=again), got)
+
+
+def test_memory_of_many_small_matrices():
+  from derl_amd import ops
+  g = torch.randn(20000, 64, 64, generator=gen(1), device=DEV)
+  out = torch.empty_like(g)
+  torch.cuda.synchronize()
+  torch.cuda.reset_peak_memory_stats()
+  before = torch.cuda.memory_allocated()
+  ops.orthogonalize(g, out=out)
+  torch.cuda.synchronize()
+  assert torch.cuda.max_memory_allocated() - before < 16e6
+  for k in (0, 19999):
+    assert torch.equal(out[k], ops.orthogonalize(g[k]))
