@@ -10,6 +10,7 @@ from ..policies import ActorCriticPolicy, sampling_seed
 from ..runners.onpolicy import make_ppo_runner
 from .factory import Factory
 
+_OPTIMIZER = dict(choices=["adam", "muon"], default="adam")  # a flag of this package's: the reference has Adam
 # flag -> (atari, mujoco); derl/factory/ppo.py:19-49
 _PRESETS = (
     ("num-train-steps", 10e6, 1e6),
@@ -25,6 +26,7 @@ _PRESETS = (
     ("max-grad-norm", 0.5, 0.5),
     ("lr", 2.5e-4, 3e-4),
     ("optimizer-epsilon", 1e-5, 1e-5),
+    ("optimizer", _OPTIMIZER, _OPTIMIZER),
 )
 _COLUMN = {"atari": 1, "mujoco": 2}
 _SKIP_CHECK = ("nenvs",)  # consumed by env construction, not by the factory
