@@ -103,7 +103,8 @@ class TokenLoss(Loss):
 class TokenPolicyLoss(TokenLoss):
   """Clipped policy loss with a KL term and an entropy bonus (``ops.token_policy_loss``).  ``data``: observations,
   actions, log_prob (of the policy that acted), advantages; optional ref_log_prob or ref_logits (of the reference
-  policy), mask.  Reference logits of a wider type than the policy's are not rounded to it: the loss is then taken of
+  policy), mask, global_batch (unmasked rows over all shards: what the gradient is divided by, so that shards' add
+  up).  Reference logits of a wider type than the policy's are not rounded to it: the loss is then taken of
   the policy's logits in the type that holds both (the gradient is rounded to theirs on its way back)."""
   tags = ("loss", "policy_loss", "entropy", "kl", "clip_fraction", "ratio", "log_prob", "tokens")
 
@@ -130,7 +131,8 @@ class TokenPolicyLoss(TokenLoss):
     given = dict(actions=self._flat(data, "actions", torch.int64), old_log_prob=self._flat(data, "log_prob", f32),
                  advantages=self._flat(data, "advantages", f32), ref_log_prob=self._flat(data, "ref_log_prob", f32, required=False),
                  ref_logits=ref_logits, mask=self._mask(data))
-    fixed = dict(cliprange=self.cliprange, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
+    fixed = dict(cliprange=self.cliprange, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef,
+                 global_batch=int(data.get("global_batch") or 0))
     terms, dlogits, _ = ops.token_policy_loss(logits, **given, **fixed)
     names = [name for name, value in given.items() if value is not None]
 
@@ -142,7 +144,8 @@ class TokenPolicyLoss(TokenLoss):
 
 class PreferenceLoss(TokenLoss):
   """Loss of paired log ratios (``ops.preference_loss``).  ``data``: observations of the packed sequences (chosen,
-  rejected, chosen, ...), actions, offsets (their borders); optional ref_log_prob (per sequence), mask."""
+  rejected, chosen, ...), actions, offsets (their borders); optional ref_log_prob (per sequence), mask, global_pairs
+  (pairs over all shards: what the gradient is divided by, so that shards' add up)."""
   tags = ("loss", "accuracy", "margin", "chosen_reward", "rejected_reward", "chosen_log_prob", "rejected_log_prob", "pairs")
 
   def __init__(self, model, beta=0.1, label_smoothing=0., name=None):
@@ -153,5 +156,5 @@ class PreferenceLoss(TokenLoss):
     actions = self._flat(data, "actions", torch.int64)
     terms, dlogits, _, workspace = ops._preference_loss(  # pylint: disable=protected-access
         logits, actions, self._flat(data, "offsets", torch.int32), self._flat(data, "ref_log_prob", torch.float32, required=False),
-        self.beta, self.label_smoothing, self._mask(data), 0)
+        self.beta, self.label_smoothing, self._mask(data), int(data.get("global_pairs") or 0))
     return terms, dlogits, ops._preference_grad_scaled, [actions, workspace]  # pylint: disable=protected-access

@@ -274,3 +274,47 @@ def test_sizes_that_no_int_holds_are_refused():
     ops.orthogonalize(wide.view(size, 1, 1))
   with pytest.raises(ValueError, match="steps"):
     ops.orthogonalize(torch.ones(2, 2, device=DEV), steps=(1 << 32) + 1)
+
+
+def test_gradients_of_shards_add_up():
+  """global_batch and global_pairs through the classes: the shards' gradients sum to the whole batch's (each of them off by
+  ``slack`` of its terms, of which there are eight, and three fp32 roundings of the library's products around them)."""
+  model = torch.nn.Linear(16, 120).to(DEV)
+  (policy, data), (preference, pairs) = losses_of(model, 24, 120, 16)
+  pairs["offsets"] = torch.tensor([0, 5, 12, 17, 24], dtype=torch.int32, device=DEV)
+  cut = lambda d, a, b: {k: v[a:b] if k != "offsets" else v for k, v in d.items()}  # noqa: E731
+  shards = [(policy, data, [dict(cut(data, 0, 9), global_batch=int(data["mask"].sum())),
+                            dict(cut(data, 9, 24), global_batch=int(data["mask"].sum()))]),
+            (preference, pairs, [dict(cut(pairs, 0, 12), offsets=pairs["offsets"][:3], global_pairs=2),
+                                 dict(cut(pairs, 12, 24), offsets=pairs["offsets"][2:] - 12, global_pairs=2)])]
+  for loss_fn, whole, parts in shards:
+    want = torch.autograd.grad(loss_fn(whole), model.parameters())
+    got = [torch.autograd.grad(loss_fn(part), model.parameters()) for part in parts]
+    for w, a, b in zip(want, *got):
+      assert float((w - a - b).norm()) <= (16 * slack(120) + 16 * 2.0 ** -24) * float(a.norm() + b.norm())
+
+
+def test_trainer_steps_a_module_with_the_losses():
+  """Trainer and Alg, a torch optimizer and a clipped norm around both losses: the step is that of the same calls by hand."""
+  from types import SimpleNamespace
+  import derl_amd as derl
+  for which in (0, 1):
+    models = []
+    for by_hand in (False, True):
+      torch.manual_seed(0)
+      model = torch.nn.Sequential(torch.nn.Linear(16, 32), torch.nn.Tanh(), torch.nn.Linear(32, 120)).to(DEV)
+      loss_fn, data = losses_of(model, 24, 120, 16)[which]
+      optimizer = torch.optim.SGD(model.parameters(), lr=0.1)
+      alg = derl.Alg(SimpleNamespace(policy=SimpleNamespace(model=model), step_count=0), derl.Trainer(optimizer, max_grad_norm=0.05), loss_fn)
+      for _ in range(2):
+        if by_hand:
+          optimizer.zero_grad()
+          loss_fn(data).backward()
+          torch.nn.utils.clip_grad_norm_(model.parameters(), 0.05)
+          optimizer.step()
+        else:
+          loss = alg.step(data)
+          assert loss.shape == () and torch.isfinite(loss)
+      models.append(model)
+    for a, b in zip(models[0].parameters(), models[1].parameters()):
+      assert torch.equal(a, b)
