@@ -318,3 +318,51 @@ def test_trainer_steps_a_module_with_the_losses():
       models.append(model)
     for a, b in zip(models[0].parameters(), models[1].parameters()):
       assert torch.equal(a, b)
+
+
+# rows, columns and distance of rows in elements of 2 bytes, the last rows past 2^32 bytes: a wave a row, rows in registers (256 and 1024
+# threads), rows read twice, pieces, and 70000 rows of 32768 side by side
+FAR = [(3, 4000, 1_200_000_000), (3, 12001, 1_200_000_000), (130, 100_003, 18_000_000), (130, 140_001, 18_000_000), (3, 40003, 1_200_000_000),
+       (70_000, 32_768, 32_768)]
+
+
+@pytest.mark.parametrize("ref", ["none", "logits"])
+@pytest.mark.parametrize("rows,vocab,pitch", FAR)
+def test_rows_past_32_bits_in_every_row_kernel(rows, vocab, pitch, ref):
+  """Rows far apart give what the same rows give side by side (or, 70000 of them, what the last ones give alone)."""
+  from derl_amd import ops
+  if torch.cuda.mem_get_info()[0] < 40e9:
+    pytest.skip("needs 30 GB of device memory")
+  few = min(rows, 130)
+  z, actions, old, adv, _, ref_z = policy_inputs(few, vocab, BF16, 3)
+  views = []
+  for source in (z, ref_z):
+    store = torch.empty((rows - 1) * pitch + vocab, dtype=BF16, device=DEV)
+    view = store.as_strided((rows, vocab), (pitch, 1))
+    if rows > few:
+      view.fill_(0.5)
+    view[rows - few:] = source
+    views.append(view)
+  view, ref_view = views[0], views[1] if ref == "logits" else None
+  wide = lambda x: torch.cat([torch.zeros(rows - few, dtype=x.dtype, device=DEV), x])  # noqa: E731
+  mask = wide(torch.ones(few, dtype=torch.bool, device=DEV))
+  offsets = torch.tensor([rows - few, rows - 2, rows], dtype=torch.int32, device=DEV)
+  near = torch.tensor([0, few - 2, few], dtype=torch.int32, device=DEV)
+  want = [ops.token_log_prob(z, actions)[0], ops.preference_loss(z, actions, near, None, 0.1)[1]]
+  got = [ops.token_log_prob(view, wide(actions), mask)[0][rows - few:], ops.preference_loss(view, wide(actions), offsets, None, 0.1)[1][rows - few:]]
+  _, dz, lp = ops.token_policy_loss(z, actions, old, adv, 0.2, kl_coef=0.1, entropy_coef=0.01, ref_logits=ref_z if ref == "logits" else None)
+  _, far, far_lp = ops.token_policy_loss(view, wide(actions), wide(old), wide(adv), 0.2, kl_coef=0.1, entropy_coef=0.01, ref_logits=ref_view,
+                                         mask=mask, dlogits_out=view)
+  assert far is view
+  if rows == few:
+    for a, b in zip([dz, lp] + want, [far, far_lp] + got):
+      assert torch.equal(a, b)
+  else:  # (other kernels, by the number of rows: off by their sums)
+    s = slack(vocab)
+    within(far_lp[rows - few:], lp, 2 * s + 2.0 ** -22 * (lp.abs() + 16), "log_prob")
+    within(got[0], want[0], 2 * s + 2.0 ** -22 * (lp.abs() + 16), "log_prob")
+    _, exact, size, _ = policy_oracle(z, actions, old, adv, 0.2, 0.1, 0.01, None, ref_z if ref == "logits" else None, None)
+    within(far[rows - few:], exact, 8 * s * size + half_step(exact, BF16), "dlogits")
+    _, exact, size, _ = preference_oracle(z, actions, near, None, 0.1, 0.0, None)
+    within(got[1], exact, (8 * s + 4 * 0.1 * few * (s + 2.0 ** -23 * 40)) * size + half_step(exact, BF16), "preference")
+    assert not far[:rows - few:977].any()
