@@ -31,7 +31,9 @@ class _LogitsLoss(torch.autograd.Function):
   @staticmethod
   def forward(ctx, logits, evaluate):
     terms, dlogits, ctx.again, inputs = evaluate(logits.detach())
-    ctx.save_for_backward(logits, *inputs)
+    ctx.save_for_backward(logits)
+    # (not saved as the logits are: what was made under inference_mode could not be)
+    ctx.inputs = [(t, None if t.is_inference() else t._version) for t in inputs]  # pylint: disable=protected-access
     ctx.dlogits = dlogits
     return terms[0].clone()
 
@@ -40,13 +42,15 @@ class _LogitsLoss(torch.autograd.Function):
     dlogits, ctx.dlogits = ctx.dlogits, None
     if dlogits is None:
       raise RuntimeError("the gradient of this loss was already handed on: evaluate the loss again to differentiate it again")
-    logits, *inputs = ctx.saved_tensors
+    (logits,), inputs, ctx.inputs = ctx.saved_tensors, ctx.inputs, None
     with torch.no_grad():
       factor = grad_output.to(torch.float32).contiguous()
       if dlogits.dtype == torch.float32:
         ops.scale_rows(dlogits, factor)
       else:
-        ctx.again(dlogits, factor, logits.detach(), *inputs)
+        if any(version is not None and t._version != version for t, version in inputs):  # pylint: disable=protected-access
+          raise RuntimeError("an input of this loss was modified by an inplace operation: its gradient is formed from it")
+        ctx.again(dlogits, factor, logits.detach(), *(t for t, _ in inputs))
     if torch.is_grad_enabled():
       dlogits = _NoSecondDerivative.apply(dlogits, logits)
     return dlogits, None

@@ -366,3 +366,22 @@ def test_rows_past_32_bits_in_every_row_kernel(rows, vocab, pitch, ref):
     _, exact, size, _ = preference_oracle(z, actions, near, None, 0.1, 0.0, None)
     within(got[1], exact, (8 * s + 4 * 0.1 * few * (s + 2.0 ** -23 * 40)) * size + half_step(exact, BF16), "preference")
     assert not far[:rows - few:977].any()
+
+
+def test_inputs_made_under_inference_mode():
+  """What a rollout stores may be inference tensors, which autograd cannot save."""
+  import derl_amd as derl
+  for dtype in (F32, F16):
+    z, actions, old, adv, _, ref_z = policy_inputs(6, 300, dtype, 1)
+    offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
+    with torch.inference_mode():
+      stored = [t.clone() for t in (actions, old, adv, ref_z)]
+    model = Table(z)
+    grads = []
+    for a, o, d, r in ((actions, old, adv, ref_z), stored):
+      model.logits.grad = None
+      policy = derl.TokenPolicyLoss(model, kl_coef=0.1)(dict(observations=None, actions=a, log_prob=o, advantages=d, ref_logits=r))
+      preference = derl.PreferenceLoss(model)(dict(observations=None, actions=a, offsets=offsets))
+      (8.0 * (policy + preference)).backward()
+      grads.append(model.logits.grad)
+    assert torch.equal(*grads)
