@@ -31,7 +31,10 @@ class _LogitsLoss(torch.autograd.Function):
   @staticmethod
   def forward(ctx, logits, evaluate):
     terms, dlogits, ctx.again, inputs = evaluate(logits.detach())
-    ctx.save_for_backward(logits)
+    if dlogits.dtype == torch.float32:  # scaled in place: the logits' values are not needed again, whatever becomes of them
+      ctx.logits = logits
+    else:
+      ctx.save_for_backward(logits)
     # (not saved as the logits are: what was made under inference_mode could not be)
     ctx.inputs = [(t, None if t.is_inference() else t._version) for t in inputs]  # pylint: disable=protected-access
     ctx.dlogits = dlogits
@@ -42,7 +45,8 @@ class _LogitsLoss(torch.autograd.Function):
     dlogits, ctx.dlogits = ctx.dlogits, None
     if dlogits is None:
       raise RuntimeError("the gradient of this loss was already handed on: evaluate the loss again to differentiate it again")
-    (logits,), inputs, ctx.inputs = ctx.saved_tensors, ctx.inputs, None
+    logits = ctx.logits if dlogits.dtype == torch.float32 else ctx.saved_tensors[0]
+    inputs, ctx.inputs, ctx.logits = ctx.inputs, None, None
     with torch.no_grad():
       factor = grad_output.to(torch.float32).contiguous()
       if dlogits.dtype == torch.float32:

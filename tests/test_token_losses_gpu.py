@@ -385,3 +385,22 @@ def test_inputs_made_under_inference_mode():
       (8.0 * (policy + preference)).backward()
       grads.append(model.logits.grad)
     assert torch.equal(*grads)
+
+
+def test_float32_logits_may_be_overwritten_behind_the_loss():
+  """Their gradient exists by then; 16-bit ones may be read again, and autograd says so."""
+  import derl_amd as derl
+  for dtype in (F32, BF16):
+    z, actions, old, adv, _, _ = policy_inputs(6, 300, dtype, 1)
+    model = Table(z)
+    data = dict(observations=None, actions=actions, log_prob=old, advantages=adv)
+    (want,) = torch.autograd.grad(3.0 * derl.TokenPolicyLoss(model)(data), model.logits)
+    loss = 3.0 * derl.TokenPolicyLoss(model)(data)
+    with torch.no_grad():
+      model.logits.mul_(0.5)
+    if dtype is F32:
+      (got,) = torch.autograd.grad(loss, model.logits)
+      assert torch.equal(got, want)
+    else:
+      with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
