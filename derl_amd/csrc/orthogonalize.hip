@@ -1051,7 +1051,7 @@ int launch_tile(NsArgs a, int batch, int splits, hipStream_t s) {
 // Tile side and parts of K for a product of `stages` stages, by the time that these constants give it (fitted to measured
 // products; us a stage of 128-byte lines).  A CU's copies bound the small tiles (28 bytes a cycle): a 64 or 128 tile costs 0.30
 // or 0.78 alone on a CU, 0.52 or 1.10 for two at a time (their ring lets two workgroups on a CU); 192 and 256 run alone, 1.2 and
-// 1.9 with the chip full, where the package's power bounds them.  Split parts exchange their sums: 8 us and 8 bytes a value.
+// 1.9 with the chip full (at 1.7 to 1.8 GHz, 2.4 in short products).  Split parts exchange their sums: 8 us and 8 bytes a value.
 // Measured, us a product (f32; * what the rule takes): 2001 x 5003 X X^T 64 121, 128 in two parts 112, in three 93 *; its update 64 171,
 // 128 153 *, 192 194, 256 158.  512 x 3136 X X^T 64 in one part 26, in seven 14 *, 128 in seven 32; its update 64 15 *, 128 23, 192 38,
 // 256 54.  4096 x 4096 X X^T 128 270, 192 201 *, 256 260; its update 128 400, 192 411, 256 364 *.  Over 14 shapes of 64 x 576 to
