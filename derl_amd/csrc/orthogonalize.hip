@@ -47,8 +47,8 @@ enum Epilogue { GRAM, POLY, UPDATE, FINAL };
 __host__ __device__ inline int power_above(float x) {
   if (!(x < 3.4e38f)) return 128;
   if (x == 0.f) return kLowest;
-  const int e = static_cast<int>(__builtin_bit_cast(uint32_t, x) >> 23);
-  return e - 126;
+  const float y = x < 1.18e-38f ? x * 0x1p64f : x;  // (a denormal number's exponent is not in its bits)
+  return static_cast<int>(__builtin_bit_cast(uint32_t, y) >> 23) - (x < 1.18e-38f ? 190 : 126);
 }
 // What is known of X before a step: its singular values are at most `top` < 2^cap, a row or column at most 2^shift times what it
 // was at the start; |b + c t| < 2^poly for their squares t.  2^E for a row that began below 2^e: E = min(e + shift, cap).
@@ -483,7 +483,8 @@ __device__ __forceinline__ Scale scale_of(double squares, float eps) {
   s.fraction = static_cast<float>(frexp(1.0 / (sqrt(squares) + eps), &s.power));
   return s;
 }
-__device__ __forceinline__ float scaled(float x, const Scale &s) { return times_power(x * s.fraction, s.power); }
+// (the power first: a denormal value's product with the fraction would lose what it has)
+__device__ __forceinline__ float scaled(float x, const Scale &s) { return times_power(x, s.power) * s.fraction; }
 // exponent of a bound of the norm of `count` scaled values of which none passes `most`
 __device__ __forceinline__ int start_bound(float most, int count, const Scale &s) {
   const int ceil_log2 = count <= 1 ? 0 : 32 - __builtin_clz(count - 1);
@@ -687,7 +688,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const PackArgs a) {
 // fp32 copies of X and A are in its registers (G too: it is read once).  What bounds it is the chain of 3 x steps dependent
 // products, not their rate.
 // LDS is addressed by plain offsets into one array: through pointers that are chosen at run time the compiler cannot see that
-// they are LDS, and flat accesses and spills made a step of 64 x 64 f32 3.9 us long (1.5 now).
+// they are LDS, and flat accesses and spills more than doubled a step.
 constexpr int kSmallWaves = 16;
 constexpr long long kSmallLds = 160 * 1024;
 

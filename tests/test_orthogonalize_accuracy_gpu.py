@@ -131,3 +131,13 @@ def test_memory_of_many_small_matrices():
   assert torch.cuda.max_memory_allocated() - before < 16e6
   for k in (0, 19999):
     assert torch.equal(out[k], ops.orthogonalize(g[k]))
+
+
+@pytest.mark.parametrize("m,n", [(20, 60), (60, 64), (130, 500), (500, 130)])
+def test_denormal_values(m, n):
+  """Entries below 2^-126, with what digits they have: a power of two times them, exactly, gives the same result."""
+  from derl_amd import ops
+  g = torch.randn(m, n, generator=gen(9), device=DEV) * 2.0 ** -100 * 2.0 ** -38
+  assert float(g.abs().max()) < 2.0 ** -126
+  want = ops.orthogonalize(g * 2.0 ** 100, eps=0.0)
+  assert float((ops.orthogonalize(g, eps=0.0) - want).abs().max()) <= 2.0 ** -18
