@@ -141,3 +141,44 @@ def test_denormal_values(m, n):
   assert float(g.abs().max()) < 2.0 ** -126
   want = ops.orthogonalize(g * 2.0 ** 100, eps=0.0)
   assert float((ops.orthogonalize(g, eps=0.0) - want).abs().max()) <= 2.0 ** -18
+
+
+def matrix_of(kind, m, n):
+  g = torch.randn(m, n, generator=gen(m + 3 * n), device=DEV)
+  k = min(m, n)
+  if kind == "low rank":
+    return g[:, :3].mm(g[:3]) + 1e-3 * g
+  if kind == "rank one":
+    return torch.ones(m, n, device=DEV)
+  if kind == "one large row":
+    g[1] *= 1e4
+    return g
+  if kind == "orthogonal":
+    q = torch.linalg.qr(g if m >= n else g.t())[0]
+    return (q if m >= n else q.t()).contiguous()
+  if kind == "sparse":
+    return torch.where(torch.rand(m, n, generator=gen(2), device=DEV) < 0.02, g, 0.0)
+  g = torch.zeros(m, n, device=DEV)
+  if kind == "diagonal":
+    g[torch.arange(k), torch.arange(k)] = torch.logspace(0, -6, k, device=DEV)
+  elif kind == "blocks":
+    g[:m // 2, :n // 3] = 1e-5 * torch.randn(m // 2, n // 3, generator=gen(4), device=DEV)
+    g[m // 2:, n // 3:] = torch.randn(m - m // 2, n - n // 3, generator=gen(5), device=DEV)
+  return g
+
+
+@pytest.mark.parametrize("kind", ["low rank", "rank one", "one large row", "orthogonal", "sparse", "diagonal", "blocks"])
+@pytest.mark.parametrize("m,n", [(20, 33), (64, 64), (60, 200), (96, 90), (130, 300), (513, 200), (700, 1500)])
+def test_matrices_that_are_not_gaussian(m, n, kind):
+  """Each step's rounding, ``unit`` / 5 of X's norm, passed on by the polynomial's slope, 4 at most (its derivative
+  a + 3 b s^2 + 5 c s^4 has its extremes 3.44, -1.61 and 3.97 on [0, 1.2024], where a step leaves every singular value); all three types against the same iteration, and zeros stay zeros."""
+  from derl_amd import ops
+  for dtype in (F32, BF16, F16):
+    g = matrix_of(kind, m, n).to(dtype)
+    want, norms = newton_schulz64(g, 5)
+    got = ops.orthogonalize(g)
+    d = unit(max(m, n)) / 5 * sum(4.0 ** (4 - k) * norm for k, norm in enumerate(norms[:5]))
+    off = (got.double() - want).abs()
+    assert float(off.norm()) <= float((want.to(dtype).double() - want).norm()) + 2 * d, (dtype, float(off.norm()), d)
+    if kind in ("diagonal", "blocks"):
+      assert not got[g.any(1).logical_not()].any()
